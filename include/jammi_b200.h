@@ -240,6 +240,26 @@ jb_status jb_op_quantize_rows_act(const void* x, int x_dtype, int activation, in
 jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamma,
                           const float* beta, void* y, int dtype, int rows, int cols,
                           float eps, void* stream);
+/* RMS norm over the last dim with the residual's addition: s = x (+ residual)
+ * in f32, y = s * rsqrt(mean(s^2) + eps) * gamma.  `sum` (NULL unless a
+ * residual is given; NULL: not wanted) receives s rounded to dtype, the next
+ * layer's residual stream.  Exactly one output form:
+ *   y [rows, cols] (dtype), with q and scale NULL; or
+ *   q int8 [rows, cols] and scale f32 [rows], with y NULL: per-row symmetric
+ *   int8 of the unrounded y, as jb_op_quantize_rows defines it (the operands
+ *   of jb_op_linear_s8).  A row whose y holds a NaN or an infinity has scale
+ *   NaN and q 0.
+ * dtype F32, BF16 or F16; gamma f32 [cols]; any cols >= 1 (cols that are a
+ * multiple of 16 bytes, up to 2048 16-byte vectors, with 16-byte aligned
+ * buffers take the vectorised kernels).  sum and y may replace x or residual.
+ * No counterpart in the reference (its encoders use LayerNorm). */
+jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma, void* sum,
+                        void* y, int8_t* q, float* scale, int dtype, int rows, int cols,
+                        float eps, void* stream);
+/* y[r, c] = q[r, c] * scale[r] rounded to dtype (F32, BF16 or F16): the values
+ * that the rows of jb_op_quantize_rows or jb_op_rmsnorm stand for. */
+jb_status jb_op_dequantize_rows(const int8_t* q, const float* scale, void* y, int dtype,
+                                int rows, int cols, void* stream);
 /* Variable-length self-attention over packed rows: qkv [T, 3*heads*d] (Q|K|V
  * column blocks, head-major inside each), cu_seqlens [batch+1] (int32),
  * ctx [T, heads*d].  softmax(Q K^T / sqrt(d)) V per (row, head) over the row's

@@ -554,6 +554,46 @@ jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamm
   });
 }
 
+jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma, void* sum, void* y,
+                        int8_t* q, float* scale, int dtype, int rows, int cols, float eps, void* stream) {
+  return guarded([&] {
+    if (rows < 0 || cols <= 0) jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: rows must be >= 0 and cols > 0");
+    if (dtype != JB_DT_F32 && dtype != JB_DT_BF16 && dtype != JB_DT_F16)
+      jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: dtype must be f32, bf16 or f16");
+    if ((y != nullptr) == (q != nullptr) || (q != nullptr) != (scale != nullptr))
+      jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: give either y, or q and scale");
+    if (sum && !residual) jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: sum without a residual");
+    if (!(eps >= 0.f)) jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: eps must be >= 0");
+    if (rows == 0) return;
+    if (!x || !gamma) jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: null buffer");
+    jb::RmsArgs a;
+    a.x = x;
+    a.resid = residual;
+    a.gamma = gamma;
+    a.sum = sum;
+    a.y = y;
+    a.q = q;
+    a.scale = scale;
+    a.rows = rows;
+    a.cols = cols;
+    a.eps = eps;
+    jb::check_cuda(jb::launch_rmsnorm(a, dtype, as_stream(stream)), "jb_op_rmsnorm");
+  });
+}
+
+jb_status jb_op_dequantize_rows(const int8_t* q, const float* scale, void* y, int dtype, int rows, int cols,
+                                void* stream) {
+  return guarded([&] {
+    if (rows < 0 || cols <= 0) jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: rows must be >= 0 and cols > 0");
+    if (dtype != JB_DT_F32 && dtype != JB_DT_BF16 && dtype != JB_DT_F16)
+      jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: dtype must be f32, bf16 or f16");
+    if (rows == 0) return;
+    if (!q || !scale || !y) jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: null buffer");
+    jb::check_cuda(jb::launch_dequantize_rows(q, scale, y, dtype, rows, cols, as_stream(stream)),
+                   "jb_op_dequantize_rows");
+  });
+}
+
 namespace {
 jb_status op_attention(const void* qkv, const int* cu_seqlens, void* ctx, int dtype, int batch,
                        int heads, int head_dim, int max_len, int causal, void* stream,

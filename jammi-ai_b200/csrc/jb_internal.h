@@ -61,6 +61,24 @@ struct LnArgs {
 };
 cudaError_t launch_layernorm(const LnArgs& a, cudaStream_t s);
 
+// RMS norm (jb_rmsnorm.cu): s = x (+ resid); sum = round(s) when both are
+// given; y, or q and scale, from the unrounded s.  Exactly one of y and q.
+struct RmsArgs {
+  const void* x = nullptr;
+  const void* resid = nullptr;
+  const float* gamma = nullptr;
+  void* sum = nullptr;
+  void* y = nullptr;
+  int8_t* q = nullptr;
+  float* scale = nullptr;
+  int rows = 0;
+  int cols = 0;
+  float eps = 0.f;
+};
+cudaError_t launch_rmsnorm(const RmsArgs& a, int dtype, cudaStream_t s);
+cudaError_t launch_dequantize_rows(const int8_t* q, const float* scale, void* y, int dtype, int rows, int cols,
+                                   cudaStream_t s);
+
 // Tabulates the bf16 GELU on the current device (once; later calls return at
 // once).  The first int8 BERT forward or GELU quantisation on a device needs
 // it: model loading calls it so that no forward (or graph capture) does.

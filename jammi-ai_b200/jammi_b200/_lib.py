@@ -85,6 +85,8 @@ _SIGS = [
     ("jb_op_quantize_rows", _I, [_P, _I, _P, _P, _I, _I, _P]),
     ("jb_op_quantize_rows_act", _I, [_P, _I, _I, _P, _P, _I, _I, _P]),
     ("jb_op_layernorm", _I, [_P, _P, _P, _P, _P, _I, _I, _I, ctypes.c_float, _P]),
+    ("jb_op_rmsnorm", _I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, ctypes.c_float, _P]),
+    ("jb_op_dequantize_rows", _I, [_P, _P, _P, _I, _I, _I, _P]),
     ("jb_op_attention", _I, [_P, _P, _P, _I, _I, _I, _I, _I, _P]),
     ("jb_op_attention_causal", _I, [_P, _P, _P, _I, _I, _I, _I, _I, _P]),
     ("jb_op_attention_rows", _I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),

@@ -84,6 +84,89 @@ def layernorm(x: torch.Tensor, gamma, beta, eps: float, residual=None) -> torch.
     return y
 
 
+def _check(name, t, shape=None, dtypes=None, device=None, optional=False):
+    """Raises ValueError unless ``t`` is a contiguous CUDA tensor of ``shape`` and one of
+    ``dtypes`` on ``device``."""
+    if t is None:
+        if optional:
+            return
+        raise ValueError(f"{name} is missing")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name} must be on {device or 'a CUDA device'}, not on {t.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise ValueError(f"{name}: {t.dtype} is not one of {', '.join(map(str, dtypes))}")
+
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_F32 = (torch.float32,)
+
+
+def _call(fn, device, *args):
+    """One library call on ``device`` and its current torch stream."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+
+
+def _rms_args(x, gamma, residual):
+    if x.dim() != 2:
+        raise ValueError("x must be [rows, cols]")
+    dev = x.device
+    _check("x", x, None, _FLOATS)
+    _check("gamma", gamma, x.shape[1:], _F32, dev)
+    _check("residual", residual, x.shape, (x.dtype,), dev, optional=True)
+
+
+def rmsnorm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=None):
+    """RMS norm of ``x`` [R, C] (+ ``residual``): ``s * rsqrt(mean(s^2) + eps) * gamma`` with
+    ``s = x + residual`` in f32.  Returns y, or (y, s rounded to x's dtype) when a residual is
+    given.  x f32, bf16 or f16; gamma f32 [C]."""
+    _rms_args(x, gamma, residual)
+    R, C = x.shape
+    y = torch.empty_like(x)
+    h = None if residual is None else torch.empty_like(x)
+    if R:
+        _call(lib().jb_op_rmsnorm, x.device, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), y.data_ptr(),
+              None, None, _DT[x.dtype], R, C, eps)
+    return y if h is None else (y, h)
+
+
+def rmsnorm_quantize(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=None):
+    """``rmsnorm`` with its output as per-row int8: (q int8 [R, C], scale f32 [R]) -- the
+    activations of ``linear_s8`` -- and the rounded sum as a third value when a residual is given.
+    The unrounded f32 norm is quantised; a row that is not finite has scale NaN and q 0."""
+    _rms_args(x, gamma, residual)
+    R, C = x.shape
+    q = torch.empty((R, C), dtype=torch.int8, device=x.device)
+    scale = torch.empty((R,), dtype=torch.float32, device=x.device)
+    h = None if residual is None else torch.empty_like(x)
+    if R:
+        _call(lib().jb_op_rmsnorm, x.device, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), None,
+              q.data_ptr(), scale.data_ptr(), _DT[x.dtype], R, C, eps)
+    return (q, scale) if h is None else (q, scale, h)
+
+
+def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values that int8 rows stand for: ``q[r, c] * scale[r]`` in ``dtype`` (f32, bf16, f16)."""
+    _check("q", q, None, (torch.int8,))
+    if q.dim() != 2:
+        raise ValueError("q must be [rows, cols]")
+    _check("scale", scale, q.shape[:1], _F32, q.device)
+    if dtype not in _FLOATS:
+        raise ValueError(f"{dtype} is not one of {', '.join(map(str, _FLOATS))}")
+    y = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if q.shape[0]:
+        _call(lib().jb_op_dequantize_rows, q.device, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype],
+              q.shape[0], q.shape[1])
+    return y
+
+
 def attention(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, max_len: int,
               causal: bool = False, tma: bool = False) -> torch.Tensor:
     """qkv [T, 3*heads*d] packed rows, cu_seqlens int32 [B+1] -> ctx [T, heads*d]
