@@ -260,6 +260,33 @@ jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma,
  * that the rows of jb_op_quantize_rows or jb_op_rmsnorm stand for. */
 jb_status jb_op_dequantize_rows(const int8_t* q, const float* scale, void* y, int dtype,
                                 int rows, int cols, void* stream);
+/* MXFP4 rows: the OCP Microscaling v1.0 4-bit format.  Every 32 consecutive
+ * elements of a row share the scale 2^E, E = floor(log2(max |x|)) - 2 clamped
+ * to [-127, 127]; an element is the e2m1 value {0, .5, 1, 1.5, 2, 3, 4, 6}
+ * nearest to x 2^-E (ties to the even code, saturated at 6) and its sign.  A
+ * block with a NaN or an infinity has the NaN scale and codes 0.
+ *   q [rows, cols / 2]: two codes per byte, the even column in the low half;
+ *   scale [jb_mxfp4_scale_bytes(rows, cols)]: E + 127 (255: NaN) in tiles of
+ *     128 rows x 128 columns, [ceil(rows / 128)][ceil(cols / 128)][512], row r
+ *     and block b of a tile at (r % 32) * 16 + (r / 32) * 4 + b -- the order
+ *     the tensor core reads.  Padding rows and blocks are 0.
+ * cols is a multiple of 32; x, q and scale are 16-byte aligned; x F32, BF16
+ * or F16. No counterpart in the reference. */
+size_t jb_mxfp4_scale_bytes(int rows, int cols);
+jb_status jb_op_quantize_mxfp4(const void* x, int x_dtype, uint8_t* q, uint8_t* scale, int rows,
+                               int cols, void* stream);
+/* y [rows, cols] (F32, BF16 or F16) = the values that MXFP4 rows stand for. */
+jb_status jb_op_dequantize_mxfp4(const uint8_t* q, const uint8_t* scale, void* y, int y_dtype,
+                                 int rows, int cols, void* stream);
+/* MXFP4 Linear: C[M,N] = epi(A[M,K] . W[N,K]^T + bias[N]) with A and W as
+ * jb_op_quantize_mxfp4 stores them (tcgen05 kind::mxf4 with block scales, f32
+ * accumulators).  c_dtype F32, BF16 or F16; residual has c's dtype; bias f32
+ * or NULL.  K is a multiple of 32, N of 8; every buffer is 16-byte aligned.
+ * C may replace the residual.  A row with a NaN scale gives NaN outputs. */
+jb_status jb_op_linear_mxfp4(const uint8_t* Aq, const uint8_t* a_scale, const uint8_t* Wq,
+                             const uint8_t* w_scale, const float* bias, const void* residual,
+                             void* C, int c_dtype, int M, int N, int K, int epilogue,
+                             void* stream);
 /* Variable-length self-attention over packed rows: qkv [T, 3*heads*d] (Q|K|V
  * column blocks, head-major inside each), cu_seqlens [batch+1] (int32),
  * ctx [T, heads*d].  softmax(Q K^T / sqrt(d)) V per (row, head) over the row's

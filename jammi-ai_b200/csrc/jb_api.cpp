@@ -595,6 +595,85 @@ jb_status jb_op_dequantize_rows(const int8_t* q, const float* scale, void* y, in
 }
 
 namespace {
+bool is_float_dtype(int dtype) { return dtype == JB_DT_F32 || dtype == JB_DT_BF16 || dtype == JB_DT_F16; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+void check_mxfp4_rows(const char* op, const void* x, int dtype, const void* q, const void* scale, int rows,
+                      int cols) {
+  const std::string name = op;
+  if (rows < 0 || cols <= 0 || cols % 32)
+    jb::fail(JB_ERR_INVALID, name + ": rows must be >= 0 and cols a positive multiple of 32");
+  if (!is_float_dtype(dtype)) jb::fail(JB_ERR_INVALID, name + ": dtype must be f32, bf16 or f16");
+  if (rows == 0) return;
+  if (!x || !q || !scale) jb::fail(JB_ERR_INVALID, name + ": null buffer");
+  if (!aligned16(x) || !aligned16(q) || !aligned16(scale))
+    jb::fail(JB_ERR_INVALID, name + ": buffers must be 16-byte aligned");
+}
+}  // namespace
+
+size_t jb_mxfp4_scale_bytes(int rows, int cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return (static_cast<size_t>(rows) + 127) / 128 * ((static_cast<size_t>(cols) + 127) / 128) * 512;
+}
+
+jb_status jb_op_quantize_mxfp4(const void* x, int x_dtype, uint8_t* q, uint8_t* scale, int rows, int cols,
+                               void* stream) {
+  return guarded([&] {
+    check_mxfp4_rows("jb_op_quantize_mxfp4", x, x_dtype, q, scale, rows, cols);
+    jb::check_cuda(jb::launch_quantize_mxfp4(x, x_dtype, q, scale, rows, cols, as_stream(stream)),
+                   "jb_op_quantize_mxfp4");
+  });
+}
+
+jb_status jb_op_dequantize_mxfp4(const uint8_t* q, const uint8_t* scale, void* y, int y_dtype, int rows, int cols,
+                                 void* stream) {
+  return guarded([&] {
+    check_mxfp4_rows("jb_op_dequantize_mxfp4", y, y_dtype, q, scale, rows, cols);
+    jb::check_cuda(jb::launch_dequantize_mxfp4(q, scale, y, y_dtype, rows, cols, as_stream(stream)),
+                   "jb_op_dequantize_mxfp4");
+  });
+}
+
+jb_status jb_op_linear_mxfp4(const uint8_t* Aq, const uint8_t* a_scale, const uint8_t* Wq, const uint8_t* w_scale,
+                             const float* bias, const void* residual, void* C, int c_dtype, int M, int N, int K,
+                             int epilogue, void* stream) {
+  return guarded([&] {
+    if (!is_float_dtype(c_dtype)) jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: C must be f32, bf16 or f16");
+    if (epilogue < JB_EPI_NONE || epilogue > JB_EPI_RESIDUAL) jb::fail(JB_ERR_INVALID, "unknown epilogue");
+    if (M < 0 || N <= 0 || K <= 0 || K % 32 || N % 8)
+      jb::fail(JB_ERR_INVALID,
+               "jb_op_linear_mxfp4: M must be >= 0, N a positive multiple of 8, K a positive multiple of 32");
+    if ((epilogue == JB_EPI_RESIDUAL) != (residual != nullptr) && M > 0)
+      jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: a residual and JB_EPI_RESIDUAL go together");
+    if (M == 0) return;
+    if (!Aq || !a_scale || !Wq || !w_scale || !C) jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: null buffer");
+    if (!aligned16(Aq) || !aligned16(a_scale) || !aligned16(Wq) || !aligned16(w_scale) || !aligned16(C) ||
+        !aligned16(residual))
+      jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: buffers must be 16-byte aligned");
+    jb::MxGemmArgs g;
+    g.aq = Aq;
+    g.a_scale = a_scale;
+    g.wq = Wq;
+    g.w_scale = w_scale;
+    g.bias = bias;
+    g.resid = residual;
+    g.C = C;
+    g.c_dtype = c_dtype;
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.epi = epilogue;
+    g.err = op_flag(current_device());
+    std::string why;
+    cudaError_t e = jb::launch_linear_mxfp4(g, as_stream(stream), &why);
+    if (e != cudaSuccess) {
+      if (!why.empty()) jb::fail(JB_ERR_INVALID, why);
+      jb::check_cuda(e, "jb_op_linear_mxfp4");
+    }
+  });
+}
+
+namespace {
 jb_status op_attention(const void* qkv, const int* cu_seqlens, void* ctx, int dtype, int batch,
                        int heads, int head_dim, int max_len, int causal, void* stream,
                        int rows = 0) {

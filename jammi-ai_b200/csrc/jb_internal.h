@@ -79,6 +79,27 @@ cudaError_t launch_rmsnorm(const RmsArgs& a, int dtype, cudaStream_t s);
 cudaError_t launch_dequantize_rows(const int8_t* q, const float* scale, void* y, int dtype, int rows, int cols,
                                    cudaStream_t s);
 
+// MXFP4 rows (jb_mxfp4.cu) and their linear layer (jb_mxfp4_gemm.cu); cols
+// and K are multiples of 32, buffers 16-byte aligned.
+cudaError_t launch_quantize_mxfp4(const void* x, int dtype, uint8_t* q, uint8_t* scale, int rows, int cols,
+                                  cudaStream_t s);
+cudaError_t launch_dequantize_mxfp4(const uint8_t* q, const uint8_t* scale, void* y, int dtype, int rows, int cols,
+                                    cudaStream_t s);
+struct MxGemmArgs {
+  const uint8_t* aq = nullptr;
+  const uint8_t* a_scale = nullptr;
+  const uint8_t* wq = nullptr;
+  const uint8_t* w_scale = nullptr;
+  const float* bias = nullptr;
+  const void* resid = nullptr;  // c_dtype
+  void* C = nullptr;
+  int c_dtype = JB_DT_BF16;
+  int M = 0, N = 0, K = 0;
+  int epi = JB_EPI_NONE;
+  int* err = nullptr;  // device flag set when a bounded wait gives up
+};
+cudaError_t launch_linear_mxfp4(const MxGemmArgs& g, cudaStream_t s, std::string* why);
+
 // Tabulates the bf16 GELU on the current device (once; later calls return at
 // once).  The first int8 BERT forward or GELU quantisation on a device needs
 // it: model loading calls it so that no forward (or graph capture) does.

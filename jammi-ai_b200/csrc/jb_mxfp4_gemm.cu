@@ -1,0 +1,535 @@
+// MXFP4 linear layers: C = epi(A . W^T + bias), A and W in the 4-bit rows and
+// scale tiles of jb_mxfp4.cu.
+//
+//   acc[m, n] = sum over blocks b of 32 columns of
+//               2^(Ea[m, b] + Ew[n, b]) * sum over k in b of a[m, k] w[n, k]
+//
+// on tcgen05.mma kind::mxf4 with block scales (one UE8M0 byte per 32
+// elements, scale_vec::2X): the tensor core multiplies the scales in, exact
+// products accumulated in f32 in TMEM, four times the bf16 rate.
+//
+// One persistent CTA per SM, output tiles of 128 x BN, K in stages of 256
+// elements (one 128-byte swizzled row of codes):
+//   warp 0     TMA producer: codes of A and W by tiled copies, their scale
+//              tiles (contiguous by construction) by plain bulk copies
+//   warp 1     TMEM allocator and single-thread MMA issuer: per stage the
+//              scale tiles go from shared memory to TMEM (tcgen05.cp
+//              32x128b.warpx4: 128 rows x 4 blocks into 4 columns), then four
+//              K = 64 products.  Each stage has its own TMEM columns for the
+//              scales, so a copy never meets a product that still reads them:
+//              the stage's shared memory, and with it its TMEM columns, comes
+//              back only after the commit of its products.
+//   warps 2..  epilogue, one warp per 32 rows x 64 columns of the tile: the
+//              accumulators go to registers at once (tcgen05.ld) and are
+//              released before any arithmetic; bias, activation and residual
+//              (a TMA-loaded box, issued before the wait for the
+//              accumulators) in f32, one rounding, one TMA store of the box.
+// The accumulator is double-buffered (2 x BN columns).
+//
+// BN = 192: the widest tile whose two accumulators leave TMEM columns for the
+// scales (384 + 4 stages x 24).  Its odd tiles start 64 rows into a scale
+// tile of W: the scale address of the product starts two columns (2 x 32
+// rows) later.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <mutex>
+
+#include "jb_common.cuh"
+#include "jb_internal.h"
+
+namespace jb {
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kStageK = 256;       // elements of K per stage: 128 bytes of codes
+constexpr int kUnitCols = 64;      // columns of an epilogue warp
+constexpr int kUnitBytes = 4096;   // its box: 32 rows of 128 bytes (64 16-bit or 32 f32 columns)
+constexpr int kSfTile = 512;       // scale bytes of 128 rows x 128 columns
+
+template <int BN>
+struct MxCfg {
+  static constexpr int A_BYTES = kBM * 128;
+  static constexpr int B_BYTES = BN * 128;
+  // 128-row scale tiles that BN rows of W may touch (tiles start at multiples of BN)
+  static constexpr int SFB_TILES = BN > 128 ? 2 : 1;
+  static constexpr int SF_BYTES = 2 * kSfTile * (1 + SFB_TILES);
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SF_BYTES;
+  static constexpr int STAGES = BN == 192 ? 4 : BN == 128 ? 5 : 6;
+  static constexpr int SF_COLS = 8 * (1 + SFB_TILES);  // TMEM columns of a stage's scales
+  static constexpr int TMEM_COLS = BN == 64 ? 256 : 512;
+  static_assert(2 * BN + STAGES * SF_COLS <= TMEM_COLS, "TMEM columns");
+  static constexpr int EPI_WARPS = 4 * (BN / kUnitCols);
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int BARS = 2 * STAGES + 4 + 1 + EPI_WARPS;
+  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * (kUnitBytes + kUnitCols * 4) + 8 * BARS + 16;
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+struct MxParams {
+  const uint8_t* a_scale;
+  const uint8_t* w_scale;
+  const float* bias;
+  int M, N, K;
+  int epi;
+  int h16;  // 16-bit output and residual are f16 (else bf16)
+  int* err;
+};
+
+// D[tmem] (+)= A . B^T over K = 64 e2m1 elements, each block of 32 scaled by
+// the UE8M0 bytes at sfa / sfb.
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 32 rows of 16 contiguous bytes -> 4 TMEM columns of lanes 0-31, repeated in
+// the other three lane quarters.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Untiled bulk copy, 16-byte aligned, a multiple of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+      : "memory");
+}
+// Descriptor of a scale tile: 8-row groups of 16-byte rows, 128 bytes apart,
+// no swizzle.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(128 >> 4) << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+// kind::mxf4, dense, K-major: A and B e2m1 (1), UE8M0 scales (bit 23), N >> 3
+// at 17, M >> 7 at 27; sf = the byte of the scale column that the product's
+// first block uses (0 or 2), for A at 29 and B at 4.
+constexpr uint32_t mx_idesc(int M, int N, uint32_t sf) {
+  return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(M >> 7) << 27) | (sf << 29);
+}
+
+// 16-byte slot `q` of row `row` of a 128-byte-swizzled box.
+__device__ __forceinline__ uint32_t box_slot(uint32_t buf, int row, int q) {
+  return buf + row * 128 + ((q ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool h16) {
+  if (h16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, bool h16) {
+  if (h16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+// Same outcome for every lane, so that no warp-collective instruction after
+// it is reached by part of the warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+}
+
+// 32 accumulators -> f32 outputs before the residual.
+template <int EPI>
+__device__ __forceinline__ void finish32(const uint32_t (&r)[32], uint32_t bias, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const uint4 b = lds128(bias + 4 * j);
+    float2 lo = __fadd2_rn(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                           make_float2(__uint_as_float(b.x), __uint_as_float(b.y)));
+    float2 hi = __fadd2_rn(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])),
+                           make_float2(__uint_as_float(b.z), __uint_as_float(b.w)));
+    if constexpr (EPI == JB_EPI_GELU) {
+      lo = gelu_tc2(lo);
+      hi = gelu_tc2(hi);
+    } else if constexpr (EPI == JB_EPI_QUICK_GELU) {
+      lo = make_float2(quick_gelu_tc(lo.x), quick_gelu_tc(lo.y));
+      hi = make_float2(quick_gelu_tc(hi.x), quick_gelu_tc(hi.y));
+    }
+    v[j] = lo.x; v[j + 1] = lo.y; v[j + 2] = hi.x; v[j + 3] = hi.y;
+  }
+}
+
+// F32: the output (and residual) is f32, else 16-bit.
+template <int BN, int EPI, bool F32>
+__global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
+    gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                      const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
+                      const MxParams p) {
+  using Cfg = MxCfg<BN>;
+  constexpr bool kRes = EPI == JB_EPI_RESIDUAL;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  // [stages][A | B] | [epilogue boxes] | [stages][scales A | scales B] |
+  // [epilogue biases] | barriers | tmem slot | abort flag
+  const uint32_t boxes = base + Cfg::STAGES * (Cfg::A_BYTES + Cfg::B_BYTES);
+  const uint32_t scales = boxes + Cfg::EPI_WARPS * kUnitBytes;
+  const uint32_t biases = scales + Cfg::STAGES * Cfg::SF_BYTES;
+  const uint32_t bars = biases + Cfg::EPI_WARPS * kUnitCols * 4;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (Cfg::STAGES + s); };
+  auto tfull_bar = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + i); };
+  auto tempty_bar = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + 2 + i); };
+  const uint32_t spare = bars + 8u * (2 * Cfg::STAGES + 4);
+  auto res_bar = [&](int w) { return bars + 8u * (2 * Cfg::STAGES + 5 + w); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + (bars - base) + 8 * Cfg::BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_tiles = (p.N + BN - 1) / BN;
+  const int total = (p.M + kBM - 1) / kBM * n_tiles;
+  const int kb_count = (p.K + kStageK - 1) / kStageK;
+  const int k_tiles = (p.K + 127) / 128;  // scale tiles along K
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(tfull_bar(i), 1);
+      mbar_init(tempty_bar(i), Cfg::EPI_WARPS);
+    }
+    mbar_init(spare, 1);
+    for (int w = 0; w < Cfg::EPI_WARPS; ++w) mbar_init(res_bar(w), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&tmA);
+    prefetch_tensormap(&tmB);
+    prefetch_tensormap(&tmC);
+    if (kRes) prefetch_tensormap(&tmR);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {  // ── producer
+      const int w_tiles = (p.N + 127) / 128;  // scale tiles along N
+      int it = 0;  // stages filled
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const int mb = t / n_tiles, nb = t % n_tiles;
+        const int wt = nb * BN / 128;
+        for (int kb = 0; kb < kb_count; ++kb, ++it) {
+          const int st = it % Cfg::STAGES;
+          if (!mbar_wait(empty_bar(st), ((it / Cfg::STAGES) & 1) ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
+          const uint32_t sf = scales + st * Cfg::SF_BYTES;
+          const uint32_t sf_bytes = min(2, k_tiles - 2 * kb) * kSfTile;
+          const int w_copies = min(Cfg::SFB_TILES, w_tiles - wt);
+          mbar_arrive_expect_tx(full_bar(st), Cfg::A_BYTES + Cfg::B_BYTES + sf_bytes * (1 + w_copies));
+          tma_load_2d(sa, &tmA, kb * 128, mb * kBM, full_bar(st));
+          tma_load_2d(sa + Cfg::A_BYTES, &tmB, kb * 128, nb * BN, full_bar(st));
+          bulk_load(sf, p.a_scale + (static_cast<size_t>(mb) * k_tiles + 2 * kb) * kSfTile, sf_bytes, full_bar(st));
+          for (int i = 0; i < w_copies; ++i)
+            bulk_load(sf + 2 * kSfTile * (1 + i),
+                      p.w_scale + (static_cast<size_t>(wt + i) * k_tiles + 2 * kb) * kSfTile, sf_bytes, full_bar(st));
+        }
+      }
+      if (!ok || *abort_flag) {  // copies in flight land before the CTA leaves (bounded)
+        volatile int no_abort = 0;
+        for (int b = max(0, it - Cfg::STAGES); b < it; ++b)
+          mbar_wait(full_bar(b % Cfg::STAGES), (b / Cfg::STAGES) & 1, &no_abort);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {  // ── MMA issuer
+      int it = 0, acc = 0;
+      uint32_t acc_ph = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const uint32_t sf_shift = static_cast<uint32_t>((t % n_tiles) * BN % 128) / 32;
+        if (!mbar_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        for (int kb = 0; kb < kb_count; ++kb, ++it) {
+          const int st = it % Cfg::STAGES;
+          if (!mbar_wait(full_bar(st), (it / Cfg::STAGES) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
+          const uint32_t sf = scales + st * Cfg::SF_BYTES;
+          const uint32_t tsa = tmem_base + 2 * BN + st * Cfg::SF_COLS;  // [2 K tiles][4]
+          const uint32_t tsb = tsa + 8;                                 // [2 K tiles][SFB_TILES][4]
+          const int k_left = p.K - kb * kStageK;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (c * 128 < k_left) {
+              tmem_cp_scales(tsa + 4 * c, scale_desc(sf + c * kSfTile));
+#pragma unroll
+              for (int i = 0; i < Cfg::SFB_TILES; ++i)
+                tmem_cp_scales(tsb + 4 * (c * Cfg::SFB_TILES + i), scale_desc(sf + (2 * (1 + i) + c) * kSfTile));
+            }
+          }
+          const uint64_t da = umma_desc_sw128(sa), db = umma_desc_sw128(sa + Cfg::A_BYTES);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k * 64 < k_left)
+              mma_mxf4(d_tmem, da + 2u * k, db + 2u * k, mx_idesc(kBM, BN, 2 * (k & 1)), tsa + 4 * (k >> 1),
+                       tsb + 4 * Cfg::SFB_TILES * (k >> 1) + sf_shift, (kb | k) != 0);
+          }
+          mma_commit(empty_bar(st));
+        }
+        if (!ok) break;
+        mma_commit(tfull_bar(acc));
+        acc ^= 1;
+        if (acc == 0) acc_ph ^= 1u;
+      }
+      if (!ok) {  // every MMA issued completes before TMEM is freed (bounded)
+        volatile int no_abort = 0;
+        mma_commit(spare);
+        mbar_wait(spare, 0, &no_abort);
+      }
+    }
+  } else {  // ── epilogue
+    const int w = warp - 2;
+    const int quarter = warp & 3, part = w >> 2;  // warps 2..5, 6..9, ...: each quarter once
+    const uint32_t box = boxes + static_cast<uint32_t>(w) * kUnitBytes;
+    const uint32_t bias = biases + static_cast<uint32_t>(w) * kUnitCols * 4;
+    auto bias_at = [&](int t, int c) {
+      const int col = (t % n_tiles) * BN + part * kUnitCols + c;
+      return p.bias && col < p.N ? __ldg(p.bias + col) : 0.f;
+    };
+    float b0 = 0.f, b1 = 0.f;
+    if (static_cast<int>(blockIdx.x) < total) {
+      b0 = bias_at(blockIdx.x, lane);
+      b1 = bias_at(blockIdx.x, 32 + lane);
+    }
+    int acc = 0, loads = 0, waited = 0;  // residual boxes issued / seen
+    uint32_t acc_ph = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      const int row0 = t / n_tiles * kBM + quarter * 32;
+      const int col0 = (t % n_tiles) * BN + part * kUnitCols;
+      const bool live = col0 < p.N && row0 < p.M;  // warp-uniform
+      auto load_res = [&](int c) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(res_bar(w), kUnitBytes);
+          tma_load_2d(box, &tmR, col0 + c, row0, res_bar(w));
+        }
+        ++loads;
+      };
+      if (lane == 0) bulk_wait_read_all();  // the box's last store has read it
+      __syncwarp();
+      if (kRes && live) load_res(0);
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(bias + 4 * lane), "f"(b0) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(bias + 4 * (32 + lane)), "f"(b1) : "memory");
+      if (t + static_cast<int>(gridDim.x) < total) {
+        b0 = bias_at(t + gridDim.x, lane);
+        b1 = bias_at(t + gridDim.x, 32 + lane);
+      }
+      __syncwarp();
+      if (!warp_wait(tfull_bar(acc), acc_ph, abort_flag)) break;
+      tc_fence_after();
+      uint32_t r[2][32];
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                             static_cast<uint32_t>(acc * BN + part * kUnitCols);
+      tmem_ld_32x32b_x32(taddr, r[0]);
+      tmem_ld_32x32b_x32(taddr + 32, r[1]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty_bar(acc));
+      acc ^= 1;
+      if (acc == 0) acc_ph ^= 1u;
+      if (!live) continue;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float v[32];
+        finish32<EPI>(r[half], bias + 128 * half, v);
+        if (F32 && half == 1) {  // the second 32 columns use the box again
+          if (col0 + 32 >= p.N) break;
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
+          if (kRes) load_res(32);
+        }
+        if (kRes && (F32 || half == 0)) {
+          if (!warp_wait(res_bar(w), waited & 1, abort_flag)) break;
+          ++waited;
+        }
+        constexpr int kSlots = F32 ? 8 : 4;  // 16-byte slots of a row for 32 columns
+#pragma unroll
+        for (int q = 0; q < kSlots; ++q) {
+          const uint32_t at = box_slot(box, lane, q + (F32 ? 0 : 4 * half));
+          if constexpr (F32) {
+            float4 o = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            if (kRes) {
+              const uint4 x = lds128(at);
+              o.x += __uint_as_float(x.x); o.y += __uint_as_float(x.y);
+              o.z += __uint_as_float(x.z); o.w += __uint_as_float(x.w);
+            }
+            sts128(at, make_uint4(__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z),
+                                  __float_as_uint(o.w)));
+          } else {
+            if (kRes) {
+              const uint4 x = lds128(at);
+              const uint32_t x4[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2(x4[e], p.h16);
+                v[8 * q + 2 * e] += f.x;
+                v[8 * q + 2 * e + 1] += f.y;
+              }
+            }
+            sts128(at, make_uint4(pack2(v[8 * q], v[8 * q + 1], p.h16), pack2(v[8 * q + 2], v[8 * q + 3], p.h16),
+                                  pack2(v[8 * q + 4], v[8 * q + 5], p.h16),
+                                  pack2(v[8 * q + 6], v[8 * q + 7], p.h16)));
+          }
+        }
+        if (F32 || half == 1) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmC, box, col0 + (F32 ? 32 * half : 0), row0);
+            bulk_commit();
+          }
+        }
+      }
+      if (*abort_flag) break;
+    }
+    if (kRes && waited < loads) {  // a load in flight lands before the CTA leaves (bounded)
+      volatile int no_abort = 0;
+      mbar_wait(res_bar(w), waited & 1, &no_abort);
+    }
+    if (lane == 0) bulk_wait_all();  // this warp's stores are complete
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && p.err) atomicOr(p.err, kErrTimeout);
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// ── host ────────────────────────────────────────────────────────────────────
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  return fn;
+}
+
+// 2-D map over a dense [rows, cols] buffer with boxes of 128 bytes x box_rows,
+// 128-byte swizzle.
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, int esz, const void* ptr, int rows, int cols,
+              int box_rows) {
+  auto enc = encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * esz};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / esz), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, int EPI, bool F32>
+cudaError_t launch_tile(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
+  using Cfg = MxCfg<BN>;
+  CUtensorMap ma, mb, mc, mr;
+  const CUtensorMapDataType ct = F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : p.h16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const int esz = F32 ? 4 : 2;
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  bool ok = make_map(&ma, u8, 1, g.aq, g.M, g.K / 2, kBM) && make_map(&mb, u8, 1, g.wq, g.N, g.K / 2, BN) &&
+            make_map(&mc, ct, esz, g.C, g.M, g.N, 32);
+  mr = mc;  // unused without a residual
+  if (ok && EPI == JB_EPI_RESIDUAL) ok = make_map(&mr, ct, esz, g.resid, g.M, g.N, 32);
+  if (!ok) {
+    if (why) *why = "linear(mxfp4): cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  auto kern = gemm_mxfp4_kernel<BN, EPI, F32>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  // the shared-memory opt-in is a property of each device's context
+  static std::atomic<uint8_t> attr_set[64];
+  if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_set[dev].store(1, std::memory_order_release);
+  }
+  const long long tiles = ((g.M + kBM - 1ll) / kBM) * ((g.N + BN - 1) / BN);
+  const int grid = static_cast<int>(std::min<long long>(num_sms(dev), tiles));
+  kern<<<grid, Cfg::THREADS, Cfg::SMEM, s>>>(ma, mb, mc, mr, p);
+  return cudaGetLastError();
+}
+
+template <int BN, bool F32>
+cudaError_t launch_epi(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
+  switch (g.epi) {
+    case JB_EPI_GELU: return launch_tile<BN, JB_EPI_GELU, F32>(g, p, s, why);
+    case JB_EPI_QUICK_GELU: return launch_tile<BN, JB_EPI_QUICK_GELU, F32>(g, p, s, why);
+    case JB_EPI_RESIDUAL: return launch_tile<BN, JB_EPI_RESIDUAL, F32>(g, p, s, why);
+    default: return launch_tile<BN, JB_EPI_NONE, F32>(g, p, s, why);
+  }
+}
+template <int BN>
+cudaError_t launch_out(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
+  return g.c_dtype == JB_DT_F32 ? launch_epi<BN, true>(g, p, s, why) : launch_epi<BN, false>(g, p, s, why);
+}
+
+}  // namespace
+
+cudaError_t launch_linear_mxfp4(const MxGemmArgs& g, cudaStream_t s, std::string* why) {
+  if (g.M == 0) return cudaSuccess;
+  const long long m_tiles = (g.M + kBM - 1ll) / kBM;
+  if (m_tiles * ((g.N + 63) / 64) > INT32_MAX / 2) {
+    if (why) *why = "linear(mxfp4): too many output tiles";
+    return cudaErrorInvalidValue;
+  }
+  MxParams p{g.a_scale, g.w_scale, g.bias, g.M, g.N, g.K, g.epi, g.c_dtype == JB_DT_F16 ? 1 : 0, g.err};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const long long sms = num_sms(dev);
+  if (m_tiles * ((g.N + 127) / 128) <= sms) return launch_out<64>(g, p, s, why);
+  // f32 outputs hold 64 accumulators and 32 results: more than 448 threads have registers for
+  if (g.c_dtype == JB_DT_F32 || m_tiles * ((g.N + 191) / 192) <= sms) return launch_out<128>(g, p, s, why);
+  return launch_epi<192, false>(g, p, s, why);
+}
+
+}  // namespace jb

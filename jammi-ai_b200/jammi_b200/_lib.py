@@ -87,6 +87,10 @@ _SIGS = [
     ("jb_op_layernorm", _I, [_P, _P, _P, _P, _P, _I, _I, _I, ctypes.c_float, _P]),
     ("jb_op_rmsnorm", _I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, ctypes.c_float, _P]),
     ("jb_op_dequantize_rows", _I, [_P, _P, _P, _I, _I, _I, _P]),
+    ("jb_mxfp4_scale_bytes", ctypes.c_size_t, [_I, _I]),
+    ("jb_op_quantize_mxfp4", _I, [_P, _I, _P, _P, _I, _I, _P]),
+    ("jb_op_dequantize_mxfp4", _I, [_P, _P, _P, _I, _I, _I, _P]),
+    ("jb_op_linear_mxfp4", _I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     ("jb_op_attention", _I, [_P, _P, _P, _I, _I, _I, _I, _I, _P]),
     ("jb_op_attention_causal", _I, [_P, _P, _P, _I, _I, _I, _I, _I, _P]),
     ("jb_op_attention_rows", _I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),

@@ -167,6 +167,69 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) 
     return y
 
 
+_U8 = (torch.uint8,)
+
+
+def _mx_scale_shape(rows, cols):
+    return ((rows + 127) // 128, (cols + 127) // 128, 512)
+
+
+def quantize_mxfp4(x: torch.Tensor):
+    """MXFP4 form of ``x`` [R, C] (f32, bf16 or f16; C a multiple of 32): codes uint8 [R, C / 2],
+    the even column in the low half, and scale bytes uint8 [ceil(R / 128), ceil(C / 128), 512] in
+    the order ``linear_mxfp4`` reads (``jb_op_quantize_mxfp4``)."""
+    _check("x", x, None, _FLOATS)
+    if x.dim() != 2 or x.shape[1] % 32 or not x.shape[1]:
+        raise ValueError("x must be [rows, cols] with cols a multiple of 32")
+    R, C = x.shape
+    q = torch.empty((R, C // 2), dtype=torch.uint8, device=x.device)
+    scale = torch.empty(_mx_scale_shape(R, C), dtype=torch.uint8, device=x.device)
+    if R:
+        _call(lib().jb_op_quantize_mxfp4, x.device, x.data_ptr(), _DT[x.dtype], q.data_ptr(), scale.data_ptr(), R, C)
+    return q, scale
+
+
+def _check_mxfp4(name, q, scale, device=None):
+    _check(name, q, None, _U8, device)
+    if q.dim() != 2 or q.shape[1] % 16 or not q.shape[1]:
+        raise ValueError(f"{name} must be [rows, cols / 2] with cols a multiple of 32")
+    _check(name + "'s scale", scale, _mx_scale_shape(q.shape[0], 2 * q.shape[1]), _U8, q.device)
+
+
+def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values [R, C] that ``quantize_mxfp4``'s codes and scales stand for, in ``dtype``."""
+    _check_mxfp4("q", q, scale)
+    if dtype not in _FLOATS:
+        raise ValueError(f"{dtype} is not one of {', '.join(map(str, _FLOATS))}")
+    R, C = q.shape[0], 2 * q.shape[1]
+    y = torch.empty((R, C), dtype=dtype, device=q.device)
+    if R:
+        _call(lib().jb_op_dequantize_mxfp4, q.device, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype], R, C)
+    return y
+
+
+def linear_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias=None,
+                 residual=None, epilogue: int = L.EPI_NONE, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """``epi(a @ w.T + bias)`` [M, N] of MXFP4 activations [M, K] and weights [N, K], both as
+    ``quantize_mxfp4`` returns them; N a multiple of 8, ``out_dtype`` f32, bf16 or f16 (the
+    residual's too), bias f32 [N]."""
+    _check_mxfp4("aq", aq, a_scale)
+    dev = aq.device
+    _check_mxfp4("wq", wq, w_scale, dev)
+    if wq.shape[1] != aq.shape[1]:
+        raise ValueError("aq and wq must have the same number of columns")
+    M, N, K = aq.shape[0], wq.shape[0], 2 * aq.shape[1]
+    if out_dtype not in _FLOATS:
+        raise ValueError(f"{out_dtype} is not one of {', '.join(map(str, _FLOATS))}")
+    _check("bias", bias, wq.shape[:1], _F32, dev, optional=True)
+    _check("residual", residual, (M, N), (out_dtype,), dev, optional=True)
+    c = torch.empty((M, N), dtype=out_dtype, device=dev)
+    if M:
+        _call(lib().jb_op_linear_mxfp4, dev, aq.data_ptr(), a_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
+              _p(bias), _p(residual), c.data_ptr(), _DT[out_dtype], M, N, K, epilogue)
+    return c
+
+
 def attention(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, max_len: int,
               causal: bool = False, tma: bool = False) -> torch.Tensor:
     """qkv [T, 3*heads*d] packed rows, cu_seqlens int32 [B+1] -> ctx [T, heads*d]

@@ -180,3 +180,209 @@ def test_rmsnorm_empty_and_refusals(dev):
             ops.rmsnorm(a["x"], a["gamma"], EPS, residual=a["residual"])
         with pytest.raises(ValueError):
             ops.rmsnorm_quantize(a["x"], a["gamma"], EPS, residual=a["residual"])
+
+
+# ── MXFP4 ───────────────────────────────────────────────────────────────────
+
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def mx_ref(x):
+    """(values, codes, scale bytes) of x's MXFP4 form in float64, block by block of 32."""
+    b = x.double().reshape(x.shape[0], -1, 32)
+    top = b.abs().amax(-1)
+    powers = torch.tensor([2.0 ** p for p in range(-149, 128)], dtype=torch.float64, device=x.device)
+    floor = torch.searchsorted(powers, top, right=True) - 1 - 149
+    e = torch.where(top > 0, floor - 2, torch.full_like(floor, -127)).clamp(-127, 127)
+    bad = ~torch.isfinite(b).all(-1)
+    z = b.abs() * torch.exp2(-e.double())[..., None]
+    gap = (z[..., None] - torch.tensor(E2M1, dtype=torch.float64, device=x.device)).abs()
+    near = gap.amin(-1, keepdim=True)
+    even = torch.tensor([i % 2 == 0 for i in range(8)], device=x.device)
+    hit = gap == near
+    code = torch.where((hit & even).any(-1), (hit & even).int().argmax(-1), hit.int().argmax(-1))
+    code = torch.where(bad[..., None], torch.zeros_like(code), code)
+    v = torch.tensor(E2M1, dtype=torch.float64, device=x.device)[code] * torch.exp2(e.double())[..., None]
+    v = torch.where(bad[..., None], torch.full_like(v, math.nan), torch.where(torch.signbit(b), -v, v))
+    neg = torch.signbit(b) & ~bad[..., None]
+    byte = torch.where(bad, torch.full_like(e, 255), e + 127)
+    return v.reshape(x.shape), (code + 8 * neg).reshape(x.shape), byte
+
+
+def scale_bytes(scale, rows, cols):
+    """The scale tiles as [rows, cols / 32], and what pads them."""
+    rt, ct, _ = scale.shape
+    full = scale.reshape(rt, ct, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(rt * 128, ct * 4).long()
+    pad = full.clone()
+    pad[:rows, :cols // 32] = 0
+    return full[:rows, :cols // 32], pad
+
+
+MX_SHAPES = [(1, 32), (1, 64), (12, 768), (127, 96), (128, 256), (129, 288), (300, 1024), (1000, 160), (40, 4096)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,cols", MX_SHAPES)
+def test_quantize_mxfp4(dev, rows, cols, dt):
+    g = _gen(rows + cols)
+    x = torch.randn((rows, cols), generator=g, device=dev)
+    x *= torch.exp2(torch.randint(-12, 12, (rows, cols // 32, 1), generator=g, device=dev).float()).expand(
+        -1, -1, 32).reshape(rows, cols)
+    x = x.to(DTYPES[dt])
+    q, scale = _ops().quantize_mxfp4(x)
+    v, code, byte = mx_ref(x)
+    got = torch.stack((q & 15, q >> 4), -1).reshape(rows, cols)
+    assert torch.equal(got.long(), code.long())
+    sb, pad = scale_bytes(scale, rows, cols)
+    assert torch.equal(sb, byte.long()) and not pad.any()
+    for t in DTYPES.values():
+        assert torch.equal(_ops().dequantize_mxfp4(q, scale, t), v.to(t))
+
+
+def test_quantize_mxfp4_borders(dev):
+    """Every border between two codes, its neighbours, saturation, tiny and huge blocks, zeros,
+    and blocks that are not finite."""
+    x = torch.zeros((12, 64), device=dev)
+    mids = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0], device=dev)
+    x[0, 0], x[0, 1:9], x[0, 9:17] = 7.75, mids, -mids  # scale 2^0; 7.75 saturates at 6
+    x[1, 0], x[1, 1:9] = 4.0, torch.nextafter(mids, torch.tensor(9.0, device=dev)).clamp(max=6.0)
+    x[2, 0], x[2, 1:9] = -4.0, torch.nextafter(mids, torch.tensor(0.0, device=dev))
+    x[3] = 2.0 ** -126
+    x[4, 3] = 1e-41
+    x[5, 40] = torch.finfo(torch.float32).max
+    x[5, 41] = -1e-30
+    x[6, 2] = math.nan
+    x[7, 63] = -math.inf
+    x[8, 31], x[8, 32] = -0.0, 2.0 ** 127
+    x[9] = -6.0
+    x[10, ::2] = 3.0
+    q, scale = _ops().quantize_mxfp4(x)
+    v, code, byte = mx_ref(x)
+    got = torch.stack((q & 15, q >> 4), -1).reshape(12, 64)
+    assert torch.equal(got.long(), code.long())
+    assert torch.equal(scale_bytes(scale, 12, 64)[0], byte.long())
+    y = _ops().dequantize_mxfp4(q, scale, torch.float32)
+    assert torch.equal(torch.nan_to_num(y, nan=-1.0), torch.nan_to_num(v.float(), nan=-1.0))
+    assert y[6, :32].isnan().all() and not y[6, 32:].isnan().any()
+
+
+def gelu64(z):
+    return 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5)))
+
+
+LIN_SHAPES = [(1, 8, 32), (12, 2304, 768), (3, 72, 64), (127, 200, 96), (129, 264, 160), (64, 1024, 4096), (300, 1536, 384),
+              (2000, 1160, 288), (5000, 768, 768), (4100, 1000, 1056)]
+
+
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("M,N,K", LIN_SHAPES)
+def test_linear_mxfp4_places(dev, M, N, K, out):
+    """One non-zero activation per row: every output is one weight exactly, which
+    shows each code and each scale byte in its place."""
+    ops, g = _ops(), _gen(M + N + K)
+    x = torch.zeros((M, K), device=dev)
+    at = torch.randint(0, K, (M,), generator=g, device=dev)
+    at[0], at[-1] = 0, K - 1
+    x[torch.arange(M, device=dev), at] = torch.exp2(torch.randint(-8, 8, (M,), generator=g, device=dev).float())
+    w = torch.randn((N, K), generator=g, device=dev)
+    w *= torch.exp2(torch.randint(-6, 6, (N, K // 32), generator=g, device=dev).float()).repeat_interleave(32, 1)
+    aq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(w)
+    c = ops.linear_mxfp4(*aq, *wq, out_dtype=DTYPES[out])
+    ops.sync()
+    # |x| <= 128 and |w| <= 2^10: inside f16; a power of two times an e2m1 value: no rounding in any type
+    want = x[torch.arange(M, device=dev), at][:, None].double() * mx_ref(w)[0][:, at].T
+    assert torch.equal(c.double(), want.to(DTYPES[out]).double())
+
+
+def linear_check(c, a, w, bias, res, epi, K):
+    """Float64 of the quantised operands.  The accumulator: the products of a
+    block are exact, and each of the K / 16 partial sums is off by at most two
+    units of 2^-24 of the terms' magnitudes (truncated alignment counted);
+    then bias, activation (1e-6 max(1, |z|)), residual and the output's own
+    rounding u."""
+    z = a @ w.T
+    mag = a.abs() @ w.abs().T
+    if bias is not None:
+        z = z + bias.double()
+        mag = mag + bias.double().abs()
+    off = (K / 16 * 2 + 4) * 2.0 ** -24 * mag
+    if epi == "gelu":
+        z, off = gelu64(z), 1.13 * off + 1e-6 * z.abs().clamp(min=1)
+    elif epi == "quick_gelu":
+        z, off = z * torch.sigmoid(1.702 * z), 1.1 * off + 1e-6 * z.abs().clamp(min=1)
+    elif epi == "residual":
+        z = z + res.double()
+        off = off + 2.0 ** -23 * res.double().abs()
+    u = torch.finfo(c.dtype).eps / 2
+    tiny = torch.finfo(c.dtype).smallest_normal * torch.finfo(c.dtype).eps
+    err = (c.double() - z).abs()
+    ok = err <= off * (1 + u) + u * z.abs() + tiny
+    assert ok.all(), (err / (off + u * z.abs() + tiny)).max()
+
+
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("epi", ["none", "gelu", "quick_gelu", "residual"])
+@pytest.mark.parametrize("M,N,K", LIN_SHAPES)
+def test_linear_mxfp4(dev, M, N, K, epi, out):
+    from jammi_b200 import _lib as L
+    ops, g, t = _ops(), _gen(M * 3 + N + K), DTYPES[out]
+    a = torch.randn((M, K), generator=g, device=dev)
+    w = torch.randn((N, K), generator=g, device=dev) / math.sqrt(K)
+    bias = torch.randn((N,), generator=g, device=dev) if epi != "quick_gelu" else None
+    res = torch.randn((M, N), generator=g, device=dev).to(t) if epi == "residual" else None
+    aq, wq = ops.quantize_mxfp4(a), ops.quantize_mxfp4(w)
+    codes = {"none": L.EPI_NONE, "gelu": L.EPI_GELU, "quick_gelu": L.EPI_QUICK_GELU, "residual": L.EPI_RESIDUAL}
+    c = ops.linear_mxfp4(*aq, *wq, bias=bias, residual=res, epilogue=codes[epi], out_dtype=t)
+    ops.sync()
+    linear_check(c, mx_ref(a)[0], mx_ref(w)[0], bias, res, epi, K)
+
+
+def test_linear_mxfp4_residual_in_place_and_nan_rows(dev):
+    from jammi_b200 import _lib as L
+    ops, g = _ops(), _gen(8)
+    M, N, K = 333, 328, 128
+    a, w = torch.randn((M, K), generator=g, device=dev), torch.randn((N, K), generator=g, device=dev)
+    a[7, 40] = math.nan
+    w[9, 100] = math.inf
+    aq, wq = ops.quantize_mxfp4(a), ops.quantize_mxfp4(w)
+    res = torch.randn((M, N), generator=g, device=dev).bfloat16()
+    want = ops.linear_mxfp4(*aq, *wq, residual=res, epilogue=L.EPI_RESIDUAL)
+    L.check(L.lib().jb_op_linear_mxfp4(aq[0].data_ptr(), aq[1].data_ptr(), wq[0].data_ptr(), wq[1].data_ptr(), None,
+                                       res.data_ptr(), res.data_ptr(), L.DT_BF16, M, N, K, L.EPI_RESIDUAL,
+                                       torch.cuda.current_stream().cuda_stream))
+    ops.sync()
+    assert torch.equal(torch.nan_to_num(res.float(), nan=1e9), torch.nan_to_num(want.float(), nan=1e9))
+    nan = want.isnan()
+    assert nan[7].all() and nan[:, 9].all() and nan.sum() == M + N - 1
+
+
+def test_mxfp4_refusals(dev):
+    ops = _ops()
+    x = torch.ones((4, 64), device=dev)
+    for bad in (x[:, :48].contiguous(), x.t(), x.double(), x.cpu(), x[0], x[:, :0]):
+        with pytest.raises(ValueError):
+            ops.quantize_mxfp4(bad)
+    q, s = ops.quantize_mxfp4(x)
+    w, ws = ops.quantize_mxfp4(torch.ones((16, 64), device=dev))
+    odd, odds = ops.quantize_mxfp4(torch.ones((15, 64), device=dev))
+    short, shorts = ops.quantize_mxfp4(torch.ones((16, 32), device=dev))
+    from jammi_b200 import _lib as L
+    from jammi_b200._lib import JbError
+    for args, kw in (((q, s, short, shorts), {}), ((q, s[0], w, ws), {}), ((q.cpu(), s, w, ws), {}),
+                     ((q, s, w, ws), dict(bias=torch.ones(15, device=dev))),
+                     ((q, s, w, ws), dict(bias=torch.ones(16, device=dev).half())),
+                     ((q, s, w, ws), dict(residual=torch.ones((4, 16), device=dev), epilogue=L.EPI_RESIDUAL)),
+                     ((q, s, w, ws), dict(out_dtype=torch.int32)), ((q.int(), s, w, ws), {})):
+        with pytest.raises(ValueError):
+            ops.linear_mxfp4(*args, **kw)
+    for args, kw in (((q, s, odd, odds), {}), ((q, s, w, ws), dict(epilogue=L.EPI_RESIDUAL)), ((q, s, w, ws), dict(epilogue=7)),
+                     ((q, s, w, ws), dict(residual=torch.ones((4, 16), device=dev).bfloat16()))):
+        with pytest.raises(JbError) as e:
+            ops.linear_mxfp4(*args, **kw)
+        assert e.value.status == L.ERR_INVALID
+    with pytest.raises(ValueError):
+        ops.dequantize_mxfp4(q, s, torch.int8)
+    none = ops.quantize_mxfp4(torch.empty((0, 64), device=dev))
+    assert none[0].shape == (0, 32) and none[1].shape == (0, 1, 512)
+    assert ops.dequantize_mxfp4(*none).shape == (0, 64)
+    assert ops.linear_mxfp4(*none, w, ws).shape == (0, 16)

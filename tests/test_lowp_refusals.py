@@ -35,3 +35,28 @@ def test_rmsnorm_refuses(kw):
 def test_dequantize_rows_refuses(kw):
     a = dict(q=P, scale=P, y=P, dtype=L.DT_F32, rows=2, cols=8) | kw
     refused(L.lib().jb_op_dequantize_rows, a["q"], a["scale"], a["y"], a["dtype"], a["rows"], a["cols"], None)
+
+
+@pytest.mark.parametrize("fn", ["jb_op_quantize_mxfp4", "jb_op_dequantize_mxfp4"])
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(cols=0), dict(cols=48), dict(cols=-32), dict(dtype=L.DT_S8), dict(x=None),
+                                dict(q=None), dict(scale=None), dict(x=P + 8), dict(q=P + 4), dict(scale=P + 2)])
+def test_mxfp4_rows_refuse(fn, kw):
+    a = dict(x=P, dtype=L.DT_BF16, q=P, scale=P, rows=4, cols=64) | kw
+    args = [a["x"], a["dtype"], a["q"], a["scale"]] if "_quantize" in fn else [a["q"], a["scale"], a["x"], a["dtype"]]
+    assert fn in refused(getattr(L.lib(), fn), *args, a["rows"], a["cols"], None)
+
+
+@pytest.mark.parametrize("kw", [dict(M=-1), dict(N=0), dict(N=12), dict(K=0), dict(K=48), dict(c_dtype=L.DT_S32),
+                                dict(epi=-1), dict(epi=4), dict(epi=L.EPI_RESIDUAL), dict(res=P), dict(aq=None),
+                                dict(ws=None), dict(c=None), dict(aq=P + 8), dict(c=P + 2), dict(asc=P + 1),
+                                dict(epi=L.EPI_RESIDUAL, res=P + 4)])
+def test_linear_mxfp4_refuses(kw):
+    a = dict(aq=P, asc=P, wq=P, ws=P, bias=None, res=None, c=P, c_dtype=L.DT_BF16, M=4, N=16, K=64, epi=L.EPI_NONE) | kw
+    refused(L.lib().jb_op_linear_mxfp4, a["aq"], a["asc"], a["wq"], a["ws"], a["bias"], a["res"], a["c"], a["c_dtype"],
+            a["M"], a["N"], a["K"], a["epi"], None)
+
+
+def test_mxfp4_scale_bytes():
+    f = L.lib().jb_mxfp4_scale_bytes
+    assert [f(1, 32), f(128, 128), f(129, 128), f(128, 160), f(0, 64), f(-1, 64)] == [512, 512, 1024, 1024, 0, 0]
+    assert f(2 ** 31 - 1, 4096) == 2 ** 24 * 32 * 512
