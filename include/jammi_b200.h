@@ -305,6 +305,21 @@ jb_status jb_op_attention_causal(const void* qkv, const int* cu_seqlens, void* c
 jb_status jb_op_attention_rows(const void* qkv, const int* cu_seqlens, void* ctx, int dtype,
                                int batch, int heads, int head_dim, int max_len, int rows,
                                int causal, void* stream);
+/* Windowed attention over packed rows: query i of a row of n tokens sees key j
+ * iff j <= i + right and (j >= i - left or j < sinks) -- a sliding window with
+ * `sinks` first tokens that stay visible behind it (right = 0: causal).
+ * softmax(Q K^T / sqrt(d)) V over those keys.  qkv [rows, (heads + 2 kv_heads)
+ * * head_dim]: Q|K|V column blocks, head-major inside each; query head h reads
+ * key / value head h / (heads / kv_heads).  ctx [rows, heads * head_dim]; rows
+ * of qkv behind cu_seqlens[batch] are not read and of ctx not written.  left,
+ * right: 0 .. 2^31 - 1 (anything >= the row's length: unbounded).  dtype F32,
+ * BF16 or F16; head_dim 8, 16, 32, 64 or 128; heads a multiple of kv_heads;
+ * max_len bounds every row's length, rows >= cu_seqlens[batch]; qkv and ctx
+ * 16-byte aligned.  No counterpart in the reference (its ModernBERT layers
+ * attend to the whole row, crates/jammi-encoders/src/modernbert.rs). */
+jb_status jb_op_attention_window(const void* qkv, const int* cu_seqlens, void* ctx, int dtype,
+                                 int batch, int heads, int kv_heads, int head_dim, int max_len,
+                                 int rows, int left, int right, int sinks, void* stream);
 /* Process-wide choice for bf16 head_dim-64 attention with TMA (model forwards;
  * f16 always runs on the tcgen05 kernel, and is refused when it is off)
  * and jb_op_attention_rows): on != 0 (the default) runs every row on the

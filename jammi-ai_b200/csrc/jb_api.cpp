@@ -1,5 +1,6 @@
 // The C ABI (include/jammi_b200.h): argument checks, exception -> status
 // mapping, the thread-local error message and the per-handle lock.
+#include <algorithm>
 #include <cstring>
 #include <mutex>
 #include <string>
@@ -711,6 +712,48 @@ jb_status jb_op_attention_rows(const void* qkv, const int* cu_seqlens, void* ctx
   if (rows < 0) return jb::record_error(JB_ERR_INVALID, "jb_op_attention_rows: rows must be >= 0");
   return op_attention(qkv, cu_seqlens, ctx, dtype, batch, heads, head_dim, max_len, causal ? 1 : 0,
                       stream, rows);
+}
+
+jb_status jb_op_attention_window(const void* qkv, const int* cu_seqlens, void* ctx, int dtype, int batch, int heads,
+                                 int kv_heads, int head_dim, int max_len, int rows, int left, int right, int sinks,
+                                 void* stream) {
+  return guarded([&] {
+    if (batch < 0 || heads <= 0 || kv_heads <= 0 || max_len < 0 || rows < 0)
+      jb::fail(JB_ERR_INVALID, "jb_op_attention_window: batch, max_len and rows must be >= 0, heads and kv_heads > 0");
+    if (heads % kv_heads) jb::fail(JB_ERR_INVALID, "jb_op_attention_window: heads must be a multiple of kv_heads");
+    if (!is_float_dtype(dtype)) jb::fail(JB_ERR_INVALID, "jb_op_attention_window: dtype must be f32, bf16 or f16");
+    if (head_dim != 8 && head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128)
+      jb::fail(JB_ERR_INVALID, "jb_op_attention_window: head_dim must be 8, 16, 32, 64 or 128");
+    if ((heads + 2ll * kv_heads) * head_dim > (1 << 24))
+      jb::fail(JB_ERR_INVALID, "jb_op_attention_window: a token's heads hold more than 2^24 elements");
+    if (left < 0 || right < 0 || sinks < 0)
+      jb::fail(JB_ERR_INVALID, "jb_op_attention_window: left, right and sinks must be >= 0");
+    if (batch == 0 || max_len == 0 || rows == 0) return;
+    if (!qkv || !cu_seqlens || !ctx) jb::fail(JB_ERR_INVALID, "jb_op_attention_window: null buffer");
+    if (!aligned16(qkv) || !aligned16(ctx))
+      jb::fail(JB_ERR_INVALID, "jb_op_attention_window: qkv and ctx must be 16-byte aligned");
+    jb::WindowArgs a;
+    a.qkv = qkv;
+    a.cu = cu_seqlens;
+    a.ctx = ctx;
+    a.dtype = dtype;
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.max_len = std::min(max_len, rows);
+    a.rows = rows;
+    a.left = left;
+    a.right = right;
+    a.sinks = sinks;
+    a.err = op_flag(current_device());
+    std::string why;
+    cudaError_t e = jb::launch_attention_window(a, as_stream(stream), &why);
+    if (e != cudaSuccess) {
+      if (!why.empty()) jb::fail(JB_ERR_INVALID, why);
+      jb::check_cuda(e, "jb_op_attention_window");
+    }
+  });
 }
 
 jb_status jb_op_wait_flag(const int* d_flag, int expect, int limit_ms, void* stream) {

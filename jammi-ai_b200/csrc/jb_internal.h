@@ -151,6 +151,20 @@ cudaError_t launch_attention(const void* qkv, const int* cu, void* ctx, int dtyp
                              int rows_cap = 0, int* err = nullptr, int causal = 0,
                              int* work = nullptr);
 
+// Windowed attention (jb_window.cu); see jb_op_attention_window.
+struct WindowArgs {
+  const void* qkv = nullptr;
+  const int* cu = nullptr;  // [batch + 1]
+  void* ctx = nullptr;
+  int dtype = JB_DT_BF16;
+  int batch = 0, heads = 0, kv_heads = 0, head_dim = 0;
+  int max_len = 0;  // bounds every row's length
+  int rows = 0;     // rows that qkv holds
+  int left = 0, right = 0, sinks = 0;
+  int* err = nullptr;  // device flag set when a bounded wait gives up
+};
+cudaError_t launch_attention_window(const WindowArgs& a, cudaStream_t s, std::string* why);
+
 // Bounded wait of one thread until *flag == expect, at most limit_ms; on
 // expiry kErrTimeout in *err (jb_wait.cu).
 cudaError_t launch_flag_wait(const int* flag, int expect, int limit_ms, int* err, cudaStream_t s);

@@ -250,6 +250,28 @@ def attention(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, max_len: 
     return ctx
 
 
+def attention_window(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, max_len: int, left: int, right: int,
+                     sinks: int = 0, kv_heads=None) -> torch.Tensor:
+    """Windowed attention over packed rows: qkv [T, (heads + 2 * kv_heads) * d] (Q|K|V), cu_seqlens
+    int32 [B+1] -> ctx [T, heads*d].  Query i of a row sees key j iff ``j <= i + right and
+    (j >= i - left or j < sinks)``; ``kv_heads`` None means ``heads``; d 8, 16, 32, 64 or 128.
+    Rows behind ``cu_seqlens[-1]`` are left unwritten."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    _check("qkv", qkv, None, _FLOATS)
+    _check("cu_seqlens", cu_seqlens, None, (torch.int32,), qkv.device)
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("heads must be a positive multiple of kv_heads")
+    if qkv.dim() != 2 or not qkv.shape[1] or qkv.shape[1] % (heads + 2 * kv_heads):
+        raise ValueError("qkv must be [tokens, (heads + 2 * kv_heads) * head_dim]")
+    if cu_seqlens.dim() != 1 or not cu_seqlens.numel():
+        raise ValueError("cu_seqlens must be [batch + 1]")
+    T, d = qkv.shape[0], qkv.shape[1] // (heads + 2 * kv_heads)
+    ctx = torch.empty((T, heads * d), dtype=qkv.dtype, device=qkv.device)
+    _call(lib().jb_op_attention_window, qkv.device, qkv.data_ptr(), cu_seqlens.data_ptr(), ctx.data_ptr(),
+          _DT[qkv.dtype], cu_seqlens.numel() - 1, heads, kv_heads, d, max_len, T, left, right, sinks)
+    return ctx
+
+
 def pool_normalize(hidden: torch.Tensor, cu_seqlens: torch.Tensor, pooling: int = L.POOL_MEAN):
     _contig(hidden, cu_seqlens)
     T, H = hidden.shape

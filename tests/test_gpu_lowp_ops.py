@@ -386,3 +386,140 @@ def test_mxfp4_refusals(dev):
     assert none[0].shape == (0, 32) and none[1].shape == (0, 1, 512)
     assert ops.dequantize_mxfp4(*none).shape == (0, 64)
     assert ops.linear_mxfp4(*none, w, ws).shape == (0, 16)
+
+
+# ── windowed attention ──────────────────────────────────────────────────────
+
+def window_ref(qkv, lens, h, hk, left, right, sinks):
+    """Float64, row by row; also sum_j p_j |v_j| / sum_j p_j and max |q k| / sqrt(d) for the error bound."""
+    d = qkv.shape[1] // (h + 2 * hk)
+    x = qkv.double()
+    out, mag = torch.zeros((qkv.shape[0], h * d), dtype=torch.float64, device=qkv.device), None
+    mag, top, at = out.clone(), 0.0, 0
+    for n in lens:
+        if n:
+            q, k, v = x[at:at + n].split([h * d, hk * d, hk * d], 1)
+            q = q.reshape(n, h, d).transpose(0, 1)
+            k = k.reshape(n, hk, d).transpose(0, 1).repeat_interleave(h // hk, 0)
+            v = v.reshape(n, hk, d).transpose(0, 1).repeat_interleave(h // hk, 0)
+            i, j = torch.arange(n, device=x.device)[:, None], torch.arange(n, device=x.device)[None]
+            seen = (j <= i + right) & ((j >= i - left) | (j < sinks))
+            s = (q @ k.transpose(1, 2) / math.sqrt(d)).masked_fill(~seen, -math.inf)
+            top = max(top, (q.abs() @ k.abs().transpose(1, 2)).max().item() / math.sqrt(d))
+            p = torch.softmax(s, -1)
+            out[at:at + n] = (p @ v).transpose(0, 1).reshape(n, h * d)
+            mag[at:at + n] = (p @ v.abs()).transpose(0, 1).reshape(n, h * d)
+        at += n
+    return out, mag, top
+
+
+def window_check(got, qkv, lens, h, hk, left, right, sinks, tensor_cores):
+    """An output is sum p v / sum p.  Scores: d products and sums in f32, off by (d + 4) 2^-24 of
+    sum |q k| / sqrt(d) =: top, so p is off by that share (and 2^-21 for the exponential and its
+    argument's rounding at |argument| <= 2 top log2 e).  On tensor cores each p is also rounded to
+    the rows' 16-bit type (u), against an unrounded sum.  The sums over up to n keys in f32 add
+    n 2^-24.  All of it is a share of sum p |v| / sum p; the store rounds once."""
+    ref, mag, top = window_ref(qkv, lens, h, hk, left, right, sinks)
+    d = qkv.shape[1] // (h + 2 * hk)
+    u = torch.finfo(qkv.dtype).eps / 2
+    share = 2 * ((d + 8) * 2.0 ** -24 * top + 2.0 ** -21) + max(lens, default=0) * 2.0 ** -23 + (u if tensor_cores else 0)
+    T = sum(lens)
+    err = (got.double() - ref)[:T].abs()
+    bound = share * mag[:T] + u * (ref[:T].abs() + share * mag[:T]) + torch.finfo(qkv.dtype).smallest_normal * 2 * u
+    assert (err <= bound).all(), (err / bound).max().item()
+
+
+WINDOWS = [(64, 64, 0), (64, 64, 1), (0, 0, 0), (0, 0, 3), (128, 0, 0), (255, 0, 4), (17, 200, 5), (300, 5, 130),
+           (2 ** 31 - 1, 2 ** 31 - 1, 0), (2 ** 31 - 1, 0, 2 ** 31 - 1), (1, 1, 700)]
+LENS = [[1], [12], [0, 5, 0, 0, 129, 64, 1, 127, 128, 0], [300, 1, 257, 512, 40], [1000]]
+
+
+def run_window(dev, lens, h, hk, d, t, left, right, sinks, seed, extra=3, scale=1.0):
+    g = _gen(seed)
+    T = sum(lens)
+    qkv = (torch.randn((T + extra, (h + 2 * hk) * d), generator=g, device=dev) * scale).to(t)
+    qkv[T:] = math.nan  # rows behind the last sequence
+    cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32).to(dev)
+    got = _ops().attention_window(qkv, cu, h, max(lens), left, right, sinks=sinks, kv_heads=hk)
+    _ops().sync()
+    return qkv, got
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("lens", LENS, ids=lambda v: "x".join(map(str, v)))
+@pytest.mark.parametrize("left,right,sinks", WINDOWS)
+def test_attention_window_64(dev, lens, left, right, sinks, dt):
+    t = DTYPES[dt]
+    qkv, got = run_window(dev, lens, 3, 3, 64, t, left, right, sinks, sum(lens) + left % 1000 + sinks % 1000)
+    window_check(got, qkv, lens, 3, 3, left, right, sinks, t != torch.float32)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 64), (6, 1, 64), (2, 2, 128), (4, 1, 128), (3, 3, 32), (4, 2, 16), (5, 5, 8)])
+@pytest.mark.parametrize("left,right,sinks", [(64, 64, 1), (100, 0, 4), (2 ** 31 - 1, 2 ** 31 - 1, 0)])
+def test_attention_window_heads(dev, h, hk, d, left, right, sinks, dt):
+    t, lens = DTYPES[dt], [200, 3, 0, 129, 391]
+    qkv, got = run_window(dev, lens, h, hk, d, t, left, right, sinks, h * 100 + d)
+    window_check(got, qkv, lens, h, hk, left, right, sinks, t != torch.float32)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+def test_attention_window_long_rows_and_large_scores(dev, dt):
+    t, lens = DTYPES[dt], [5000, 17, 2049]
+    qkv, got = run_window(dev, lens, 2, 2, 64, t, 64, 64, 2, 5, scale=3.0)
+    window_check(got, qkv, lens, 2, 2, 64, 64, 2, t != torch.float32)
+
+
+def test_attention_window_unbounded_is_full_attention(dev):
+    """The framework's own full and causal attention are the window's limits."""
+    ops, lens = _ops(), [130, 64, 1, 300]
+    qkv, got = run_window(dev, lens, 4, 4, 64, torch.float32, 10 ** 6, 10 ** 6, 0, 11, extra=0)
+    cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32).to(dev)
+    # both f32: scores differ by the order of 64 products
+    assert (ops.attention(qkv, cu, 4, 300) - got).abs().max() <= 2e-5
+    _, causal = run_window(dev, lens, 4, 4, 64, torch.float32, 10 ** 6, 0, 0, 11, extra=0)
+    assert (ops.attention(qkv, cu, 4, 300, causal=True) - causal).abs().max() <= 2e-5
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_attention_window_leaves_other_rows(dev, dt):
+    """ctx rows behind the last sequence keep their bytes; NaN in keys that the window hides does
+    not reach the output."""
+    from jammi_b200 import _lib as L
+    t, g = DTYPES[dt], _gen(2)
+    n, h, d = 400, 2, 64
+    qkv = torch.randn((n + 70, 3 * h * d), generator=g, device=dev).to(t)
+    clean = qkv.clone()
+    qkv[:, h * d:][n:] = math.inf
+    qkv[5:100, h * d:] = math.nan  # hidden from queries >= 200 by a window of 64
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    ctx = torch.full((n + 70, h * d), 7.0, device=dev, dtype=t)
+    L.check(L.lib().jb_op_attention_window(qkv.data_ptr(), cu.data_ptr(), ctx.data_ptr(), L.DT_BF16 if dt == "bf16" else
+                                           L.DT_F32, 1, h, h, d, n, n + 70, 64, 64, 2,
+                                           torch.cuda.current_stream().cuda_stream))
+    want = _ops().attention_window(clean, cu, h, n, 64, 64, sinks=2)
+    _ops().sync()
+    assert (ctx[n:] == 7.0).all()
+    assert torch.equal(ctx[200:n], want[200:n])
+    assert ctx[5:100].isnan().all()
+
+
+def test_attention_window_refusals(dev):
+    from jammi_b200 import _lib as L
+    from jammi_b200._lib import JbError
+    ops = _ops()
+    qkv, cu = torch.ones((10, 3 * 64), device=dev), torch.tensor([0, 10], dtype=torch.int32, device=dev)
+    for a in ((qkv.t(), cu, 1), (qkv.cpu(), cu, 1), (qkv, cu.cpu(), 1), (qkv, cu.long(), 1), (qkv, cu, 5), (qkv, cu, 0),
+              (qkv.double(), cu, 1), (qkv[0], cu, 1), (qkv, cu[:0], 1), (qkv, cu.reshape(1, 2), 1)):
+        with pytest.raises(ValueError):
+            ops.attention_window(*a, 10, 4, 4)
+    with pytest.raises(ValueError):
+        ops.attention_window(qkv, cu, 2, 10, 4, 4, kv_heads=3)
+    for kw in (dict(left=-1), dict(right=-1), dict(sinks=-2), dict(max_len=-1)):
+        a = dict(max_len=10, left=4, right=4, sinks=0) | kw
+        with pytest.raises(JbError) as e:
+            ops.attention_window(qkv, cu, 1, a["max_len"], a["left"], a["right"], sinks=a["sinks"])
+        assert e.value.status == L.ERR_INVALID
+    with pytest.raises(JbError):
+        ops.attention_window(torch.ones((4, 3 * 24), device=dev), cu, 1, 4, 1, 1)  # head_dim 24
+    assert ops.attention_window(qkv[:0], cu[:1], 1, 0, 4, 4).shape == (0, 64)

@@ -60,3 +60,14 @@ def test_mxfp4_scale_bytes():
     f = L.lib().jb_mxfp4_scale_bytes
     assert [f(1, 32), f(128, 128), f(129, 128), f(128, 160), f(0, 64), f(-1, 64)] == [512, 512, 1024, 1024, 0, 0]
     assert f(2 ** 31 - 1, 4096) == 2 ** 24 * 32 * 512
+
+
+@pytest.mark.parametrize("kw", [dict(batch=-1), dict(heads=0), dict(kv=0), dict(kv=3), dict(d=24), dict(d=256), dict(d=0),
+                                dict(max_len=-1), dict(rows=-1), dict(left=-1), dict(right=-5), dict(sinks=-1),
+                                dict(dtype=L.DT_S8), dict(qkv=None), dict(cu=None), dict(ctx=None), dict(qkv=P + 2),
+                                dict(ctx=P + 8), dict(heads=2 ** 22, kv=2 ** 21)])
+def test_attention_window_refuses(kw):
+    a = dict(qkv=P, cu=P, ctx=P, dtype=L.DT_BF16, batch=2, heads=4, kv=2, d=64, max_len=16, rows=32, left=4, right=4,
+             sinks=0) | kw
+    refused(L.lib().jb_op_attention_window, a["qkv"], a["cu"], a["ctx"], a["dtype"], a["batch"], a["heads"], a["kv"],
+            a["d"], a["max_len"], a["rows"], a["left"], a["right"], a["sinks"], None)
