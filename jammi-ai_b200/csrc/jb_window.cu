@@ -13,7 +13,12 @@
 // qkv [T, (heads + 2 kv_heads) * d]: the query heads, then the key heads, then
 // the value heads of a token; query head h reads key / value head
 // h / (heads / kv_heads).
+#include <cudaTypedefs.h>
+
 #include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <type_traits>
 
 #include "jb_common.cuh"
 #include "jb_internal.h"
@@ -26,6 +31,7 @@ struct WinParams {
   const int* cu;
   void* ctx;
   int heads, kv_heads;
+  int rows;      // rows that qkv and ctx hold
   int q_blocks;  // query blocks of the longest row
   int left, right, sinks;
   float scale_log2;
@@ -55,9 +61,9 @@ __global__ void __launch_bounds__(kSimtThreads) window_simt_kernel(WinParams p) 
   __shared__ __align__(16) float Vs[kSimtKeys][D];
   const int qb = blockIdx.x % p.q_blocks;
   const int h = blockIdx.x / p.q_blocks % p.heads, b = blockIdx.x / p.q_blocks / p.heads;
-  const int start = p.cu[b], n = p.cu[b + 1] - start;
+  const int start = p.cu[b], n = min(p.cu[b + 1], p.rows) - start;  // never past the buffers
   const int q0 = qb * C::QUERIES;
-  if (q0 >= n) return;
+  if (start < 0 || q0 >= n) return;
   const int hk = h / (p.heads / p.kv_heads);
   const int ld = (p.heads + 2 * p.kv_heads) * D;
   const T* row = static_cast<const T*>(p.qkv) + static_cast<size_t>(start) * ld;
@@ -204,6 +210,547 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
   }
 }
 
+// ── tcgen05, 16-bit rows with head_dim 64 or 128 ────────────────────────────
+// A persistent CTA per SM runs two independent slots, each on its own items
+// (row, head, kQ-query block) with its own shared memory and half of TMEM:
+//   TMA warp      finds the slot's next items (32 candidates a time, one per
+//                 lane), publishes each in a two-entry ring and loads its Q
+//                 and then, per key block, K and V.
+//   MMA warp      S = Q K^T (M = 128, N = the block's keys) into columns
+//                 [0, N), then O (+)= P V with P read from TMEM.
+//   4 softmax     one thread per query row.  Two passes over the scores in
+//   warps         TMEM (maximum; exponentials and sum), 32 keys at a time; a
+//                 warp skips the 32-key pieces that none of its 32 queries
+//                 sees.  P (16-bit pairs) overwrites the scores that the same
+//                 thread has read: keys [16 c, 16 c + 16) go to columns
+//                 [8 c, 8 c + 8).  O / sum is stored after the last block.
+// The keys of an item are its window [k_begin, k_end), padded to 16, then the
+// first keys [0, s_end) that the window has left behind, padded to 16.  With
+// head_dim 64, an item of up to 256 keys is ONE block: no running maximum, no
+// rescaling, three hand-overs in all (S, P, O), and O takes columns
+// [128, 192) once every score is read.  That covers windows of up to
+// left + right = 128 around 128 queries (and 112 queries with up to 16 sinks),
+// the case this operator is for.  Longer ranges go in blocks of 128 keys with
+// a lazily rescaled running maximum (raised only by more than 2^8).
+//
+// A masked value contributes 0 * v, which is not 0 when v is not finite.  V
+// rows behind the item's last key are zeroed in shared memory; for the rest
+// an output that is not finite is computed again, by its thread, over the
+// visible keys only (window_row_exact).
+//
+// Every wait is bounded; on a timeout each role stops, copies and MMAs in
+// flight are waited for (bounded), the error flag is set and TMEM is freed.
+constexpr int kTcThreads = 384;  // 2 TMA, 2 MMA, 8 softmax warps
+constexpr float kRescale = 8.f;  // lazy-rescaling threshold, log2 units
+
+template <int D>
+struct TcCfg {
+  static constexpr int HALVES = D / 64;                    // 64-element column blocks (128 bytes)
+  static constexpr int KEYS = D == 64 ? 256 : 128;         // key rows of a K or V buffer
+  static constexpr int Q_BYTES = HALVES * 128 * 128;
+  static constexpr int KV_BYTES = HALVES * KEYS * 128;
+  static constexpr int SLOT_BYTES = Q_BYTES + 2 * KV_BYTES;
+  static constexpr int META_BYTES = 512;
+  static constexpr int SMEM = 1024 + 2 * SLOT_BYTES + META_BYTES;
+  static constexpr int O_COL = 128;
+};
+
+struct TcItem {
+  int live, start, n, h, q0, k_begin, nw, s_end, nb;
+};
+struct TcParams {
+  WinParams w;
+  long long items;  // batch * q_blocks * heads
+  int kq;           // queries per item
+  int* err;
+};
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+template <bool H16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (H16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__host__ __device__ constexpr int ceil16(int v) { return (v + 15) & ~15; }
+// bits [0, c) of 32, c clamped to 0 .. 32
+__device__ __forceinline__ uint32_t low_bits(int c) {
+  return c <= 0 ? 0u : c >= 32 ? 0xffffffffu : (1u << c) - 1u;
+}
+
+// One query row over its visible keys only, in f32 from global memory: the
+// rows whose tensor-core output is not finite.
+template <typename T, int D>
+__device__ __noinline__ void window_row_exact(const WinParams& p, int start, int n, int h, int qi) {
+  const int ld = (p.heads + 2 * p.kv_heads) * D;
+  const T* row = static_cast<const T*>(p.qkv) + static_cast<size_t>(start) * ld;
+  const T* q = row + static_cast<size_t>(qi) * ld + h * D;
+  const T* k = row + (p.heads + h / (p.heads / p.kv_heads)) * D;
+  const T* v = k + p.kv_heads * D;
+  T* out = static_cast<T*>(p.ctx) + (static_cast<size_t>(start + qi) * p.heads + h) * D;
+  const int lo = qi - min(p.left, qi), hi = qi + min(p.right, n - 1 - qi);
+  const int behind = min(p.sinks, lo);  // sinks in front of the window
+  auto score = [&](int j) {
+    float s = 0.f;
+    for (int d = 0; d < D; ++d) s = fmaf(to_f(q[d]), to_f(k[static_cast<size_t>(j) * ld + d]), s);
+    return s * p.scale_log2;
+  };
+  float m = -INFINITY, l = 0.f;
+  for (int j = behind > 0 ? 0 : lo; j <= hi; j = j + 1 == behind ? lo : j + 1) m = fmaxf(m, score(j));
+  if (m == -INFINITY) m = 0.f;
+  for (int c = 0; c < D; c += 16) {  // 16 output columns a pass
+    float o[16] = {};
+    l = 0.f;
+    for (int j = behind > 0 ? 0 : lo; j <= hi; j = j + 1 == behind ? lo : j + 1) {
+      const float e = exp2f(score(j) - m);
+      l += e;
+      for (int d = 0; d < 16; ++d) o[d] = fmaf(e, to_f(v[static_cast<size_t>(j) * ld + c + d]), o[d]);
+    }
+    for (int d = 0; d < 16; ++d) out[c + d] = from_f<T>(o[d] / l);
+  }
+}
+
+template <int D, bool H16>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    window_tc_kernel(const TcParams p, const __grid_constant__ CUtensorMap tm64,
+                     const __grid_constant__ CUtensorMap tm16) {
+  using C = TcCfg<D>;
+  using T = typename std::conditional<H16, f16, bf16>::type;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* meta = smem_raw + (base + 2 * C::SLOT_BYTES - raw);
+  const int g = warp < 4 ? warp & 1 : (warp - 4) >> 2;  // this warp's slot
+  const uint32_t sQ = base + g * C::SLOT_BYTES, sK = sQ + C::Q_BYTES, sV = sK + C::KV_BYTES;
+  const uint32_t bars = smem_u32(meta) + g * 96;
+  const uint32_t ifull = bars;         // [2] an item is published
+  const uint32_t kfull = bars + 16;    // K (and Q) of a block loaded
+  const uint32_t vfull = bars + 24;
+  const uint32_t sfull = bars + 32;    // S written: K (and Q) read
+  const uint32_t pfull = bars + 40;    // P written
+  const uint32_t ofull = bars + 48;    // P V done: V read
+  const uint32_t sfree = bars + 56;    // O read: the slot's TMEM is free
+  const uint32_t spare = bars + 64;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(meta + 192);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 196);
+  volatile TcItem* ring = reinterpret_cast<volatile TcItem*>(meta + 256) + 2 * g;
+  static_assert(256 + 4 * sizeof(TcItem) <= C::META_BYTES, "meta layout");
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t b = smem_u32(meta) + s * 96;
+      for (int i = 0; i < 5; ++i) mbar_init(b + 8 * i, 1);
+      mbar_init(b + 40, 4);
+      mbar_init(b + 48, 1);
+      mbar_init(b + 56, 4);
+      mbar_init(b + 64, 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc(smem_u32(tslot), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot + static_cast<uint32_t>(g) * 256;
+  const WinParams& w = p.w;
+  // keys of block j of an item, in its own order: window, then sinks
+  auto block_of = [&](int nv, int nb, int j, int& v0, int& v1) {
+    v0 = nb == 1 ? 0 : 128 * j;
+    v1 = nb == 1 ? nv : min(nv, v0 + 128);
+  };
+
+  if (warp < 2) {  // ── TMA
+    const long long stride = 2ll * gridDim.x;
+    int bc = 0, m = 0;  // blocks loaded, items published
+    bool ok = true;
+    const int hk_div = w.heads / w.kv_heads;
+    for (long long f0 = static_cast<long long>(g) * gridDim.x + blockIdx.x; f0 < p.items && ok; f0 += 32 * stride) {
+      const long long f = f0 + lane * stride;
+      int start = 0, n = 0, h = 0, q0 = 0;
+      if (f < p.items) {
+        h = static_cast<int>(f % w.heads);
+        const long long bq = f / w.heads;
+        const int b = static_cast<int>(bq / w.q_blocks);
+        q0 = static_cast<int>(bq % w.q_blocks) * p.kq;
+        start = w.cu[b];
+        n = min(w.cu[b + 1], w.rows) - start;  // never past the buffers
+      }
+      unsigned todo = __ballot_sync(0xffffffffu, f < p.items && start >= 0 && q0 < n);
+      while (todo && ok) {
+        const int src = __ffs(todo) - 1;
+        todo &= todo - 1;
+        TcItem it;
+        it.live = 1;
+        it.start = __shfl_sync(0xffffffffu, start, src);
+        it.n = __shfl_sync(0xffffffffu, n, src);
+        it.h = __shfl_sync(0xffffffffu, h, src);
+        it.q0 = __shfl_sync(0xffffffffu, q0, src);
+        if (lane == 0) {
+          const int q_last = min(it.n, it.q0 + p.kq) - 1;
+          const int k_end = q_last + min(w.right, it.n - 1 - q_last) + 1;
+          it.k_begin = it.q0 - min(w.left, it.q0);
+          // no gap between sinks and window, or a row short enough to read whole
+          if (w.sinks >= it.k_begin || (w.sinks > 0 && k_end <= C::KEYS)) it.k_begin = 0;
+          it.s_end = min(w.sinks, it.k_begin);
+          it.nw = k_end - it.k_begin;
+          const int nv = ceil16(it.nw) + ceil16(it.s_end);
+          it.nb = nv <= C::KEYS ? 1 : (nv + 127) / 128;
+          const int xk = (w.heads + it.h / hk_div) * D, xv = xk + w.kv_heads * D;
+          for (int j = 0; j < it.nb; ++j, ++bc) {
+            int v0, v1;
+            block_of(nv, it.nb, j, v0, v1);
+            auto load_keys = [&](uint32_t dst, int x, uint32_t bar) {
+              int v = v0;
+              while (v < v1) {
+                const bool win = v < ceil16(it.nw);
+                const int stop = win ? min(v1, ceil16(it.nw)) : v1;
+                const int key = win ? it.k_begin + v : v - ceil16(it.nw);
+                const bool big = stop - v >= 64;
+                for (int half = 0; half < C::HALVES; ++half)
+                  tma_load_2d(dst + half * (C::KEYS * 128) + (v - v0) * 128, big ? &tm64 : &tm16, x + 64 * half,
+                              it.start + key, bar);
+                v += big ? 64 : 16;
+              }
+            };
+            if (bc > 0 && !mbar_wait(sfull, (bc - 1) & 1, abort_flag)) { ok = false; break; }
+            uint32_t bytes = static_cast<uint32_t>(v1 - v0) * 128 * C::HALVES;
+            if (j == 0) {
+              volatile TcItem& e = ring[m & 1];
+              e.live = 1; e.start = it.start; e.n = it.n; e.h = it.h; e.q0 = it.q0;
+              e.k_begin = it.k_begin; e.nw = it.nw; e.s_end = it.s_end; e.nb = it.nb;
+              mbar_arrive(ifull + 8 * (m & 1));
+              ++m;
+              const int boxes = (min(it.n - it.q0, p.kq) + 63) >> 6;
+              mbar_arrive_expect_tx(kfull, bytes + boxes * 64 * 128 * C::HALVES);
+              for (int i = 0; i < boxes; ++i)
+                for (int half = 0; half < C::HALVES; ++half)
+                  tma_load_2d(sQ + half * (128 * 128) + i * (64 * 128), &tm64, it.h * D + 64 * half,
+                              it.start + it.q0 + 64 * i, kfull);
+            } else {
+              mbar_arrive_expect_tx(kfull, bytes);
+            }
+            load_keys(sK, xk, kfull);
+            if (bc > 0 && !mbar_wait(ofull, (bc - 1) & 1, abort_flag)) {
+              volatile int no_abort = 0;
+              mbar_wait(kfull, bc & 1, &no_abort);  // this block's copies land (bounded)
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(vfull, bytes);
+            load_keys(sV, xv, vfull);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      }
+    }
+    if (lane == 0) {
+      if (ok && (bc == 0 || mbar_wait(sfull, (bc - 1) & 1, abort_flag))) {  // no more items
+        ring[m & 1].live = 0;
+        mbar_arrive(ifull + 8 * (m & 1));
+        mbar_arrive(kfull);
+      }
+      if (*abort_flag && bc > 0) {  // the last copies land before the CTA leaves (bounded)
+        volatile int no_abort = 0;
+        mbar_wait(kfull, (bc - 1) & 1, &no_abort);
+        mbar_wait(vfull, (bc - 1) & 1, &no_abort);
+      }
+    }
+  } else if (warp < 4) {
+    if (lane == 0) {  // ── MMA
+      const uint32_t idesc_pv = (H16 ? idesc_f16_f32(128, 64) : idesc_bf16_f32(128, 64)) | (1u << 16);  // V MN-major
+      int bc = 0;
+      bool ok = true;
+      for (int m = 0; ok; ++m) {
+        if (!mbar_wait(kfull, bc & 1, abort_flag)) { ok = false; break; }
+        const volatile TcItem& e = ring[m & 1];
+        if (!e.live) break;
+        const int nv = ceil16(e.nw) + ceil16(e.s_end), nb = e.nb;
+        if (m > 0 && !mbar_wait(sfree, (m - 1) & 1, abort_flag)) { ok = false; break; }
+        for (int j = 0; j < nb; ++j, ++bc) {
+          int v0, v1;
+          block_of(nv, nb, j, v0, v1);
+          // S_j replaces P_{j-1}, which P V has read
+          if (j > 0 && (!mbar_wait(kfull, bc & 1, abort_flag) || !mbar_wait(ofull, (bc - 1) & 1, abort_flag))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t idesc = H16 ? idesc_f16_f32(128, v1 - v0) : idesc_bf16_f32(128, v1 - v0);
+#pragma unroll
+          for (int half = 0; half < C::HALVES; ++half) {
+            const uint64_t dq = umma_desc_sw128(sQ + half * (128 * 128));
+            const uint64_t dk = umma_desc_sw128(sK + half * (C::KEYS * 128));
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem, dq + 2u * kk, dk + 2u * kk, idesc, (half | kk) != 0);
+          }
+          mma_commit(sfull);
+          if (!mbar_wait(pfull, bc & 1, abort_flag) || !mbar_wait(vfull, bc & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < (v1 - v0) >> 4; ++c) {
+#pragma unroll
+            for (int half = 0; half < C::HALVES; ++half)
+              mma_bf16_ta(tmem + C::O_COL + 64 * half, tmem + 8u * c,
+                          umma_desc_sw128(sV + half * (C::KEYS * 128)) + 128u * c, idesc_pv, (j > 0 || c > 0) ? 1u : 0u);
+          }
+          mma_commit(ofull);
+        }
+      }
+      if (!ok) {  // every MMA issued completes before TMEM is freed (bounded)
+        volatile int no_abort = 0;
+        mma_commit(spare);
+        mbar_wait(spare, 0, &no_abort);
+      }
+    }
+  } else {  // ── softmax
+    const int quarter = warp & 3;
+    const int r = 32 * quarter + lane;
+    const uint32_t trow = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    int bc = 0;
+    bool ok = true;
+    for (int m = 0; ok; ++m) {
+      if (!warp_wait(ifull + 8 * (m & 1), (m >> 1) & 1, abort_flag)) break;
+      const volatile TcItem& e = ring[m & 1];
+      if (!e.live) break;
+      const int start = e.start, n = e.n, h = e.h, q0 = e.q0, k_begin = e.k_begin, nw = e.nw, s_end = e.s_end,
+                nb = e.nb;
+      const int nw16 = ceil16(nw), nv = nw16 + ceil16(s_end);
+      const int qi = q0 + r;
+      const bool mine = r < p.kq && qi < n;
+      const bool active = __any_sync(0xffffffffu, mine);
+      // visible keys of this row, relative to k_begin
+      const int lo = qi - min(w.left, qi) - k_begin;
+      const int hi = mine ? qi + min(w.right, n - 1 - qi) - k_begin : -1;
+      const int first = min(w.sinks - k_begin, hi + 1);  // sinks inside the window's range
+      auto visible = [&](int v) -> uint32_t {  // keys [v, v + 32) of the item's order
+        uint32_t bits = 0;
+        if (v < nw16) bits = (low_bits(hi + 1 - v) & ~low_bits(lo - v)) | low_bits(first - v);
+        if (v + 32 > nw16 && s_end > 0 && mine) {
+          const int c = nw16 - v;  // the sinks' first bit
+          bits |= c >= 0 ? low_bits(s_end) << c : low_bits(s_end + c);
+        }
+        return bits;
+      };
+      float mref = -INFINITY, l = 0.f;
+      for (int j = 0; j < nb; ++j, ++bc) {
+        int v0, v1;
+        block_of(nv, nb, j, v0, v1);
+        if (!warp_wait(sfull, bc & 1, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        if (active) {
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < v1 - v0; c += 32) {
+            uint32_t bits = visible(v0 + c);
+            if (!__any_sync(0xffffffffu, bits != 0)) continue;
+            uint32_t s[32];
+            tmem_ld_32x32b_x32(trow + c, s);
+            tmem_wait_ld();
+            if (__all_sync(0xffffffffu, bits == 0xffffffffu)) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2)
+                mx = fmaxf(mx, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (bits >> i & 1) mx = fmaxf(mx, __uint_as_float(s[i]));
+            }
+          }
+          const float mb = mx * w.scale_log2;
+          if (j == 0) {
+            mref = mb == -INFINITY ? 0.f : mb;  // nothing visible yet: p stays 0
+          } else {
+            const bool up = mb > mref + kRescale;
+            if (__any_sync(0xffffffffu, up)) {
+              const float alpha = up ? ex2_approx(mref - mb) : 1.f;
+              l *= alpha;
+#pragma unroll 1
+              for (int c = 0; c < D; c += 8) {
+                uint32_t o8[8];
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(o8[0]), "=r"(o8[1]), "=r"(o8[2]), "=r"(o8[3]), "=r"(o8[4]), "=r"(o8[5]),
+                               "=r"(o8[6]), "=r"(o8[7])
+                             : "r"(trow + C::O_COL + c));
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o8[i] = __float_as_uint(__uint_as_float(o8[i]) * alpha);
+                tmem_st_32x32b_x8(trow + C::O_COL + c, o8);
+              }
+              tmem_wait_st();
+              if (up) mref = mb;
+            }
+          }
+          float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+          for (int c = 0; c < v1 - v0; c += 32) {
+            const uint32_t bits = visible(v0 + c);
+            uint32_t pk[16];
+            if (!__any_sync(0xffffffffu, bits != 0)) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = 0;
+            } else {
+              uint32_t s[32];
+              tmem_ld_32x32b_x32(trow + c, s);
+              tmem_wait_ld();
+              const bool full = __all_sync(0xffffffffu, bits == 0xffffffffu);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float2 z = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
+                                      f2(w.scale_log2), f2(-mref));
+                if (!full) {
+                  if (!(bits >> i & 1)) z.x = -INFINITY;
+                  if (!(bits >> (i + 1) & 1)) z.y = -INFINITY;
+                }
+                const float p0 = ex2_approx(z.x), p1 = ex2_approx(z.y);
+                l0 += p0;
+                l1 += p1;
+                pk[i >> 1] = pack16<H16>(p0, p1);
+              }
+            }
+            tmem_st_32x32b_x16(trow + (c >> 1), pk);
+          }
+          l += l0 + l1;
+          tmem_wait_st();
+        }
+        // V rows [nw, nw16) belong to no key of the item: their product with
+        // P = 0 must be 0
+        if (nw16 > nw && nw16 > v0 && nw16 <= v1) {
+          if (!warp_wait(vfull, bc & 1, abort_flag)) { ok = false; break; }
+          for (int i = r; i < (nw16 - nw) * 8 * C::HALVES; i += 128) {
+            const int row = i >> 3, half = row / (nw16 - nw);
+            const uint32_t a = sV + half * (C::KEYS * 128) +
+                               static_cast<uint32_t>(nw - v0 + row - half * (nw16 - nw)) * 128 + (i & 7) * 16;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory");
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pfull);
+      }
+      if (!ok) break;
+      if (!warp_wait(ofull, (bc - 1) & 1, abort_flag)) break;
+      tc_fence_after();
+      const float inv = 1.f / l;
+      T* out = static_cast<T*>(w.ctx) + (static_cast<size_t>(start + (mine ? qi : 0)) * w.heads + h) * D;
+      bool finite = true;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (active) {
+          tmem_ld_32x32b_x32(trow + C::O_COL + c, o);
+          tmem_wait_ld();
+        }
+        if (c + 32 == D) {  // the slot's TMEM may be overwritten
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sfree);
+        }
+        if (mine) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              v[i] = __uint_as_float(o[8 * q + i]) * inv;
+              finite = finite && fabsf(v[i]) < INFINITY;
+            }
+            *reinterpret_cast<uint4*>(out + c + 8 * q) =
+                make_uint4(pack16<H16>(v[0], v[1]), pack16<H16>(v[2], v[3]), pack16<H16>(v[4], v[5]),
+                           pack16<H16>(v[6], v[7]));
+          }
+        }
+      }
+      if (mine && !finite) window_row_exact<T, D>(w, start, n, h, qi);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && p.err) atomicOr(p.err, kErrTimeout);
+  if (warp == 2) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(*tslot, 512);
+  }
+}
+
+// Map over qkv [rows, cols] of 16-bit elements with boxes of 64 columns (128
+// swizzled bytes) x box_rows.
+bool make_map(CUtensorMap* map, const void* qkv, bool h16, int rows, int cols, int box_rows) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  if (!enc) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(map, h16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(qkv),
+             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Queries per item: 128, or fewer where that keeps a long row's window and
+// sinks inside one 256-key block (head_dim 64).
+int queries_per_item(const WindowArgs& a) {
+  if (a.head_dim != 64 || a.sinks == 0 || a.max_len <= 256) return 128;
+  const long long spare = 256ll - a.left - a.right - ((a.sinks + 15ll) & ~15ll);
+  return spare >= 128 || spare < 64 ? 128 : static_cast<int>(spare) & ~15;
+}
+
+template <int D, bool H16>
+cudaError_t launch_tc(const WindowArgs& a, WinParams w, cudaStream_t s, std::string* why) {
+  CUtensorMap tm64, tm16;
+  const int cols = (a.heads + 2 * a.kv_heads) * D;
+  if (!make_map(&tm64, a.qkv, H16, a.rows, cols, 64) || !make_map(&tm16, a.qkv, H16, a.rows, cols, 16)) {
+    if (why) *why = "attention_window: cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  auto kern = window_tc_kernel<D, H16>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  // the shared-memory opt-in is a property of each device's context
+  static std::atomic<uint8_t> attr_set[64];
+  if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<D>::SMEM);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_set[dev].store(1, std::memory_order_release);
+  }
+  TcParams p;
+  p.kq = queries_per_item(a);
+  w.q_blocks = (a.max_len + p.kq - 1) / p.kq;
+  p.w = w;
+  p.items = static_cast<long long>(a.batch) * w.q_blocks * a.heads;
+  p.err = a.err;
+  const int grid = static_cast<int>(std::min<long long>(num_sms(dev), p.items));
+  kern<<<grid, kTcThreads, TcCfg<D>::SMEM, s>>>(p, tm64, tm16);
+  return cudaGetLastError();
+}
+
 }  // namespace
 
 cudaError_t launch_attention_window(const WindowArgs& a, cudaStream_t s, std::string* why) {
@@ -214,6 +761,7 @@ cudaError_t launch_attention_window(const WindowArgs& a, cudaStream_t s, std::st
   p.ctx = a.ctx;
   p.heads = a.heads;
   p.kv_heads = a.kv_heads;
+  p.rows = a.rows;
   p.q_blocks = 0;
   p.left = a.left;
   p.right = a.right;
@@ -221,8 +769,14 @@ cudaError_t launch_attention_window(const WindowArgs& a, cudaStream_t s, std::st
   p.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(a.head_dim));
   switch (a.dtype) {
     case JB_DT_F32: return launch_simt<float>(p, a.head_dim, a.batch, a.max_len, s, why);
-    case JB_DT_BF16: return launch_simt<bf16>(p, a.head_dim, a.batch, a.max_len, s, why);
-    case JB_DT_F16: return launch_simt<f16>(p, a.head_dim, a.batch, a.max_len, s, why);
+    case JB_DT_BF16:
+      if (a.head_dim == 64) return launch_tc<64, false>(a, p, s, why);
+      if (a.head_dim == 128) return launch_tc<128, false>(a, p, s, why);
+      return launch_simt<bf16>(p, a.head_dim, a.batch, a.max_len, s, why);
+    case JB_DT_F16:
+      if (a.head_dim == 64) return launch_tc<64, true>(a, p, s, why);
+      if (a.head_dim == 128) return launch_tc<128, true>(a, p, s, why);
+      return launch_simt<f16>(p, a.head_dim, a.batch, a.max_len, s, why);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -413,7 +413,7 @@ def window_ref(qkv, lens, h, hk, left, right, sinks):
     return out, mag, top
 
 
-def window_check(got, qkv, lens, h, hk, left, right, sinks, tensor_cores):
+def window_check(got, qkv, lens, h, hk, left, right, sinks, tensor_cores, first=0):
     """An output is sum p v / sum p.  Scores: d products and sums in f32, off by (d + 4) 2^-24 of
     sum |q k| / sqrt(d) =: top, so p is off by that share (and 2^-21 for the exponential and its
     argument's rounding at |argument| <= 2 top log2 e).  On tensor cores each p is also rounded to
@@ -425,8 +425,9 @@ def window_check(got, qkv, lens, h, hk, left, right, sinks, tensor_cores):
     share = 2 * ((d + 8) * 2.0 ** -24 * top + 2.0 ** -21) + max(lens, default=0) * 2.0 ** -23 + (u if tensor_cores else 0)
     T = sum(lens)
     err = (got.double() - ref)[:T].abs()
+    assert got.dtype == qkv.dtype and got.shape == ref.shape
     bound = share * mag[:T] + u * (ref[:T].abs() + share * mag[:T]) + torch.finfo(qkv.dtype).smallest_normal * 2 * u
-    assert (err <= bound).all(), (err / bound).max().item()
+    assert (err <= bound)[first:].all(), (err / bound)[first:].max().item()
 
 
 WINDOWS = [(64, 64, 0), (64, 64, 1), (0, 0, 0), (0, 0, 3), (128, 0, 0), (255, 0, 4), (17, 200, 5), (300, 5, 130),
@@ -497,10 +498,16 @@ def test_attention_window_leaves_other_rows(dev, dt):
     L.check(L.lib().jb_op_attention_window(qkv.data_ptr(), cu.data_ptr(), ctx.data_ptr(), L.DT_BF16 if dt == "bf16" else
                                            L.DT_F32, 1, h, h, d, n, n + 70, 64, 64, 2,
                                            torch.cuda.current_stream().cuda_stream))
-    want = _ops().attention_window(clean, cu, h, n, 64, 64, sinks=2)
     _ops().sync()
     assert (ctx[n:] == 7.0).all()
-    assert torch.equal(ctx[200:n], want[200:n])
+    # the hidden keys may be anything: the float64 reference of the clean rows
+    # is the value for queries 200 and up.  Rows that share a block of queries
+    # with NaN keys are computed again with unrounded p, the others with p
+    # rounded to 16 bits: two values, each inside the bound, which counts that
+    # rounding once (so bits cannot be compared)
+    clean[n:] = 0
+    full = torch.where(torch.arange(n + 70, device=dev)[:, None] < n, ctx, torch.zeros_like(ctx))
+    window_check(full, clean, [n], h, h, 64, 64, 2, dt == "bf16", first=200)
     assert ctx[5:100].isnan().all()
 
 
