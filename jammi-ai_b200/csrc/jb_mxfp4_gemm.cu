@@ -230,64 +230,68 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    if (lane == 0) {  // ── producer
-      const int w_tiles = (p.N + 127) / 128;  // scale tiles along N
-      int it = 0;  // stages filled
-      bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const int mb = t / n_tiles, nb = t % n_tiles;
-        const int wt = nb * BN / 128;
-        for (int kb = 0; kb < kb_count; ++kb, ++it) {
-          const int st = it % Cfg::STAGES;
-          if (!mbar_wait(empty_bar(st), ((it / Cfg::STAGES) & 1) ^ 1u, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
-          const uint32_t sf = scales + st * Cfg::SF_BYTES;
-          const uint32_t sf_bytes = min(2, k_tiles - 2 * kb) * kSfTile;
-          const int w_copies = min(Cfg::SFB_TILES, w_tiles - wt);
+  // The producer and the issuer walk their loops as whole warps and elect one
+  // lane around each stage's group of instructions: the operands stay in
+  // uniform registers.  (Loops inside `if (lane == 0)` issue one product per
+  // about 250 clocks whatever its width, against the 96 that a 192-column
+  // product of K = 64 takes.)
+  if (warp == 0) {  // ── producer
+    const int w_tiles = (p.N + 127) / 128;  // scale tiles along N
+    int it = 0;  // stages filled
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      const int mb = t / n_tiles, nb = t % n_tiles;
+      const int wt = nb * BN / 128;
+      const int w_copies = min(Cfg::SFB_TILES, w_tiles - wt);
+      const uint8_t* sfa_src = p.a_scale + static_cast<size_t>(mb) * k_tiles * kSfTile;
+      const uint8_t* sfb_src = p.w_scale + static_cast<size_t>(wt) * k_tiles * kSfTile;
+      for (int kb = 0; kb < kb_count; ++kb, ++it) {
+        const int st = it % Cfg::STAGES;
+        ok = warp_wait(empty_bar(st), ((it / Cfg::STAGES) & 1) ^ 1u, abort_flag);
+        if (!ok) break;
+        const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
+        const uint32_t sf = scales + st * Cfg::SF_BYTES;
+        const uint32_t sf_bytes = min(2, k_tiles - 2 * kb) * kSfTile;
+        if (elect_one()) {
           mbar_arrive_expect_tx(full_bar(st), Cfg::A_BYTES + Cfg::B_BYTES + sf_bytes * (1 + w_copies));
           tma_load_2d(sa, &tmA, kb * 128, mb * kBM, full_bar(st));
           tma_load_2d(sa + Cfg::A_BYTES, &tmB, kb * 128, nb * BN, full_bar(st));
-          bulk_load(sf, p.a_scale + (static_cast<size_t>(mb) * k_tiles + 2 * kb) * kSfTile, sf_bytes, full_bar(st));
-          for (int i = 0; i < w_copies; ++i)
-            bulk_load(sf + 2 * kSfTile * (1 + i),
-                      p.w_scale + (static_cast<size_t>(wt + i) * k_tiles + 2 * kb) * kSfTile, sf_bytes, full_bar(st));
+          bulk_load(sf, sfa_src + 2 * kb * kSfTile, sf_bytes, full_bar(st));
+          bulk_load(sf + 2 * kSfTile, sfb_src + 2 * kb * kSfTile, sf_bytes, full_bar(st));
+          if (w_copies > 1)
+            bulk_load(sf + 4 * kSfTile, sfb_src + (k_tiles + 2 * kb) * static_cast<size_t>(kSfTile), sf_bytes,
+                      full_bar(st));
         }
-      }
-      if (!ok || *abort_flag) {  // copies in flight land before the CTA leaves (bounded)
-        volatile int no_abort = 0;
-        for (int b = max(0, it - Cfg::STAGES); b < it; ++b)
-          mbar_wait(full_bar(b % Cfg::STAGES), (b / Cfg::STAGES) & 1, &no_abort);
+        __syncwarp();
       }
     }
-  } else if (warp == 1) {
-    if (lane == 0) {  // ── MMA issuer
-      int it = 0, acc = 0;
-      uint32_t acc_ph = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const uint32_t sf_shift = static_cast<uint32_t>((t % n_tiles) * BN % 128) / 32;
-        if (!mbar_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag)) {
-          ok = false;
-          break;
-        }
+    if (*abort_flag) {  // copies in flight land before the CTA leaves (bounded)
+      volatile int no_abort = 0;
+      for (int b = max(0, it - Cfg::STAGES); b < it; ++b)
+        mbar_wait(full_bar(b % Cfg::STAGES), (b / Cfg::STAGES) & 1, &no_abort);
+    }
+  } else if (warp == 1) {  // ── MMA issuer
+    int it = 0, acc = 0;
+    uint32_t acc_ph = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      const uint32_t sf_shift = static_cast<uint32_t>((t % n_tiles) * BN % 128) / 32;
+      ok = warp_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+      for (int kb = 0; kb < kb_count; ++kb, ++it) {
+        const int st = it % Cfg::STAGES;
+        ok = warp_wait(full_bar(st), (it / Cfg::STAGES) & 1, abort_flag);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-        for (int kb = 0; kb < kb_count; ++kb, ++it) {
-          const int st = it % Cfg::STAGES;
-          if (!mbar_wait(full_bar(st), (it / Cfg::STAGES) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
-          const uint32_t sf = scales + st * Cfg::SF_BYTES;
-          const uint32_t tsa = tmem_base + 2 * BN + st * Cfg::SF_COLS;  // [2 K tiles][4]
-          const uint32_t tsb = tsa + 8;                                 // [2 K tiles][SFB_TILES][4]
-          const int k_left = p.K - kb * kStageK;
+        const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
+        const uint32_t sf = scales + st * Cfg::SF_BYTES;
+        const uint32_t tsa = tmem_base + 2 * BN + st * Cfg::SF_COLS;  // [2 K tiles][4]
+        const uint32_t tsb = tsa + 8;                                 // [2 K tiles][SFB_TILES][4]
+        const int k_left = p.K - kb * kStageK;
+        const uint64_t da = umma_desc_sw128(sa), db = umma_desc_sw128(sa + Cfg::A_BYTES);
+        if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             if (c * 128 < k_left) {
@@ -297,7 +301,6 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
                 tmem_cp_scales(tsb + 4 * (c * Cfg::SFB_TILES + i), scale_desc(sf + (2 * (1 + i) + c) * kSfTile));
             }
           }
-          const uint64_t da = umma_desc_sw128(sa), db = umma_desc_sw128(sa + Cfg::A_BYTES);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             if (k * 64 < k_left)
@@ -305,17 +308,18 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
                        tsb + 4 * Cfg::SFB_TILES * (k >> 1) + sf_shift, (kb | k) != 0);
           }
           mma_commit(empty_bar(st));
+          if (kb == kb_count - 1) mma_commit(tfull_bar(acc));
         }
-        if (!ok) break;
-        mma_commit(tfull_bar(acc));
-        acc ^= 1;
-        if (acc == 0) acc_ph ^= 1u;
+        __syncwarp();
       }
-      if (!ok) {  // every MMA issued completes before TMEM is freed (bounded)
-        volatile int no_abort = 0;
-        mma_commit(spare);
-        mbar_wait(spare, 0, &no_abort);
-      }
+      acc ^= 1;
+      if (acc == 0) acc_ph ^= 1u;
+    }
+    if (!ok) {  // every MMA issued completes before TMEM is freed (bounded)
+      volatile int no_abort = 0;
+      if (elect_one()) mma_commit(spare);
+      __syncwarp();
+      warp_wait(spare, 0, &no_abort);
     }
   } else {  // ── epilogue
     const int w = warp - 2;

@@ -401,44 +401,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         it.n = __shfl_sync(0xffffffffu, n, src);
         it.h = __shfl_sync(0xffffffffu, h, src);
         it.q0 = __shfl_sync(0xffffffffu, q0, src);
-        if (lane == 0) {
-          const int q_last = min(it.n, it.q0 + p.kq) - 1;
-          const int k_end = q_last + min(w.right, it.n - 1 - q_last) + 1;
-          it.k_begin = it.q0 - min(w.left, it.q0);
-          // no gap between sinks and window, or a row short enough to read whole
-          if (w.sinks >= it.k_begin || (w.sinks > 0 && k_end <= C::KEYS)) it.k_begin = 0;
-          it.s_end = min(w.sinks, it.k_begin);
-          it.nw = k_end - it.k_begin;
-          const int nv = ceil16(it.nw) + ceil16(it.s_end);
-          it.nb = nv <= C::KEYS ? 1 : (nv + 127) / 128;
-          const int xk = (w.heads + it.h / hk_div) * D, xv = xk + w.kv_heads * D;
-          for (int j = 0; j < it.nb; ++j, ++bc) {
-            int v0, v1;
-            block_of(nv, it.nb, j, v0, v1);
-            auto load_keys = [&](uint32_t dst, int x, uint32_t bar) {
-              int v = v0;
-              while (v < v1) {
-                const bool win = v < ceil16(it.nw);
-                const int stop = win ? min(v1, ceil16(it.nw)) : v1;
-                const int key = win ? it.k_begin + v : v - ceil16(it.nw);
-                const bool big = stop - v >= 64;
-                for (int half = 0; half < C::HALVES; ++half)
-                  tma_load_2d(dst + half * (C::KEYS * 128) + (v - v0) * 128, big ? &tm64 : &tm16, x + 64 * half,
-                              it.start + key, bar);
-                v += big ? 64 : 16;
-              }
-            };
-            if (bc > 0 && !mbar_wait(sfull, (bc - 1) & 1, abort_flag)) { ok = false; break; }
-            uint32_t bytes = static_cast<uint32_t>(v1 - v0) * 128 * C::HALVES;
+        const int q_last = min(it.n, it.q0 + p.kq) - 1;
+        const int k_end = q_last + min(w.right, it.n - 1 - q_last) + 1;
+        it.k_begin = it.q0 - min(w.left, it.q0);
+        // no gap between sinks and window, or a row short enough to read whole
+        if (w.sinks >= it.k_begin || (w.sinks > 0 && k_end <= C::KEYS)) it.k_begin = 0;
+        it.s_end = min(w.sinks, it.k_begin);
+        it.nw = k_end - it.k_begin;
+        const int nw16 = ceil16(it.nw), nv = nw16 + ceil16(it.s_end);
+        it.nb = nv <= C::KEYS ? 1 : (nv + 127) / 128;
+        const int xk = (w.heads + it.h / hk_div) * D, xv = xk + w.kv_heads * D;
+        for (int j = 0; j < it.nb; ++j, ++bc) {
+          int v0, v1;
+          block_of(nv, it.nb, j, v0, v1);
+          // window keys, then sinks, in boxes of 64 and 16 rows
+          auto load_keys = [&](uint32_t dst, int x, uint32_t bar) {
+            int v = v0;
+            while (v < v1) {
+              const bool win = v < nw16;
+              const int stop = win ? min(v1, nw16) : v1;
+              const int y = it.start + (win ? it.k_begin + v : v - nw16);
+              const bool big = stop - v >= 64;
+#pragma unroll
+              for (int half = 0; half < C::HALVES; ++half)
+                tma_load_2d(dst + half * (C::KEYS * 128) + (v - v0) * 128, big ? &tm64 : &tm16, x + 64 * half, y, bar);
+              v += big ? 64 : 16;
+            }
+          };
+          if (bc > 0 && !warp_wait(sfull, (bc - 1) & 1, abort_flag)) { ok = false; break; }
+          const uint32_t bytes = static_cast<uint32_t>(v1 - v0) * 128 * C::HALVES;
+          const int boxes = (min(it.n - it.q0, p.kq) + 63) >> 6;
+          if (elect_one()) {
             if (j == 0) {
               volatile TcItem& e = ring[m & 1];
               e.live = 1; e.start = it.start; e.n = it.n; e.h = it.h; e.q0 = it.q0;
               e.k_begin = it.k_begin; e.nw = it.nw; e.s_end = it.s_end; e.nb = it.nb;
               mbar_arrive(ifull + 8 * (m & 1));
-              ++m;
-              const int boxes = (min(it.n - it.q0, p.kq) + 63) >> 6;
               mbar_arrive_expect_tx(kfull, bytes + boxes * 64 * 128 * C::HALVES);
               for (int i = 0; i < boxes; ++i)
+#pragma unroll
                 for (int half = 0; half < C::HALVES; ++half)
                   tma_load_2d(sQ + half * (128 * 128) + i * (64 * 128), &tm64, it.h * D + 64 * half,
                               it.start + it.q0 + 64 * i, kfull);
@@ -446,17 +447,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               mbar_arrive_expect_tx(kfull, bytes);
             }
             load_keys(sK, xk, kfull);
-            if (bc > 0 && !mbar_wait(ofull, (bc - 1) & 1, abort_flag)) {
-              volatile int no_abort = 0;
-              mbar_wait(kfull, bc & 1, &no_abort);  // this block's copies land (bounded)
-              ok = false;
-              break;
-            }
+          }
+          __syncwarp();
+          if (j == 0) ++m;
+          if (bc > 0 && !warp_wait(ofull, (bc - 1) & 1, abort_flag)) {
+            volatile int no_abort = 0;
+            warp_wait(kfull, bc & 1, &no_abort);  // this block's copies land (bounded)
+            ok = false;
+            break;
+          }
+          if (elect_one()) {
             mbar_arrive_expect_tx(vfull, bytes);
             load_keys(sV, xv, vfull);
           }
+          __syncwarp();
         }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
     }
     if (lane == 0) {
@@ -472,26 +477,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
   } else if (warp < 4) {
-    if (lane == 0) {  // ── MMA
-      const uint32_t idesc_pv = (H16 ? idesc_f16_f32(128, 64) : idesc_bf16_f32(128, 64)) | (1u << 16);  // V MN-major
-      int bc = 0;
-      bool ok = true;
-      for (int m = 0; ok; ++m) {
-        if (!mbar_wait(kfull, bc & 1, abort_flag)) { ok = false; break; }
-        const volatile TcItem& e = ring[m & 1];
-        if (!e.live) break;
-        const int nv = ceil16(e.nw) + ceil16(e.s_end), nb = e.nb;
-        if (m > 0 && !mbar_wait(sfree, (m - 1) & 1, abort_flag)) { ok = false; break; }
-        for (int j = 0; j < nb; ++j, ++bc) {
-          int v0, v1;
-          block_of(nv, nb, j, v0, v1);
-          // S_j replaces P_{j-1}, which P V has read
-          if (j > 0 && (!mbar_wait(kfull, bc & 1, abort_flag) || !mbar_wait(ofull, (bc - 1) & 1, abort_flag))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t idesc = H16 ? idesc_f16_f32(128, v1 - v0) : idesc_bf16_f32(128, v1 - v0);
+    // ── MMA: the warp walks its loop whole and elects a lane around each group
+    // of products, so that the operands stay in uniform registers (see
+    // jb_mxfp4_gemm.cu)
+    const uint32_t idesc_pv = (H16 ? idesc_f16_f32(128, 64) : idesc_bf16_f32(128, 64)) | (1u << 16);  // V MN-major
+    int bc = 0;
+    bool ok = true;
+    for (int m = 0; ok; ++m) {
+      if (!warp_wait(kfull, bc & 1, abort_flag)) { ok = false; break; }
+      const volatile TcItem& e = ring[m & 1];
+      if (!e.live) break;
+      const int nv = ceil16(e.nw) + ceil16(e.s_end), nb = e.nb;
+      __syncwarp();
+      if (m > 0 && !warp_wait(sfree, (m - 1) & 1, abort_flag)) { ok = false; break; }
+      for (int j = 0; j < nb; ++j, ++bc) {
+        int v0, v1;
+        block_of(nv, nb, j, v0, v1);
+        // S_j replaces P_{j-1}, which P V has read
+        if (j > 0 && (!warp_wait(kfull, bc & 1, abort_flag) || !warp_wait(ofull, (bc - 1) & 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t idesc = H16 ? idesc_f16_f32(128, v1 - v0) : idesc_bf16_f32(128, v1 - v0);
+        if (elect_one()) {
 #pragma unroll
           for (int half = 0; half < C::HALVES; ++half) {
             const uint64_t dq = umma_desc_sw128(sQ + half * (128 * 128));
@@ -500,26 +509,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem, dq + 2u * kk, dk + 2u * kk, idesc, (half | kk) != 0);
           }
           mma_commit(sfull);
-          if (!mbar_wait(pfull, bc & 1, abort_flag) || !mbar_wait(vfull, bc & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < (v1 - v0) >> 4; ++c) {
+        }
+        __syncwarp();
+        if (!warp_wait(pfull, bc & 1, abort_flag) || !warp_wait(vfull, bc & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int steps = (v1 - v0) >> 4;
+        if (elect_one()) {
 #pragma unroll
-            for (int half = 0; half < C::HALVES; ++half)
-              mma_bf16_ta(tmem + C::O_COL + 64 * half, tmem + 8u * c,
-                          umma_desc_sw128(sV + half * (C::KEYS * 128)) + 128u * c, idesc_pv, (j > 0 || c > 0) ? 1u : 0u);
+          for (int half = 0; half < C::HALVES; ++half) {
+            const uint64_t dv = umma_desc_sw128(sV + half * (C::KEYS * 128));
+#pragma unroll
+            for (int c = 0; c < C::KEYS / 16; ++c)
+              if (c < steps)
+                mma_bf16_ta(tmem + C::O_COL + 64 * half, tmem + 8u * c, dv + 128u * c, idesc_pv,
+                            (j > 0 || c > 0) ? 1u : 0u);
           }
           mma_commit(ofull);
         }
+        __syncwarp();
       }
-      if (!ok) {  // every MMA issued completes before TMEM is freed (bounded)
-        volatile int no_abort = 0;
-        mma_commit(spare);
-        mbar_wait(spare, 0, &no_abort);
-      }
+    }
+    if (!ok) {  // every MMA issued completes before TMEM is freed (bounded)
+      volatile int no_abort = 0;
+      if (elect_one()) mma_commit(spare);
+      __syncwarp();
+      warp_wait(spare, 0, &no_abort);
     }
   } else {  // ── softmax
     const int quarter = warp & 3;
