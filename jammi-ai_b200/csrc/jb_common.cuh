@@ -185,6 +185,19 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// mbar_wait for waits on a kernel's critical path: it polls 64 times before it
+// reads %globaltimer for the first time (a read that costs more than a short
+// wait), under the same limit, and gives every lane of the warp the same
+// answer, so that no warp-collective instruction after it is reached by part
+// of the warp.
+__device__ __forceinline__ bool warp_mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  bool ok = mbar_try_wait(bar, parity);
+#pragma unroll 1
+  for (int i = 0; i < 64 && !ok; ++i) ok = mbar_try_wait(bar, parity);
+  if (!ok) ok = mbar_wait(bar, parity, abort);
+  return __all_sync(0xffffffffu, ok);
+}
+
 // ── TMA (non-multicast only) ────────────────────────────────────────────────
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
                                             uint32_t bar) {

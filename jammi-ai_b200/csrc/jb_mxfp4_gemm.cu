@@ -59,7 +59,7 @@ struct MxCfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SF_BYTES;
   static constexpr int STAGES = BN == 192 ? 4 : BN == 128 ? 5 : 6;
   static constexpr int SF_COLS = 8 * (1 + SFB_TILES);  // TMEM columns of a stage's scales
-  static constexpr int TMEM_COLS = BN == 64 ? 256 : 512;
+  static constexpr int TMEM_COLS = 512;  // all of it (one CTA per SM): the base is column 0
   static_assert(2 * BN + STAGES * SF_COLS <= TMEM_COLS, "TMEM columns");
   static constexpr int EPI_WARPS = 4 * (BN / kUnitCols);
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
@@ -73,10 +73,11 @@ struct MxParams {
   const uint8_t* w_scale;
   const float* bias;
   int M, N, K;
-  int epi;
-  int h16;  // 16-bit output and residual are f16 (else bf16)
   int* err;
 };
+
+// Type of the output and the residual.
+enum Out { kBf16, kF16, kF32 };
 
 // D[tmem] (+)= A . B^T over K = 64 e2m1 elements, each block of 32 scaled by
 // the UE8M0 bytes at sfa / sfb.
@@ -120,16 +121,18 @@ constexpr uint32_t mx_idesc(int M, int N, uint32_t sf) {
 __device__ __forceinline__ uint32_t box_slot(uint32_t buf, int row, int q) {
   return buf + row * 128 + ((q ^ (row & 7)) << 4);
 }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool h16) {
-  if (h16) {
+template <Out OUT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (OUT == kF16) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);
 }
-__device__ __forceinline__ float2 unpack2(uint32_t w, bool h16) {
-  if (h16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+template <Out OUT>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (OUT == kF16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -144,10 +147,27 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
 }
-// Same outcome for every lane, so that no warp-collective instruction after
-// it is reached by part of the warp.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+
+// GELU(x) = max(x, 0) - a h(a), a = min(|x|, 8), h(a) = erfc(a / sqrt 2) / 2.
+// log2 h is smooth and nearly quadratic: a polynomial of degree 6, fitted here
+// to log2(erfc(a / sqrt 2) / 2) on [0, 6] for the least error of a h(a), gives
+// h as one 2^x: |error of GELU| <= 2e-7, 13 instructions per pair with the two
+// exponentials (a 16-bit output keeps 2^-9 of its value).  Behind a = 6 the
+// polynomial stays far below -30 up to the clamp.  NaN stays NaN.
+__device__ __forceinline__ float max0_nan(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 gelu_pair(float2 x) {
+  const float2 a = make_float2(fmaxf(-fabsf(x.x), -8.f), fmaxf(-fabsf(x.y), -8.f));  // -a
+  float2 q = __ffma2_rn(a, f2(3.231512164e-05f), f2(7.549100555e-04f));
+  q = __ffma2_rn(a, q, f2(8.007442579e-03f));
+  q = __ffma2_rn(a, q, f2(5.325423181e-02f));
+  q = __ffma2_rn(a, q, f2(-4.589267671e-01f));
+  q = __ffma2_rn(a, q, f2(1.151135921f));
+  q = __ffma2_rn(a, q, f2(-1.000002146f));
+  return __ffma2_rn(a, make_float2(ex2_approx(q.x), ex2_approx(q.y)), make_float2(max0_nan(x.x), max0_nan(x.y)));
 }
 
 // 32 accumulators -> f32 outputs before the residual.
@@ -161,8 +181,8 @@ __device__ __forceinline__ void finish32(const uint32_t (&r)[32], uint32_t bias,
     float2 hi = __fadd2_rn(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])),
                            make_float2(__uint_as_float(b.z), __uint_as_float(b.w)));
     if constexpr (EPI == JB_EPI_GELU) {
-      lo = gelu_tc2(lo);
-      hi = gelu_tc2(hi);
+      lo = gelu_pair(lo);
+      hi = gelu_pair(hi);
     } else if constexpr (EPI == JB_EPI_QUICK_GELU) {
       lo = make_float2(quick_gelu_tc(lo.x), quick_gelu_tc(lo.y));
       hi = make_float2(quick_gelu_tc(hi.x), quick_gelu_tc(hi.y));
@@ -171,14 +191,14 @@ __device__ __forceinline__ void finish32(const uint32_t (&r)[32], uint32_t bias,
   }
 }
 
-// F32: the output (and residual) is f32, else 16-bit.
-template <int BN, int EPI, bool F32>
+template <int BN, int EPI, Out OUT>
 __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
     gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
                       const MxParams p) {
   using Cfg = MxCfg<BN>;
   constexpr bool kRes = EPI == JB_EPI_RESIDUAL;
+  constexpr bool F32 = OUT == kF32;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -198,7 +218,8 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + (bars - base) + 8 * Cfg::BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform to the compiler too
+  const int lane = threadIdx.x & 31;
   const int n_tiles = (p.N + BN - 1) / BN;
   const int total = (p.M + kBM - 1) / kBM * n_tiles;
   const int kb_count = (p.K + kStageK - 1) / kStageK;
@@ -228,18 +249,18 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  constexpr uint32_t tmem_base = 0;
 
-  // The producer and the issuer walk their loops as whole warps and elect one
-  // lane around each stage's group of instructions: the operands stay in
-  // uniform registers.  (Loops inside `if (lane == 0)` issue one product per
-  // about 250 clocks whatever its width, against the 96 that a 192-column
-  // product of K = 64 takes.)
+  // The producer and the issuer walk their loops as whole warps, without
+  // exits (a wait that gives up turns the later ones off), and elect one lane
+  // around each stage's group of instructions: every operand is then in a
+  // uniform register.  With one lane in `if (lane == 0)` a product of any width
+  // takes about 250 clocks to issue; a 192-column product of K = 64 runs in 96.
   if (warp == 0) {  // ── producer
     const int w_tiles = (p.N + 127) / 128;  // scale tiles along N
-    int it = 0;  // stages filled
+    int it = 0, filled = 0;  // stages
     bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
       const int mb = t / n_tiles, nb = t % n_tiles;
       const int wt = nb * BN / 128;
       const int w_copies = min(Cfg::SFB_TILES, w_tiles - wt);
@@ -247,12 +268,11 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
       const uint8_t* sfb_src = p.w_scale + static_cast<size_t>(wt) * k_tiles * kSfTile;
       for (int kb = 0; kb < kb_count; ++kb, ++it) {
         const int st = it % Cfg::STAGES;
-        ok = warp_wait(empty_bar(st), ((it / Cfg::STAGES) & 1) ^ 1u, abort_flag);
-        if (!ok) break;
+        if (ok) ok = warp_mbar_wait(empty_bar(st), ((it / Cfg::STAGES) & 1) ^ 1u, abort_flag);
         const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
         const uint32_t sf = scales + st * Cfg::SF_BYTES;
         const uint32_t sf_bytes = min(2, k_tiles - 2 * kb) * kSfTile;
-        if (elect_one()) {
+        if (elect_one() && ok) {
           mbar_arrive_expect_tx(full_bar(st), Cfg::A_BYTES + Cfg::B_BYTES + sf_bytes * (1 + w_copies));
           tma_load_2d(sa, &tmA, kb * 128, mb * kBM, full_bar(st));
           tma_load_2d(sa + Cfg::A_BYTES, &tmB, kb * 128, nb * BN, full_bar(st));
@@ -263,54 +283,66 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
                       full_bar(st));
         }
         __syncwarp();
+        filled += ok ? 1 : 0;
       }
     }
     if (*abort_flag) {  // copies in flight land before the CTA leaves (bounded)
       volatile int no_abort = 0;
-      for (int b = max(0, it - Cfg::STAGES); b < it; ++b)
+      for (int b = max(0, filled - Cfg::STAGES); b < filled; ++b)
         mbar_wait(full_bar(b % Cfg::STAGES), (b / Cfg::STAGES) & 1, &no_abort);
     }
   } else if (warp == 1) {  // ── MMA issuer
-    int it = 0, acc = 0;
-    uint32_t acc_ph = 0;
+    constexpr uint32_t kStageDesc = (Cfg::A_BYTES + Cfg::B_BYTES) >> 4;  // descriptors count 16 bytes
+    constexpr uint32_t kTileDesc = kSfTile >> 4;
+    const uint64_t da0 = umma_desc_sw128(base), db0 = umma_desc_sw128(base + Cfg::A_BYTES);
+    const uint64_t ds0 = scale_desc(scales);
+    int acc = 0, st = 0;
+    uint32_t acc_ph = 0, ph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
       const uint32_t sf_shift = static_cast<uint32_t>((t % n_tiles) * BN % 128) / 32;
-      ok = warp_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag);
-      if (!ok) break;
+      if (ok) ok = warp_mbar_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag);
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-      for (int kb = 0; kb < kb_count; ++kb, ++it) {
-        const int st = it % Cfg::STAGES;
-        ok = warp_wait(full_bar(st), (it / Cfg::STAGES) & 1, abort_flag);
-        if (!ok) break;
+#pragma unroll 1
+      for (int kb = 0; kb < kb_count; ++kb) {
+        if (ok) ok = warp_mbar_wait(full_bar(st), ph, abort_flag);
         tc_fence_after();
-        const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
-        const uint32_t sf = scales + st * Cfg::SF_BYTES;
+        const uint64_t da = da0 + static_cast<uint32_t>(st) * kStageDesc;
+        const uint64_t db = db0 + static_cast<uint32_t>(st) * kStageDesc;
+        const uint64_t ds = ds0 + static_cast<uint32_t>(st) * (Cfg::SF_BYTES >> 4);
         const uint32_t tsa = tmem_base + 2 * BN + st * Cfg::SF_COLS;  // [2 K tiles][4]
         const uint32_t tsb = tsa + 8;                                 // [2 K tiles][SFB_TILES][4]
-        const int k_left = p.K - kb * kStageK;
-        const uint64_t da = umma_desc_sw128(sa), db = umma_desc_sw128(sa + Cfg::A_BYTES);
-        if (elect_one()) {
+        auto products = [&](int steps) {  // K = 64 each; constant but in the last stage
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            if (c * 128 < k_left) {
-              tmem_cp_scales(tsa + 4 * c, scale_desc(sf + c * kSfTile));
+            if (2 * c < steps) {
+              tmem_cp_scales(tsa + 4 * c, ds + c * kTileDesc);
 #pragma unroll
               for (int i = 0; i < Cfg::SFB_TILES; ++i)
-                tmem_cp_scales(tsb + 4 * (c * Cfg::SFB_TILES + i), scale_desc(sf + (2 * (1 + i) + c) * kSfTile));
+                tmem_cp_scales(tsb + 4 * (c * Cfg::SFB_TILES + i), ds + (2 * (1 + i) + c) * kTileDesc);
             }
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (k * 64 < k_left)
+          for (int k = 0; k < 4; ++k)
+            if (k < steps)
               mma_mxf4(d_tmem, da + 2u * k, db + 2u * k, mx_idesc(kBM, BN, 2 * (k & 1)), tsa + 4 * (k >> 1),
                        tsb + 4 * Cfg::SFB_TILES * (k >> 1) + sf_shift, (kb | k) != 0);
-          }
+        };
+        const int steps = (p.K - kb * kStageK + 63) / 64;
+        if (elect_one() && ok) {
+          if (steps >= 4)
+            products(4);
+          else
+            products(steps);
           mma_commit(empty_bar(st));
           if (kb == kb_count - 1) mma_commit(tfull_bar(acc));
         }
         __syncwarp();
+        if (++st == Cfg::STAGES) {
+          st = 0;
+          ph ^= 1u;
+        }
       }
       acc ^= 1;
       if (acc == 0) acc_ph ^= 1u;
@@ -319,7 +351,7 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
       volatile int no_abort = 0;
       if (elect_one()) mma_commit(spare);
       __syncwarp();
-      warp_wait(spare, 0, &no_abort);
+      warp_mbar_wait(spare, 0, &no_abort);
     }
   } else {  // ── epilogue
     const int w = warp - 2;
@@ -358,7 +390,7 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
         b1 = bias_at(t + gridDim.x, 32 + lane);
       }
       __syncwarp();
-      if (!warp_wait(tfull_bar(acc), acc_ph, abort_flag)) break;
+      if (!warp_mbar_wait(tfull_bar(acc), acc_ph, abort_flag)) break;
       tc_fence_after();
       uint32_t r[2][32];
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
@@ -383,7 +415,7 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
           if (kRes) load_res(32);
         }
         if (kRes && (F32 || half == 0)) {
-          if (!warp_wait(res_bar(w), waited & 1, abort_flag)) break;
+          if (!warp_mbar_wait(res_bar(w), waited & 1, abort_flag)) break;
           ++waited;
         }
         constexpr int kSlots = F32 ? 8 : 4;  // 16-byte slots of a row for 32 columns
@@ -405,14 +437,13 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
               const uint32_t x4[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2(x4[e], p.h16);
+                const float2 f = unpack2<OUT>(x4[e]);
                 v[8 * q + 2 * e] += f.x;
                 v[8 * q + 2 * e + 1] += f.y;
               }
             }
-            sts128(at, make_uint4(pack2(v[8 * q], v[8 * q + 1], p.h16), pack2(v[8 * q + 2], v[8 * q + 3], p.h16),
-                                  pack2(v[8 * q + 4], v[8 * q + 5], p.h16),
-                                  pack2(v[8 * q + 6], v[8 * q + 7], p.h16)));
+            sts128(at, make_uint4(pack2<OUT>(v[8 * q], v[8 * q + 1]), pack2<OUT>(v[8 * q + 2], v[8 * q + 3]),
+                                  pack2<OUT>(v[8 * q + 4], v[8 * q + 5]), pack2<OUT>(v[8 * q + 6], v[8 * q + 7])));
           }
         }
         if (F32 || half == 1) {
@@ -438,7 +469,7 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+    tmem_dealloc(*tmem_slot, Cfg::TMEM_COLS);
   }
 }
 
@@ -470,14 +501,14 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, int esz, const void* p
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, int EPI, bool F32>
+template <int BN, int EPI, Out OUT>
 cudaError_t launch_tile(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
   using Cfg = MxCfg<BN>;
   CUtensorMap ma, mb, mc, mr;
-  const CUtensorMapDataType ct = F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                 : p.h16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const int esz = F32 ? 4 : 2;
+  const CUtensorMapDataType ct = OUT == kF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : OUT == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const int esz = OUT == kF32 ? 4 : 2;
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   bool ok = make_map(&ma, u8, 1, g.aq, g.M, g.K / 2, kBM) && make_map(&mb, u8, 1, g.wq, g.N, g.K / 2, BN) &&
             make_map(&mc, ct, esz, g.C, g.M, g.N, 32);
@@ -487,7 +518,7 @@ cudaError_t launch_tile(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, 
     if (why) *why = "linear(mxfp4): cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  auto kern = gemm_mxfp4_kernel<BN, EPI, F32>;
+  auto kern = gemm_mxfp4_kernel<BN, EPI, OUT>;
   int dev = 0;
   cudaGetDevice(&dev);
   // the shared-memory opt-in is a property of each device's context
@@ -503,18 +534,23 @@ cudaError_t launch_tile(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, 
   return cudaGetLastError();
 }
 
-template <int BN, bool F32>
+template <int BN, Out OUT>
 cudaError_t launch_epi(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
   switch (g.epi) {
-    case JB_EPI_GELU: return launch_tile<BN, JB_EPI_GELU, F32>(g, p, s, why);
-    case JB_EPI_QUICK_GELU: return launch_tile<BN, JB_EPI_QUICK_GELU, F32>(g, p, s, why);
-    case JB_EPI_RESIDUAL: return launch_tile<BN, JB_EPI_RESIDUAL, F32>(g, p, s, why);
-    default: return launch_tile<BN, JB_EPI_NONE, F32>(g, p, s, why);
+    case JB_EPI_GELU: return launch_tile<BN, JB_EPI_GELU, OUT>(g, p, s, why);
+    case JB_EPI_QUICK_GELU: return launch_tile<BN, JB_EPI_QUICK_GELU, OUT>(g, p, s, why);
+    case JB_EPI_RESIDUAL: return launch_tile<BN, JB_EPI_RESIDUAL, OUT>(g, p, s, why);
+    default: return launch_tile<BN, JB_EPI_NONE, OUT>(g, p, s, why);
   }
 }
 template <int BN>
 cudaError_t launch_out(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
-  return g.c_dtype == JB_DT_F32 ? launch_epi<BN, true>(g, p, s, why) : launch_epi<BN, false>(g, p, s, why);
+  if (g.c_dtype == JB_DT_F16) return launch_epi<BN, kF16>(g, p, s, why);
+  // f32 outputs hold 64 accumulators and 32 results: more than the 448
+  // threads of BN = 192 have registers for
+  if constexpr (BN < 192)
+    if (g.c_dtype == JB_DT_F32) return launch_epi<BN, kF32>(g, p, s, why);
+  return launch_epi<BN, kBf16>(g, p, s, why);
 }
 
 }  // namespace
@@ -526,14 +562,13 @@ cudaError_t launch_linear_mxfp4(const MxGemmArgs& g, cudaStream_t s, std::string
     if (why) *why = "linear(mxfp4): too many output tiles";
     return cudaErrorInvalidValue;
   }
-  MxParams p{g.a_scale, g.w_scale, g.bias, g.M, g.N, g.K, g.epi, g.c_dtype == JB_DT_F16 ? 1 : 0, g.err};
+  MxParams p{g.a_scale, g.w_scale, g.bias, g.M, g.N, g.K, g.err};
   int dev = 0;
   cudaGetDevice(&dev);
   const long long sms = num_sms(dev);
   if (m_tiles * ((g.N + 127) / 128) <= sms) return launch_out<64>(g, p, s, why);
-  // f32 outputs hold 64 accumulators and 32 results: more than 448 threads have registers for
   if (g.c_dtype == JB_DT_F32 || m_tiles * ((g.N + 191) / 192) <= sms) return launch_out<128>(g, p, s, why);
-  return launch_epi<192, false>(g, p, s, why);
+  return launch_out<192>(g, p, s, why);
 }
 
 }  // namespace jb

@@ -265,9 +265,6 @@ struct TcParams {
   int* err;
 };
 
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
-}
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -428,7 +425,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               v += big ? 64 : 16;
             }
           };
-          if (bc > 0 && !warp_wait(sfull, (bc - 1) & 1, abort_flag)) { ok = false; break; }
+          if (bc > 0 && !warp_mbar_wait(sfull, (bc - 1) & 1, abort_flag)) { ok = false; break; }
           const uint32_t bytes = static_cast<uint32_t>(v1 - v0) * 128 * C::HALVES;
           const int boxes = (min(it.n - it.q0, p.kq) + 63) >> 6;
           if (elect_one()) {
@@ -450,9 +447,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           __syncwarp();
           if (j == 0) ++m;
-          if (bc > 0 && !warp_wait(ofull, (bc - 1) & 1, abort_flag)) {
+          if (bc > 0 && !warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag)) {
             volatile int no_abort = 0;
-            warp_wait(kfull, bc & 1, &no_abort);  // this block's copies land (bounded)
+            warp_mbar_wait(kfull, bc & 1, &no_abort);  // this block's copies land (bounded)
             ok = false;
             break;
           }
@@ -484,17 +481,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int bc = 0;
     bool ok = true;
     for (int m = 0; ok; ++m) {
-      if (!warp_wait(kfull, bc & 1, abort_flag)) { ok = false; break; }
+      if (!warp_mbar_wait(kfull, bc & 1, abort_flag)) { ok = false; break; }
       const volatile TcItem& e = ring[m & 1];
       if (!e.live) break;
       const int nv = ceil16(e.nw) + ceil16(e.s_end), nb = e.nb;
       __syncwarp();
-      if (m > 0 && !warp_wait(sfree, (m - 1) & 1, abort_flag)) { ok = false; break; }
+      if (m > 0 && !warp_mbar_wait(sfree, (m - 1) & 1, abort_flag)) { ok = false; break; }
       for (int j = 0; j < nb; ++j, ++bc) {
         int v0, v1;
         block_of(nv, nb, j, v0, v1);
         // S_j replaces P_{j-1}, which P V has read
-        if (j > 0 && (!warp_wait(kfull, bc & 1, abort_flag) || !warp_wait(ofull, (bc - 1) & 1, abort_flag))) {
+        if (j > 0 && (!warp_mbar_wait(kfull, bc & 1, abort_flag) || !warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag))) {
           ok = false;
           break;
         }
@@ -511,7 +508,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mma_commit(sfull);
         }
         __syncwarp();
-        if (!warp_wait(pfull, bc & 1, abort_flag) || !warp_wait(vfull, bc & 1, abort_flag)) {
+        if (!warp_mbar_wait(pfull, bc & 1, abort_flag) || !warp_mbar_wait(vfull, bc & 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -536,7 +533,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       volatile int no_abort = 0;
       if (elect_one()) mma_commit(spare);
       __syncwarp();
-      warp_wait(spare, 0, &no_abort);
+      warp_mbar_wait(spare, 0, &no_abort);
     }
   } else {  // ── softmax
     const int quarter = warp & 3;
@@ -545,7 +542,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int bc = 0;
     bool ok = true;
     for (int m = 0; ok; ++m) {
-      if (!warp_wait(ifull + 8 * (m & 1), (m >> 1) & 1, abort_flag)) break;
+      if (!warp_mbar_wait(ifull + 8 * (m & 1), (m >> 1) & 1, abort_flag)) break;
       const volatile TcItem& e = ring[m & 1];
       if (!e.live) break;
       const int start = e.start, n = e.n, h = e.h, q0 = e.q0, k_begin = e.k_begin, nw = e.nw, s_end = e.s_end,
@@ -571,7 +568,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int j = 0; j < nb; ++j, ++bc) {
         int v0, v1;
         block_of(nv, nb, j, v0, v1);
-        if (!warp_wait(sfull, bc & 1, abort_flag)) { ok = false; break; }
+        if (!warp_mbar_wait(sfull, bc & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         if (active) {
           float mx = -INFINITY;
@@ -651,7 +648,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // V rows [nw, nw16) belong to no key of the item: their product with
         // P = 0 must be 0
         if (nw16 > nw && nw16 > v0 && nw16 <= v1) {
-          if (!warp_wait(vfull, bc & 1, abort_flag)) { ok = false; break; }
+          if (!warp_mbar_wait(vfull, bc & 1, abort_flag)) { ok = false; break; }
           for (int i = r; i < (nw16 - nw) * 8 * C::HALVES; i += 128) {
             const int row = i >> 3, half = row / (nw16 - nw);
             const uint32_t a = sV + half * (C::KEYS * 128) +
@@ -665,7 +662,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive(pfull);
       }
       if (!ok) break;
-      if (!warp_wait(ofull, (bc - 1) & 1, abort_flag)) break;
+      if (!warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag)) break;
       tc_fence_after();
       const float inv = 1.f / l;
       T* out = static_cast<T*>(w.ctx) + (static_cast<size_t>(start + (mine ? qi : 0)) * w.heads + h) * D;
