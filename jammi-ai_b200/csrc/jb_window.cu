@@ -212,36 +212,46 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 
 // ── tcgen05, 16-bit rows with head_dim 64 or 128 ────────────────────────────
 // A persistent CTA per SM runs two independent slots, each on its own items
-// (row, head, kQ-query block) with its own shared memory and half of TMEM:
-//   TMA warp      finds the slot's next items (32 candidates a time, one per
-//                 lane), publishes each in a two-entry ring and loads its Q
-//                 and then, per key block, K and V.
+// (row, head, kq-query block) with its own shared memory and half of TMEM:
+//   TMA warp      publishes the slot's items in a two-entry ring and loads
+//                 each one's Q and then, per key block, K and V.
 //   MMA warp      S = Q K^T (M = 128, N = the block's keys) into columns
 //                 [0, N), then O (+)= P V with P read from TMEM.
-//   4 softmax     one thread per query row.  Two passes over the scores in
-//   warps         TMEM (maximum; exponentials and sum), 32 keys at a time; a
-//                 warp skips the 32-key pieces that none of its 32 queries
-//                 sees.  P (16-bit pairs) overwrites the scores that the same
-//                 thread has read: keys [16 c, 16 c + 16) go to columns
-//                 [8 c, 8 c + 8).  O / sum is stored after the last block.
+//   8 softmax     two threads per query row, which take the block's 32-key
+//   warps         pieces in turn (even / odd) and exchange their maxima and
+//                 sums.  Two passes over the scores in TMEM (maximum;
+//                 exponentials and sum); a warp skips the pieces that none of
+//                 its 32 queries sees.  P (16-bit pairs) overwrites the
+//                 scores of its own piece: no thread writes where the other
+//                 one still reads.  O / sum goes out through shared memory in
+//                 whole row segments.
 // The keys of an item are its window [k_begin, k_end), padded to 16, then the
 // first keys [0, s_end) that the window has left behind, padded to 16.  With
 // head_dim 64, an item of up to 256 keys is ONE block: no running maximum, no
-// rescaling, three hand-overs in all (S, P, O), and O takes columns
-// [128, 192) once every score is read.  That covers windows of up to
-// left + right = 128 around 128 queries (and 112 queries with up to 16 sinks),
-// the case this operator is for.  Longer ranges go in blocks of 128 keys with
-// a lazily rescaled running maximum (raised only by more than 2^8).
+// rescaling, three hand-overs in all (S, P, O); O takes the columns of pieces
+// 6 and 7 once every score is read, and their P goes to the free halves of
+// pieces 0 and 1.  That covers windows of up to left + right = 128 around 128
+// queries (and 112 queries with up to 16 sinks), the case this operator is
+// for.  Longer ranges go in blocks of 128 keys with a lazily rescaled running
+// maximum (raised only by more than 2^8).
 //
 // A masked value contributes 0 * v, which is not 0 when v is not finite.  V
 // rows behind the item's last key are zeroed in shared memory; for the rest
-// an output that is not finite is computed again, by its thread, over the
+// outputs that are not finite are computed again, by their thread, over the
 // visible keys only (window_row_exact).
+//
+// Items are numbered over the query blocks that exist (a prefix sum of the
+// rows' blocks in shared memory, for batches of up to kPrefixRows) and dealt
+// to the slots in turn; no counter in global memory, so calls and replayed
+// graphs share nothing.
 //
 // Every wait is bounded; on a timeout each role stops, copies and MMAs in
 // flight are waited for (bounded), the error flag is set and TMEM is freed.
-constexpr int kTcThreads = 384;  // 2 TMA, 2 MMA, 8 softmax warps
-constexpr float kRescale = 8.f;  // lazy-rescaling threshold, log2 units
+constexpr int kTcWarps = 20;      // 2 TMA, 2 MMA, 16 softmax
+constexpr int kTcThreads = 32 * kTcWarps;
+constexpr int kGroupWarps = 8;    // softmax warps of a slot
+constexpr int kPrefixRows = 2048;
+constexpr float kRescale = 8.f;   // lazy-rescaling threshold, log2 units
 
 template <int D>
 struct TcCfg {
@@ -250,9 +260,13 @@ struct TcCfg {
   static constexpr int Q_BYTES = HALVES * 128 * 128;
   static constexpr int KV_BYTES = HALVES * KEYS * 128;
   static constexpr int SLOT_BYTES = Q_BYTES + 2 * KV_BYTES;
+  static constexpr int O_COL = 256 - D;                    // O's columns of a slot
+  static constexpr int SEG = D == 64 ? 64 : 32;            // bytes of a row that a warp stores at once
+  static constexpr int STAGE_BYTES = 2 * kGroupWarps * 32 * SEG;
+  static constexpr int XCH_BYTES = 2 * (2 + 1) * 4 * 2 * 32 * 4;  // [slot][max 0, max 1, sum][quarter][half][lane]
   static constexpr int META_BYTES = 512;
-  static constexpr int SMEM = 1024 + 2 * SLOT_BYTES + META_BYTES;
-  static constexpr int O_COL = 128;
+  static constexpr int SMEM = 1024 + 2 * SLOT_BYTES + STAGE_BYTES + XCH_BYTES + (kPrefixRows + 4) * 4 + META_BYTES;
+  static_assert(SMEM <= 232448, "shared memory");
 };
 
 struct TcItem {
@@ -260,8 +274,8 @@ struct TcItem {
 };
 struct TcParams {
   WinParams w;
-  long long items;  // batch * q_blocks * heads
-  int kq;           // queries per item
+  int batch;
+  int kq;    // queries per item
   int* err;
 };
 
@@ -272,6 +286,11 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
 template <bool H16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -288,11 +307,18 @@ __host__ __device__ constexpr int ceil16(int v) { return (v + 15) & ~15; }
 __device__ __forceinline__ uint32_t low_bits(int c) {
   return c <= 0 ? 0u : c >= 32 ? 0xffffffffu : (1u << c) - 1u;
 }
+// First column of the P of keys [16 k, 16 k + 16): the first half of their
+// 32-key piece's own score columns; pieces 6 and 7 lie in the second halves of
+// pieces 0 and 1 (same parity: the same thread's columns).
+__host__ __device__ constexpr uint32_t p_col(int k) {
+  const int piece = k >> 1;
+  return static_cast<uint32_t>((piece < 6 ? 32 * piece : 32 * (piece - 6) + 16) + 8 * (k & 1));
+}
 
-// One query row over its visible keys only, in f32 from global memory: the
-// rows whose tensor-core output is not finite.
+// Output columns [c0, c1) of one query row over its visible keys
+// only, in f32 from global memory: rows whose tensor-core output is not finite.
 template <typename T, int D>
-__device__ __noinline__ void window_row_exact(const WinParams& p, int start, int n, int h, int qi) {
+__device__ __noinline__ void window_row_exact(const WinParams& p, int start, int n, int h, int qi, int c0, int c1) {
   const int ld = (p.heads + 2 * p.kv_heads) * D;
   const T* row = static_cast<const T*>(p.qkv) + static_cast<size_t>(start) * ld;
   const T* q = row + static_cast<size_t>(qi) * ld + h * D;
@@ -306,12 +332,11 @@ __device__ __noinline__ void window_row_exact(const WinParams& p, int start, int
     for (int d = 0; d < D; ++d) s = fmaf(to_f(q[d]), to_f(k[static_cast<size_t>(j) * ld + d]), s);
     return s * p.scale_log2;
   };
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY;
   for (int j = behind > 0 ? 0 : lo; j <= hi; j = j + 1 == behind ? lo : j + 1) m = fmaxf(m, score(j));
   if (m == -INFINITY) m = 0.f;
-  for (int c = 0; c < D; c += 16) {  // 16 output columns a pass
-    float o[16] = {};
-    l = 0.f;
+  for (int c = c0; c < c1; c += 16) {  // 16 output columns a pass
+    float o[16] = {}, l = 0.f;
     for (int j = behind > 0 ? 0 : lo; j <= hi; j = j + 1 == behind ? lo : j + 1) {
       const float e = exp2f(score(j) - m);
       l += e;
@@ -327,14 +352,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      const __grid_constant__ CUtensorMap tm16) {
   using C = TcCfg<D>;
   using T = typename std::conditional<H16, f16, bf16>::type;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform to the compiler too
+  const int lane = threadIdx.x & 31;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
-  uint8_t* meta = smem_raw + (base + 2 * C::SLOT_BYTES - raw);
-  const int g = warp < 4 ? warp & 1 : (warp - 4) >> 2;  // this warp's slot
+  const uint32_t staging = base + 2 * C::SLOT_BYTES;
+  float* xch = reinterpret_cast<float*>(smem_raw + (staging + C::STAGE_BYTES - raw));
+  int* prefix = reinterpret_cast<int*>(xch) + C::XCH_BYTES / 4;  // [batch + 1] query blocks before each row
+  uint8_t* meta = reinterpret_cast<uint8_t*>(prefix + kPrefixRows + 4);
+  const int g = warp < 4 ? warp & 1 : (warp - 4) / kGroupWarps;  // this warp's slot
   const uint32_t sQ = base + g * C::SLOT_BYTES, sK = sQ + C::Q_BYTES, sV = sK + C::KV_BYTES;
-  const uint32_t bars = smem_u32(meta) + g * 96;
+  const uint32_t bars = smem_u32(meta) + g * 112;
   const uint32_t ifull = bars;         // [2] an item is published
   const uint32_t kfull = bars + 16;    // K (and Q) of a block loaded
   const uint32_t vfull = bars + 24;
@@ -343,57 +372,92 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t ofull = bars + 48;    // P V done: V read
   const uint32_t sfree = bars + 56;    // O read: the slot's TMEM is free
   const uint32_t spare = bars + 64;
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(meta + 192);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 196);
+  const uint32_t pairs = bars + 72;    // [4] the two warps of a lane quarter meet
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(meta + 224);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 228);
   volatile TcItem* ring = reinterpret_cast<volatile TcItem*>(meta + 256) + 2 * g;
   static_assert(256 + 4 * sizeof(TcItem) <= C::META_BYTES, "meta layout");
+  const WinParams& w = p.w;
+  const bool counted = p.batch <= kPrefixRows;
 
-  if (threadIdx.x == 0) {
+  if (warp == 0 && counted) {  // query blocks before each row
+    int sum = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      int blocks = 0;
+      if (b0 + lane < p.batch) {
+        const int start = w.cu[b0 + lane], n = min(w.cu[b0 + lane + 1], w.rows) - start;  // never past the buffers
+        if (start >= 0 && n > 0) blocks = (min(n, w.q_blocks * p.kq) + p.kq - 1) / p.kq;
+      }
+      int incl = blocks;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      if (b0 + lane < p.batch) prefix[b0 + lane] = sum + incl - blocks;
+      sum += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) prefix[p.batch] = sum;
+  }
+  if (threadIdx.x == 64) {
     for (int s = 0; s < 2; ++s) {
-      const uint32_t b = smem_u32(meta) + s * 96;
-      for (int i = 0; i < 5; ++i) mbar_init(b + 8 * i, 1);
-      mbar_init(b + 40, 4);
-      mbar_init(b + 48, 1);
-      mbar_init(b + 56, 4);
-      mbar_init(b + 64, 1);
+      const uint32_t b = smem_u32(meta) + s * 112;
+      for (int i = 0; i < 9; ++i) mbar_init(b + 8 * i, i == 5 || i == 7 ? kGroupWarps : 1);  // 5: pfull, 7: sfree
+      for (int i = 9; i < 13; ++i) mbar_init(b + 8 * i, 2);
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 2) tmem_alloc(smem_u32(tslot), 512);
+  if (warp == 3) tmem_alloc(smem_u32(tslot), 512);  // all of it (one CTA per SM): the base is column 0
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tslot + static_cast<uint32_t>(g) * 256;
-  const WinParams& w = p.w;
+  const uint32_t tmem = static_cast<uint32_t>(g) * 256;
   // keys of block j of an item, in its own order: window, then sinks
   auto block_of = [&](int nv, int nb, int j, int& v0, int& v1) {
     v0 = nb == 1 ? 0 : 128 * j;
     v1 = nb == 1 ? nv : min(nv, v0 + 128);
   };
 
+  // The TMA and MMA warps walk their loops whole and elect one lane around
+  // each group of instructions, so that the operands stay in uniform
+  // registers (see jb_mxfp4_gemm.cu).
   if (warp < 2) {  // ── TMA
+    const long long items =
+        (counted ? static_cast<long long>(prefix[p.batch]) : static_cast<long long>(p.batch) * w.q_blocks) * w.heads;
     const long long stride = 2ll * gridDim.x;
     int bc = 0, m = 0;  // blocks loaded, items published
     bool ok = true;
     const int hk_div = w.heads / w.kv_heads;
-    for (long long f0 = static_cast<long long>(g) * gridDim.x + blockIdx.x; f0 < p.items && ok; f0 += 32 * stride) {
+    for (long long f0 = static_cast<long long>(g) * gridDim.x + blockIdx.x; f0 < items && ok; f0 += 32 * stride) {
       const long long f = f0 + lane * stride;
-      int start = 0, n = 0, h = 0, q0 = 0;
-      if (f < p.items) {
+      int start = 0, n = 0, h = 0, q0 = 0;  // this lane's candidate
+      if (f < items) {
         h = static_cast<int>(f % w.heads);
         const long long bq = f / w.heads;
-        const int b = static_cast<int>(bq / w.q_blocks);
-        q0 = static_cast<int>(bq % w.q_blocks) * p.kq;
+        int b, qb;
+        if (counted) {
+          int lo = 0, hi = p.batch;  // prefix[lo] <= bq < prefix[hi]
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] <= bq) lo = mid;
+            else hi = mid;
+          }
+          b = lo;
+          qb = static_cast<int>(bq) - prefix[lo];
+        } else {
+          b = static_cast<int>(bq / w.q_blocks);
+          qb = static_cast<int>(bq % w.q_blocks);
+        }
+        q0 = qb * p.kq;
         start = w.cu[b];
         n = min(w.cu[b + 1], w.rows) - start;  // never past the buffers
       }
-      unsigned todo = __ballot_sync(0xffffffffu, f < p.items && start >= 0 && q0 < n);
+      unsigned todo = __ballot_sync(0xffffffffu, f < items && start >= 0 && q0 < n);
       while (todo && ok) {
         const int src = __ffs(todo) - 1;
         todo &= todo - 1;
         TcItem it;
-        it.live = 1;
         it.start = __shfl_sync(0xffffffffu, start, src);
         it.n = __shfl_sync(0xffffffffu, n, src);
         it.h = __shfl_sync(0xffffffffu, h, src);
@@ -473,10 +537,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_wait(vfull, (bc - 1) & 1, &no_abort);
       }
     }
-  } else if (warp < 4) {
-    // ── MMA: the warp walks its loop whole and elects a lane around each group
-    // of products, so that the operands stay in uniform registers (see
-    // jb_mxfp4_gemm.cu)
+  } else if (warp < 4) {  // ── MMA
     const uint32_t idesc_pv = (H16 ? idesc_f16_f32(128, 64) : idesc_bf16_f32(128, 64)) | (1u << 16);  // V MN-major
     int bc = 0;
     bool ok = true;
@@ -484,14 +545,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!warp_mbar_wait(kfull, bc & 1, abort_flag)) { ok = false; break; }
       const volatile TcItem& e = ring[m & 1];
       if (!e.live) break;
-      const int nv = ceil16(e.nw) + ceil16(e.s_end), nb = e.nb;
-      __syncwarp();
+      const int nv = __shfl_sync(0xffffffffu, ceil16(e.nw) + ceil16(e.s_end), 0);
+      const int nb = __shfl_sync(0xffffffffu, e.nb, 0);
       if (m > 0 && !warp_mbar_wait(sfree, (m - 1) & 1, abort_flag)) { ok = false; break; }
       for (int j = 0; j < nb; ++j, ++bc) {
         int v0, v1;
         block_of(nv, nb, j, v0, v1);
         // S_j replaces P_{j-1}, which P V has read
-        if (j > 0 && (!warp_mbar_wait(kfull, bc & 1, abort_flag) || !warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag))) {
+        if (j > 0 &&
+            (!warp_mbar_wait(kfull, bc & 1, abort_flag) || !warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag))) {
           ok = false;
           break;
         }
@@ -521,7 +583,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int c = 0; c < C::KEYS / 16; ++c)
               if (c < steps)
-                mma_bf16_ta(tmem + C::O_COL + 64 * half, tmem + 8u * c, dv + 128u * c, idesc_pv,
+                mma_bf16_ta(tmem + C::O_COL + 64 * half, tmem + p_col(c), dv + 128u * c, idesc_pv,
                             (j > 0 || c > 0) ? 1u : 0u);
           }
           mma_commit(ofull);
@@ -536,9 +598,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       warp_mbar_wait(spare, 0, &no_abort);
     }
   } else {  // ── softmax
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, half = ((warp - 4) >> 2) & 1;
     const int r = 32 * quarter + lane;
     const uint32_t trow = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    const uint32_t pair = pairs + 8 * quarter;
+    // [3] max (by block parity), sum; then [half][lane]
+    float* xq = xch + ((g * 3) * 4 + quarter) * 64 + lane;
+    int meets = 0;
+    auto meet = [&]() -> bool {  // what both warps wrote before is visible to both
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair);
+      return warp_mbar_wait(pair, (meets++) & 1, abort_flag);
+    };
+    const uint32_t stage = staging + static_cast<uint32_t>(warp - 4) * 32 * C::SEG;
     int bc = 0;
     bool ok = true;
     for (int m = 0; ok; ++m) {
@@ -549,8 +621,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 nb = e.nb;
       const int nw16 = ceil16(nw), nv = nw16 + ceil16(s_end);
       const int qi = q0 + r;
-      const bool mine = r < p.kq && qi < n;
-      const bool active = __any_sync(0xffffffffu, mine);
+      const int rows = min(p.kq, n - q0) - 32 * quarter;  // rows of this warp's quarter (32 and more: all)
+      const bool mine = lane < rows;
+      const bool active = rows > 0;
       // visible keys of this row, relative to k_begin
       const int lo = qi - min(w.left, qi) - k_begin;
       const int hi = mine ? qi + min(w.right, n - 1 - qi) - k_begin : -1;
@@ -573,8 +646,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (active) {
           float mx = -INFINITY;
 #pragma unroll 1
-          for (int c = 0; c < v1 - v0; c += 32) {
-            uint32_t bits = visible(v0 + c);
+          for (int c = 32 * half; c < v1 - v0; c += 64) {
+            const uint32_t bits = visible(v0 + c);
             if (!__any_sync(0xffffffffu, bits != 0)) continue;
             uint32_t s[32];
             tmem_ld_32x32b_x32(trow + c, s);
@@ -589,21 +662,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (bits >> i & 1) mx = fmaxf(mx, __uint_as_float(s[i]));
             }
           }
+          float* xm = xq + (bc & 1) * 256;
+          xm[32 * half] = mx;
+          if (!meet()) { ok = false; break; }
+          mx = fmaxf(mx, xm[32 * (half ^ 1)]);
           const float mb = mx * w.scale_log2;
           if (j == 0) {
             mref = mb == -INFINITY ? 0.f : mb;  // nothing visible yet: p stays 0
           } else {
+            // both threads of a row decide alike; each rescales its half of O
             const bool up = mb > mref + kRescale;
             if (__any_sync(0xffffffffu, up)) {
               const float alpha = up ? ex2_approx(mref - mb) : 1.f;
               l *= alpha;
 #pragma unroll 1
-              for (int c = 0; c < D; c += 8) {
+              for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 8) {
                 uint32_t o8[8];
-                asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                             : "=r"(o8[0]), "=r"(o8[1]), "=r"(o8[2]), "=r"(o8[3]), "=r"(o8[4]), "=r"(o8[5]),
-                               "=r"(o8[6]), "=r"(o8[7])
-                             : "r"(trow + C::O_COL + c));
+                tmem_ld_32x32b_x8(trow + C::O_COL + c, o8);
                 tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o8[i] = __float_as_uint(__uint_as_float(o8[i]) * alpha);
@@ -615,7 +690,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           float l0 = 0.f, l1 = 0.f;
 #pragma unroll 1
-          for (int c = 0; c < v1 - v0; c += 32) {
+          for (int c = 32 * half; c < v1 - v0; c += 64) {
             const uint32_t bits = visible(v0 + c);
             uint32_t pk[16];
             if (!__any_sync(0xffffffffu, bits != 0)) {
@@ -640,7 +715,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 pk[i >> 1] = pack16<H16>(p0, p1);
               }
             }
-            tmem_st_32x32b_x16(trow + (c >> 1), pk);
+            tmem_st_32x32b_x16(trow + p_col(c >> 4), pk);
           }
           l += l0 + l1;
           tmem_wait_st();
@@ -649,10 +724,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // P = 0 must be 0
         if (nw16 > nw && nw16 > v0 && nw16 <= v1) {
           if (!warp_mbar_wait(vfull, bc & 1, abort_flag)) { ok = false; break; }
-          for (int i = r; i < (nw16 - nw) * 8 * C::HALVES; i += 128) {
-            const int row = i >> 3, half = row / (nw16 - nw);
-            const uint32_t a = sV + half * (C::KEYS * 128) +
-                               static_cast<uint32_t>(nw - v0 + row - half * (nw16 - nw)) * 128 + (i & 7) * 16;
+          for (int i = r + 128 * half; i < (nw16 - nw) * 8 * C::HALVES; i += 256) {
+            const int row = i >> 3, blk = row / (nw16 - nw);
+            const uint32_t a = sV + blk * (C::KEYS * 128) +
+                               static_cast<uint32_t>(nw - v0 + row - blk * (nw16 - nw)) * 128 + (i & 7) * 16;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory");
           }
           fence_proxy_async_smem();
@@ -662,45 +737,77 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive(pfull);
       }
       if (!ok) break;
+      float inv = 0.f;
+      if (active) {
+        float* xs = xq + 2 * 256;
+        xs[32 * half] = l;
+        if (!meet()) break;
+        inv = 1.f / (l + xs[32 * (half ^ 1)]);
+      }
       if (!warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag)) break;
       tc_fence_after();
-      const float inv = 1.f / l;
-      T* out = static_cast<T*>(w.ctx) + (static_cast<size_t>(start + (mine ? qi : 0)) * w.heads + h) * D;
+      // this thread's D / 2 columns, 32 at a time
+      T* out = static_cast<T*>(w.ctx) + (static_cast<size_t>(start + q0 + 32 * quarter) * w.heads + h) * D;
       bool finite = true;
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int c = 0; c < D / 2; c += 32) {
         uint32_t o[32];
         if (active) {
-          tmem_ld_32x32b_x32(trow + C::O_COL + c, o);
+          tmem_ld_32x32b_x32(trow + C::O_COL + half * (D / 2) + c, o);
           tmem_wait_ld();
         }
-        if (c + 32 == D) {  // the slot's TMEM may be overwritten
+        if (c + 32 == D / 2) {  // the slot's TMEM may be overwritten
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(sfree);
         }
-        if (mine) {
+        if (active) {
+          constexpr int kSlots = C::SEG / 16, kShift = kSlots == 4 ? 1 : 2;  // 16-byte slots of a staged row
+          constexpr int kRowsPerIns = 32 / kSlots;
+          auto slot_at = [&](int row, int q) {
+            return stage + row * C::SEG + ((q ^ ((row >> kShift) & (kSlots - 1))) << 4);
+          };
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float v[8];
+          for (int c1 = 0; c1 < 32; c1 += C::SEG / 2) {  // columns staged at once
+            __syncwarp();  // the staged rows before have been read
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              v[i] = __uint_as_float(o[8 * q + i]) * inv;
-              finite = finite && fabsf(v[i]) < INFINITY;
+            for (int q = 0; q < kSlots; ++q) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float a = __uint_as_float(o[c1 + 8 * q + 2 * i]) * inv;
+                const float b = __uint_as_float(o[c1 + 8 * q + 2 * i + 1]) * inv;
+                finite = finite && fabsf(a) < INFINITY && fabsf(b) < INFINITY;
+                pk[i] = pack16<H16>(a, b);
+              }
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot_at(lane, q)), "r"(pk[0]), "r"(pk[1]),
+                           "r"(pk[2]), "r"(pk[3])
+                           : "memory");
             }
-            *reinterpret_cast<uint4*>(out + c + 8 * q) =
-                make_uint4(pack16<H16>(v[0], v[1]), pack16<H16>(v[2], v[3]), pack16<H16>(v[4], v[5]),
-                           pack16<H16>(v[6], v[7]));
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) {
+              const int row = i * kRowsPerIns + lane / kSlots, q = lane % kSlots;
+              uint32_t v0, v1, v2, v3;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(v0), "=r"(v1), "=r"(v2), "=r"(v3)
+                           : "r"(slot_at(row, q))
+                           : "memory");
+              if (row < rows)
+                *reinterpret_cast<uint4*>(out + static_cast<size_t>(row) * w.heads * D + half * (D / 2) + c + c1 + 8 * q) =
+                    make_uint4(v0, v1, v2, v3);
+            }
           }
         }
       }
-      if (mine && !finite) window_row_exact<T, D>(w, start, n, h, qi);
+      __syncwarp();
+      if (mine && !finite) window_row_exact<T, D>(w, start, n, h, qi, half * (D / 2), (half + 1) * (D / 2));
     }
   }
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag && p.err) atomicOr(p.err, kErrTimeout);
-  if (warp == 2) {
+  if (warp == 3) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(*tslot, 512);
@@ -758,9 +865,10 @@ cudaError_t launch_tc(const WindowArgs& a, WinParams w, cudaStream_t s, std::str
   p.kq = queries_per_item(a);
   w.q_blocks = (a.max_len + p.kq - 1) / p.kq;
   p.w = w;
-  p.items = static_cast<long long>(a.batch) * w.q_blocks * a.heads;
+  p.batch = a.batch;
   p.err = a.err;
-  const int grid = static_cast<int>(std::min<long long>(num_sms(dev), p.items));
+  const long long most = static_cast<long long>(a.batch) * w.q_blocks * a.heads;
+  const int grid = static_cast<int>(std::min<long long>(num_sms(dev), most));
   kern<<<grid, kTcThreads, TcCfg<D>::SMEM, s>>>(p, tm64, tm16);
   return cudaGetLastError();
 }
