@@ -643,7 +643,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         block_of(nv, nb, j, v0, v1);
         if (!warp_mbar_wait(sfull, bc & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        if (active) {
+        if (active && !H16 && nb == 1) {
+          // The reference is the row's score with its own key, which it always
+          // sees: bf16 P has f32's range, so any reference within 2^100 of the
+          // maximum gives the same relative rounding, and no maximum is needed.
+          // (p beyond f32 makes the outputs not finite: window_row_exact.)
+          const int d0 = q0 + 32 * quarter - k_begin;  // lane 0's own column
+          const int col = min(d0, 256 - 32);           // inside the slot's columns
+          uint32_t s[32];
+          tmem_ld_32x32b_x32(trow + col, s);
+          const int at = min(lane + d0 - col, 31);
+          tmem_wait_ld();
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < o; ++i) s[i] = at & o ? s[i + o] : s[i];
+          mref = mine ? __uint_as_float(s[0]) * w.scale_log2 : 0.f;
+        } else if (active) {
           float mx = -INFINITY;
 #pragma unroll 1
           for (int c = 32 * half; c < v1 - v0; c += 64) {
@@ -688,7 +704,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               if (up) mref = mb;
             }
           }
-          float l0 = 0.f, l1 = 0.f;
+        }
+        if (active) {
+          float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll 1
           for (int c = 32 * half; c < v1 - v0; c += 64) {
             const uint32_t bits = visible(v0 + c);
@@ -709,15 +727,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                   if (!(bits >> i & 1)) z.x = -INFINITY;
                   if (!(bits >> (i + 1) & 1)) z.y = -INFINITY;
                 }
-                const float p0 = ex2_approx(z.x), p1 = ex2_approx(z.y);
-                l0 += p0;
-                l1 += p1;
-                pk[i >> 1] = pack16<H16>(p0, p1);
+                const float2 e2 = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+                l2 = __fadd2_rn(l2, e2);
+                pk[i >> 1] = pack16<H16>(e2.x, e2.y);
               }
             }
             tmem_st_32x32b_x16(trow + p_col(c >> 4), pk);
           }
-          l += l0 + l1;
+          l += l2.x + l2.y;
           tmem_wait_st();
         }
         // V rows [nw, nw16) belong to no key of the item: their product with
