@@ -647,6 +647,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // The reference is the row's score with its own key, which it always
           // sees: bf16 P has f32's range, so any reference within 2^100 of the
           // maximum gives the same relative rounding, and no maximum is needed.
+          // Both warps of a row read it.
           // (p beyond f32 makes the outputs not finite: window_row_exact.)
           const int d0 = q0 + 32 * quarter - k_begin;  // lane 0's own column
           const int col = min(d0, 256 - 32);           // inside the slot's columns
@@ -659,6 +660,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int i = 0; i < o; ++i) s[i] = at & o ? s[i + o] : s[i];
           mref = mine ? __uint_as_float(s[0]) * w.scale_log2 : 0.f;
+          // the column may lie in a piece that the other warp overwrites with P
+          tc_fence_before();
+          if (!meet()) { ok = false; break; }
+          tc_fence_after();
         } else if (active) {
           float mx = -INFINITY;
 #pragma unroll 1
