@@ -105,13 +105,25 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _F32 = (torch.float32,)
 
 
-def _call(fn, device, *args):
+# The current stream's handle without building a Stream object (3 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_entry = {}
+
+
+def _call(name, device, *args):
     """One library call on ``device`` and its current torch stream."""
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(lib(), name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status)
 
 
 def _rms_args(x, gamma, residual):
@@ -132,7 +144,7 @@ def rmsnorm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=None):
     y = torch.empty_like(x)
     h = None if residual is None else torch.empty_like(x)
     if R:
-        _call(lib().jb_op_rmsnorm, x.device, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), y.data_ptr(),
+        _call("jb_op_rmsnorm", x.device, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), y.data_ptr(),
               None, None, _DT[x.dtype], R, C, eps)
     return y if h is None else (y, h)
 
@@ -143,11 +155,11 @@ def rmsnorm_quantize(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=
     The unrounded f32 norm is quantised; a row that is not finite has scale NaN and q 0."""
     _rms_args(x, gamma, residual)
     R, C = x.shape
-    q = torch.empty((R, C), dtype=torch.int8, device=x.device)
-    scale = torch.empty((R,), dtype=torch.float32, device=x.device)
+    q = x.new_empty((R, C), dtype=torch.int8)
+    scale = x.new_empty((R,), dtype=torch.float32)
     h = None if residual is None else torch.empty_like(x)
     if R:
-        _call(lib().jb_op_rmsnorm, x.device, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), None,
+        _call("jb_op_rmsnorm", x.device, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), None,
               q.data_ptr(), scale.data_ptr(), _DT[x.dtype], R, C, eps)
     return (q, scale) if h is None else (q, scale, h)
 
@@ -160,9 +172,9 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) 
     _check("scale", scale, q.shape[:1], _F32, q.device)
     if dtype not in _FLOATS:
         raise ValueError(f"{dtype} is not one of {', '.join(map(str, _FLOATS))}")
-    y = torch.empty(q.shape, dtype=dtype, device=q.device)
+    y = q.new_empty(q.shape, dtype=dtype)
     if q.shape[0]:
-        _call(lib().jb_op_dequantize_rows, q.device, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype],
+        _call("jb_op_dequantize_rows", q.device, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype],
               q.shape[0], q.shape[1])
     return y
 
@@ -182,10 +194,10 @@ def quantize_mxfp4(x: torch.Tensor):
     if x.dim() != 2 or x.shape[1] % 32 or not x.shape[1]:
         raise ValueError("x must be [rows, cols] with cols a multiple of 32")
     R, C = x.shape
-    q = torch.empty((R, C // 2), dtype=torch.uint8, device=x.device)
-    scale = torch.empty(_mx_scale_shape(R, C), dtype=torch.uint8, device=x.device)
+    q = x.new_empty((R, C // 2), dtype=torch.uint8)
+    scale = q.new_empty(_mx_scale_shape(R, C))
     if R:
-        _call(lib().jb_op_quantize_mxfp4, x.device, x.data_ptr(), _DT[x.dtype], q.data_ptr(), scale.data_ptr(), R, C)
+        _call("jb_op_quantize_mxfp4", x.device, x.data_ptr(), _DT[x.dtype], q.data_ptr(), scale.data_ptr(), R, C)
     return q, scale
 
 
@@ -202,9 +214,9 @@ def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16)
     if dtype not in _FLOATS:
         raise ValueError(f"{dtype} is not one of {', '.join(map(str, _FLOATS))}")
     R, C = q.shape[0], 2 * q.shape[1]
-    y = torch.empty((R, C), dtype=dtype, device=q.device)
+    y = q.new_empty((R, C), dtype=dtype)
     if R:
-        _call(lib().jb_op_dequantize_mxfp4, q.device, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype], R, C)
+        _call("jb_op_dequantize_mxfp4", q.device, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype], R, C)
     return y
 
 
@@ -223,9 +235,9 @@ def linear_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w_sc
         raise ValueError(f"{out_dtype} is not one of {', '.join(map(str, _FLOATS))}")
     _check("bias", bias, wq.shape[:1], _F32, dev, optional=True)
     _check("residual", residual, (M, N), (out_dtype,), dev, optional=True)
-    c = torch.empty((M, N), dtype=out_dtype, device=dev)
+    c = aq.new_empty((M, N), dtype=out_dtype)
     if M:
-        _call(lib().jb_op_linear_mxfp4, dev, aq.data_ptr(), a_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
+        _call("jb_op_linear_mxfp4", dev, aq.data_ptr(), a_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
               _p(bias), _p(residual), c.data_ptr(), _DT[out_dtype], M, N, K, epilogue)
     return c
 
@@ -266,8 +278,8 @@ def attention_window(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, ma
     if cu_seqlens.dim() != 1 or not cu_seqlens.numel():
         raise ValueError("cu_seqlens must be [batch + 1]")
     T, d = qkv.shape[0], qkv.shape[1] // (heads + 2 * kv_heads)
-    ctx = torch.empty((T, heads * d), dtype=qkv.dtype, device=qkv.device)
-    _call(lib().jb_op_attention_window, qkv.device, qkv.data_ptr(), cu_seqlens.data_ptr(), ctx.data_ptr(),
+    ctx = qkv.new_empty((T, heads * d))
+    _call("jb_op_attention_window", qkv.device, qkv.data_ptr(), cu_seqlens.data_ptr(), ctx.data_ptr(),
           _DT[qkv.dtype], cu_seqlens.numel() - 1, heads, kv_heads, d, max_len, T, left, right, sinks)
     return ctx
 
