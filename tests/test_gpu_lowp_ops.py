@@ -464,6 +464,19 @@ def test_attention_window_heads(dev, h, hk, d, left, right, sinks, dt):
     window_check(got, qkv, lens, h, hk, left, right, sinks, t != torch.float32)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("h,hk,d", [(12, 12, 64), (6, 3, 64), (8, 4, 128)])
+@pytest.mark.parametrize("left,right,sinks", [(64, 64, 1), (64, 64, 0), (300, 20, 4)])
+@pytest.mark.parametrize("batch,lo,hi", [(256, 32, 256), (40, 0, 700), (2100, 1, 20)])
+def test_attention_window_many_rows(dev, batch, lo, hi, left, right, sinks, h, hk, d, dt):
+    """More query blocks than any GPU has slots for: every slot works through several, of mixed
+    sizes; 2100 rows pass the kernel's table of row offsets."""
+    t = DTYPES[dt]
+    lens = torch.randint(lo, hi + 1, (batch,), generator=torch.Generator().manual_seed(batch)).tolist()
+    qkv, got = run_window(dev, lens, h, hk, d, t, left, right, sinks, batch + left + d)
+    window_check(got, qkv, lens, h, hk, left, right, sinks, t != torch.float32)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 def test_attention_window_long_rows_and_large_scores(dev, dt):
     t, lens = DTYPES[dt], [5000, 17, 2049]
