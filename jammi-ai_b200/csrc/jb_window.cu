@@ -196,21 +196,20 @@ cudaError_t launch_simt_d(WinParams p, int batch, int max_len, cudaStream_t s, s
   window_simt_kernel<T, D><<<static_cast<unsigned>(grid), kSimtThreads, 0, s>>>(p);
   return cudaGetLastError();
 }
+// 16-bit rows of head_dim 32 and more run on the tensor cores.
 template <typename T>
 cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaStream_t s, std::string* why) {
-  switch (d) {
-    case 8: return launch_simt_d<T, 8>(p, batch, max_len, s, why);
-    case 16: return launch_simt_d<T, 16>(p, batch, max_len, s, why);
-    case 32: return launch_simt_d<T, 32>(p, batch, max_len, s, why);
-    case 64: return launch_simt_d<T, 64>(p, batch, max_len, s, why);
-    case 128: return launch_simt_d<T, 128>(p, batch, max_len, s, why);
-    default:
-      if (why) *why = "attention_window: head_dim must be 8, 16, 32, 64 or 128";
-      return cudaErrorInvalidValue;
+  if (d == 8) return launch_simt_d<T, 8>(p, batch, max_len, s, why);
+  if (d == 16) return launch_simt_d<T, 16>(p, batch, max_len, s, why);
+  if constexpr (sizeof(T) == 4) {
+    if (d == 32) return launch_simt_d<T, 32>(p, batch, max_len, s, why);
+    if (d == 64) return launch_simt_d<T, 64>(p, batch, max_len, s, why);
+    if (d == 128) return launch_simt_d<T, 128>(p, batch, max_len, s, why);
   }
+  return cudaErrorInvalidValue;
 }
 
-// ── tcgen05, 16-bit rows with head_dim 64 or 128 ────────────────────────────
+// ── tcgen05, 16-bit rows with head_dim 32, 64 or 128 ────────────────────────
 // A persistent CTA per SM runs two independent slots, each on its own items
 // (row, head, kq-query block) with its own shared memory and half of TMEM:
 //   TMA warp      publishes the slot's items in a two-entry ring and loads
@@ -227,8 +226,8 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 //                 whole row segments.
 // The keys of an item are its window [k_begin, k_end), padded to 16, then the
 // first keys [0, s_end) that the window has left behind, padded to 16.  With
-// head_dim 64, an item of up to 256 keys is ONE block: no running maximum, no
-// rescaling, three hand-overs in all (S, P, O); O takes the columns of pieces
+// head_dim 32 or 64, an item of up to 256 keys is ONE block: no running maximum, no
+// rescaling, three hand-overs in all (S, P, O); O takes columns of pieces
 // 6 and 7 once every score is read, and their P goes to the free halves of
 // pieces 0 and 1.  That covers windows of up to left + right = 128 around 128
 // queries (and 112 queries with up to 16 sinks), the case this operator is
@@ -255,17 +254,21 @@ constexpr float kRescale = 8.f;   // lazy-rescaling threshold, log2 units
 
 template <int D>
 struct TcCfg {
-  static constexpr int HALVES = D / 64;                    // 64-element column blocks (128 bytes)
-  static constexpr int KEYS = D == 64 ? 256 : 128;         // key rows of a K or V buffer
-  static constexpr int Q_BYTES = HALVES * 128 * 128;
-  static constexpr int KV_BYTES = HALVES * KEYS * 128;
+  static constexpr int ROW = D == 32 ? 64 : 128;           // bytes of a swizzled shared-memory row
+  static constexpr int HCOLS = ROW / 2;                    // its elements
+  static constexpr int HALVES = D / HCOLS;                 // column blocks of a head
+  static constexpr int KEYS = D == 128 ? 128 : 256;        // key rows of a K or V buffer
+  static constexpr int Q_BYTES = HALVES * 128 * ROW;
+  static constexpr int KV_BYTES = HALVES * KEYS * ROW;
   static constexpr int SLOT_BYTES = Q_BYTES + 2 * KV_BYTES;
   static constexpr int O_COL = 256 - D;                    // O's columns of a slot
   static constexpr int SEG = D == 64 ? 64 : 32;            // bytes of a row that a warp stores at once
   static constexpr int STAGE_BYTES = 2 * kGroupWarps * 32 * SEG;
   static constexpr int XCH_BYTES = 2 * (2 + 1) * 4 * 2 * 32 * 4;  // [slot][max 0, max 1, sum][quarter][half][lane]
   static constexpr int META_BYTES = 512;
-  static constexpr int SMEM = 1024 + 2 * SLOT_BYTES + STAGE_BYTES + XCH_BYTES + (kPrefixRows + 4) * 4 + META_BYTES;
+  static constexpr int USED = 1024 + 2 * SLOT_BYTES + STAGE_BYTES + XCH_BYTES + (kPrefixRows + 4) * 4 + META_BYTES;
+  // more than half of an SM's: two CTAs cannot share its TMEM
+  static constexpr int SMEM = USED > 120 * 1024 ? USED : 120 * 1024;
   static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -344,6 +347,16 @@ __device__ __noinline__ void window_row_exact(const WinParams& p, int start, int
     }
     for (int d = 0; d < 16; ++d) out[c + d] = from_f<T>(o[d] / l);
   }
+}
+
+// Descriptor of a K-major (or, for V, MN-major) tile of 64- or 128-byte
+// swizzled rows: 8-row groups contiguous.
+template <int ROW>
+__device__ __forceinline__ uint64_t tile_desc(uint32_t smem_addr) {
+  if constexpr (ROW == 128) return umma_desc_sw128(smem_addr);
+  return static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(1) << 16) |
+         (static_cast<uint64_t>(8 * ROW >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+         (static_cast<uint64_t>(4) << 61);  // SWIZZLE_64B
 }
 
 template <int D, bool H16>
@@ -485,12 +498,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               const bool big = stop - v >= 64;
 #pragma unroll
               for (int half = 0; half < C::HALVES; ++half)
-                tma_load_2d(dst + half * (C::KEYS * 128) + (v - v0) * 128, big ? &tm64 : &tm16, x + 64 * half, y, bar);
+                tma_load_2d(dst + half * (C::KEYS * C::ROW) + (v - v0) * C::ROW, big ? &tm64 : &tm16,
+                            x + C::HCOLS * half, y, bar);
               v += big ? 64 : 16;
             }
           };
           if (bc > 0 && !warp_mbar_wait(sfull, (bc - 1) & 1, abort_flag)) { ok = false; break; }
-          const uint32_t bytes = static_cast<uint32_t>(v1 - v0) * 128 * C::HALVES;
+          const uint32_t bytes = static_cast<uint32_t>(v1 - v0) * C::ROW * C::HALVES;
           const int boxes = (min(it.n - it.q0, p.kq) + 63) >> 6;
           if (elect_one()) {
             if (j == 0) {
@@ -498,11 +512,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               e.live = 1; e.start = it.start; e.n = it.n; e.h = it.h; e.q0 = it.q0;
               e.k_begin = it.k_begin; e.nw = it.nw; e.s_end = it.s_end; e.nb = it.nb;
               mbar_arrive(ifull + 8 * (m & 1));
-              mbar_arrive_expect_tx(kfull, bytes + boxes * 64 * 128 * C::HALVES);
+              mbar_arrive_expect_tx(kfull, bytes + boxes * 64 * C::ROW * C::HALVES);
               for (int i = 0; i < boxes; ++i)
 #pragma unroll
                 for (int half = 0; half < C::HALVES; ++half)
-                  tma_load_2d(sQ + half * (128 * 128) + i * (64 * 128), &tm64, it.h * D + 64 * half,
+                  tma_load_2d(sQ + half * (128 * C::ROW) + i * (64 * C::ROW), &tm64, it.h * D + C::HCOLS * half,
                               it.start + it.q0 + 64 * i, kfull);
             } else {
               mbar_arrive_expect_tx(kfull, bytes);
@@ -538,7 +552,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
   } else if (warp < 4) {  // ── MMA
-    const uint32_t idesc_pv = (H16 ? idesc_f16_f32(128, 64) : idesc_bf16_f32(128, 64)) | (1u << 16);  // V MN-major
+    const uint32_t idesc_pv =
+        (H16 ? idesc_f16_f32(128, C::HCOLS) : idesc_bf16_f32(128, C::HCOLS)) | (1u << 16);  // V MN-major
     int bc = 0;
     bool ok = true;
     for (int m = 0; ok; ++m) {
@@ -562,10 +577,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (elect_one()) {
 #pragma unroll
           for (int half = 0; half < C::HALVES; ++half) {
-            const uint64_t dq = umma_desc_sw128(sQ + half * (128 * 128));
-            const uint64_t dk = umma_desc_sw128(sK + half * (C::KEYS * 128));
+            const uint64_t dq = tile_desc<C::ROW>(sQ + half * (128 * C::ROW));
+            const uint64_t dk = tile_desc<C::ROW>(sK + half * (C::KEYS * C::ROW));
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem, dq + 2u * kk, dk + 2u * kk, idesc, (half | kk) != 0);
+            for (int kk = 0; kk < C::HCOLS / 16; ++kk) mma_bf16(tmem, dq + 2u * kk, dk + 2u * kk, idesc, (half | kk) != 0);
           }
           mma_commit(sfull);
         }
@@ -579,11 +594,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (elect_one()) {
 #pragma unroll
           for (int half = 0; half < C::HALVES; ++half) {
-            const uint64_t dv = umma_desc_sw128(sV + half * (C::KEYS * 128));
+            const uint64_t dv = tile_desc<C::ROW>(sV + half * (C::KEYS * C::ROW));
 #pragma unroll
             for (int c = 0; c < C::KEYS / 16; ++c)
               if (c < steps)
-                mma_bf16_ta(tmem + C::O_COL + 64 * half, tmem + p_col(c), dv + 128u * c, idesc_pv,
+                mma_bf16_ta(tmem + C::O_COL + C::HCOLS * half, tmem + p_col(c), dv + static_cast<uint32_t>(C::ROW) * c, idesc_pv,
                             (j > 0 || c > 0) ? 1u : 0u);
           }
           mma_commit(ofull);
@@ -723,15 +738,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               uint32_t s[32];
               tmem_ld_32x32b_x32(trow + c, s);
               tmem_wait_ld();
-              const bool full = __all_sync(0xffffffffu, bits == 0xffffffffu);
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
                 float2 z = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
                                       f2(w.scale_log2), f2(-mref));
-                if (!full) {
-                  if (!(bits >> i & 1)) z.x = -INFINITY;
-                  if (!(bits >> (i + 1) & 1)) z.y = -INFINITY;
-                }
+                // (a second, unmasked copy of this code is slower: it does not fit
+                // the instruction cache beside the rest)
+                if (!(bits >> i & 1)) z.x = -INFINITY;
+                if (!(bits >> (i + 1) & 1)) z.y = -INFINITY;
                 const float2 e2 = make_float2(ex2_approx(z.x), ex2_approx(z.y));
                 l2 = __fadd2_rn(l2, e2);
                 pk[i >> 1] = pack16<H16>(e2.x, e2.y);
@@ -746,10 +760,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // P = 0 must be 0
         if (nw16 > nw && nw16 > v0 && nw16 <= v1) {
           if (!warp_mbar_wait(vfull, bc & 1, abort_flag)) { ok = false; break; }
-          for (int i = r + 128 * half; i < (nw16 - nw) * 8 * C::HALVES; i += 256) {
-            const int row = i >> 3, blk = row / (nw16 - nw);
-            const uint32_t a = sV + blk * (C::KEYS * 128) +
-                               static_cast<uint32_t>(nw - v0 + row - blk * (nw16 - nw)) * 128 + (i & 7) * 16;
+          constexpr int kChunks = C::ROW / 16;
+          for (int i = r + 128 * half; i < (nw16 - nw) * kChunks * C::HALVES; i += 256) {
+            const int row = i / kChunks, blk = row / (nw16 - nw);
+            const uint32_t a = sV + blk * (C::KEYS * C::ROW) +
+                               static_cast<uint32_t>(nw - v0 + row - blk * (nw16 - nw)) * C::ROW + i % kChunks * 16;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory");
           }
           fence_proxy_async_smem();
@@ -759,26 +774,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive(pfull);
       }
       if (!ok) break;
-      float inv = 0.f;
+      float inv = 0.f, l_row = 0.f;
       if (active) {
         float* xs = xq + 2 * 256;
         xs[32 * half] = l;
         if (!meet()) break;
-        inv = 1.f / (l + xs[32 * (half ^ 1)]);
+        l_row = l + xs[32 * (half ^ 1)];
+        inv = 1.f / l_row;
       }
       if (!warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag)) break;
       tc_fence_after();
-      // this thread's D / 2 columns, 32 at a time
+      // this thread's D / 2 columns, up to 32 at a time
+      constexpr int kCols = D / 2 < 32 ? D / 2 : 32;
       T* out = static_cast<T*>(w.ctx) + (static_cast<size_t>(start + q0 + 32 * quarter) * w.heads + h) * D;
-      bool finite = true;
+      float2 zero2 = make_float2(0.f, 0.f);  // sum of o * 0: NaN if any output is not finite
 #pragma unroll
-      for (int c = 0; c < D / 2; c += 32) {
-        uint32_t o[32];
+      for (int c = 0; c < D / 2; c += kCols) {
+        uint32_t o[kCols];
         if (active) {
-          tmem_ld_32x32b_x32(trow + C::O_COL + half * (D / 2) + c, o);
+          if constexpr (kCols == 16) tmem_ld_32x32b_x16(trow + C::O_COL + half * (D / 2) + c, o);
+          else tmem_ld_32x32b_x32(trow + C::O_COL + half * (D / 2) + c, o);
           tmem_wait_ld();
         }
-        if (c + 32 == D / 2) {  // the slot's TMEM may be overwritten
+        if (c + kCols == D / 2) {  // the slot's TMEM may be overwritten
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(sfree);
@@ -790,17 +808,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             return stage + row * C::SEG + ((q ^ ((row >> kShift) & (kSlots - 1))) << 4);
           };
 #pragma unroll
-          for (int c1 = 0; c1 < 32; c1 += C::SEG / 2) {  // columns staged at once
+          for (int c1 = 0; c1 < kCols; c1 += C::SEG / 2) {  // columns staged at once
             __syncwarp();  // the staged rows before have been read
 #pragma unroll
             for (int q = 0; q < kSlots; ++q) {
               uint32_t pk[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float a = __uint_as_float(o[c1 + 8 * q + 2 * i]) * inv;
-                const float b = __uint_as_float(o[c1 + 8 * q + 2 * i + 1]) * inv;
-                finite = finite && fabsf(a) < INFINITY && fabsf(b) < INFINITY;
-                pk[i] = pack16<H16>(a, b);
+                const float2 y = __fmul2_rn(make_float2(__uint_as_float(o[c1 + 8 * q + 2 * i]),
+                                                        __uint_as_float(o[c1 + 8 * q + 2 * i + 1])), f2(inv));
+                zero2 = __ffma2_rn(y, make_float2(0.f, 0.f), zero2);
+                pk[i] = pack16<H16>(y.x, y.y);
               }
               asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot_at(lane, q)), "r"(pk[0]), "r"(pk[1]),
                            "r"(pk[2]), "r"(pk[3])
@@ -823,7 +841,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       __syncwarp();
-      if (mine && !finite) window_row_exact<T, D>(w, start, n, h, qi, half * (D / 2), (half + 1) * (D / 2));
+      // a sum that is NaN has a NaN score in it: the outputs are NaN.  Else a
+      // value that the row does not see may be the one that is not finite.
+      if (mine && !(zero2.x + zero2.y == 0.f) && l_row == l_row) window_row_exact<T, D>(w, start, n, h, qi, half * (D / 2), (half + 1) * (D / 2));
     }
   }
   tc_fence_before();
@@ -836,9 +856,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
-// Map over qkv [rows, cols] of 16-bit elements with boxes of 64 columns (128
-// swizzled bytes) x box_rows.
-bool make_map(CUtensorMap* map, const void* qkv, bool h16, int rows, int cols, int box_rows) {
+// Map over qkv [rows, cols] of 16-bit elements with boxes of row_bytes (64 or
+// 128, swizzled) x box_rows.
+bool make_map(CUtensorMap* map, const void* qkv, bool h16, int rows, int cols, int row_bytes, int box_rows) {
   static const PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -850,17 +870,18 @@ bool make_map(CUtensorMap* map, const void* qkv, bool h16, int rows, int cols, i
   if (!enc) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
-  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(row_bytes / 2), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t estr[2] = {1, 1};
   return enc(map, h16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(qkv),
-             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Queries per item: 128, or fewer where that keeps a long row's window and
-// sinks inside one 256-key block (head_dim 64).
+// sinks inside one 256-key block (head_dim 32 or 64).
 int queries_per_item(const WindowArgs& a) {
-  if (a.head_dim != 64 || a.sinks == 0 || a.max_len <= 256) return 128;
+  if (a.head_dim == 128 || a.sinks == 0 || a.max_len <= 256) return 128;
   const long long spare = 256ll - a.left - a.right - ((a.sinks + 15ll) & ~15ll);
   return spare >= 128 || spare < 64 ? 128 : static_cast<int>(spare) & ~15;
 }
@@ -869,7 +890,8 @@ template <int D, bool H16>
 cudaError_t launch_tc(const WindowArgs& a, WinParams w, cudaStream_t s, std::string* why) {
   CUtensorMap tm64, tm16;
   const int cols = (a.heads + 2 * a.kv_heads) * D;
-  if (!make_map(&tm64, a.qkv, H16, a.rows, cols, 64) || !make_map(&tm16, a.qkv, H16, a.rows, cols, 16)) {
+  if (!make_map(&tm64, a.qkv, H16, a.rows, cols, TcCfg<D>::ROW, 64) ||
+      !make_map(&tm16, a.qkv, H16, a.rows, cols, TcCfg<D>::ROW, 16)) {
     if (why) *why = "attention_window: cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
@@ -914,13 +936,19 @@ cudaError_t launch_attention_window(const WindowArgs& a, cudaStream_t s, std::st
   switch (a.dtype) {
     case JB_DT_F32: return launch_simt<float>(p, a.head_dim, a.batch, a.max_len, s, why);
     case JB_DT_BF16:
-      if (a.head_dim == 64) return launch_tc<64, false>(a, p, s, why);
-      if (a.head_dim == 128) return launch_tc<128, false>(a, p, s, why);
-      return launch_simt<bf16>(p, a.head_dim, a.batch, a.max_len, s, why);
+      switch (a.head_dim) {
+        case 32: return launch_tc<32, false>(a, p, s, why);
+        case 64: return launch_tc<64, false>(a, p, s, why);
+        case 128: return launch_tc<128, false>(a, p, s, why);
+        default: return launch_simt<bf16>(p, a.head_dim, a.batch, a.max_len, s, why);
+      }
     case JB_DT_F16:
-      if (a.head_dim == 64) return launch_tc<64, true>(a, p, s, why);
-      if (a.head_dim == 128) return launch_tc<128, true>(a, p, s, why);
-      return launch_simt<f16>(p, a.head_dim, a.batch, a.max_len, s, why);
+      switch (a.head_dim) {
+        case 32: return launch_tc<32, true>(a, p, s, why);
+        case 64: return launch_tc<64, true>(a, p, s, why);
+        case 128: return launch_tc<128, true>(a, p, s, why);
+        default: return launch_simt<f16>(p, a.head_dim, a.batch, a.max_len, s, why);
+      }
     default: return cudaErrorInvalidValue;
   }
 }

@@ -456,7 +456,7 @@ def test_attention_window_64(dev, lens, left, right, sinks, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("h,hk,d", [(4, 2, 64), (6, 1, 64), (2, 2, 128), (4, 1, 128), (3, 3, 32), (4, 2, 16), (5, 5, 8)])
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 64), (6, 1, 64), (2, 2, 128), (4, 1, 128), (3, 3, 32), (4, 2, 32), (4, 2, 16), (5, 5, 8)])
 @pytest.mark.parametrize("left,right,sinks", [(64, 64, 1), (100, 0, 4), (2 ** 31 - 1, 2 ** 31 - 1, 0)])
 def test_attention_window_heads(dev, h, hk, d, left, right, sinks, dt):
     t, lens = DTYPES[dt], [200, 3, 0, 129, 391]
@@ -465,7 +465,7 @@ def test_attention_window_heads(dev, h, hk, d, left, right, sinks, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("h,hk,d", [(12, 12, 64), (6, 3, 64), (8, 4, 128)])
+@pytest.mark.parametrize("h,hk,d", [(12, 12, 64), (6, 3, 64), (8, 4, 128), (12, 12, 32)])
 @pytest.mark.parametrize("left,right,sinks", [(64, 64, 1), (64, 64, 0), (300, 20, 4)])
 @pytest.mark.parametrize("batch,lo,hi", [(256, 32, 256), (40, 0, 700), (2100, 1, 20)])
 def test_attention_window_many_rows(dev, batch, lo, hi, left, right, sinks, h, hk, d, dt):
