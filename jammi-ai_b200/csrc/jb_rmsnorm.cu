@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) rmsnorm_kernel(RmsArgs 
   constexpr int kLanes = 32 * W;  // lanes of a row
   // x, r of up to four vectors are fetched a row ahead; wider rows lean on
   // the other CTAs of the SM instead of on more registers
-  constexpr bool kAhead = W == 1 && MAXV * (RES ? 2 : 1) <= 8;
+  constexpr bool kAhead = MAXV * (RES ? 2 : 1) <= 8;
   __shared__ float red[W == 1 ? 1 : 2 * W];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int at = W == 1 ? lane : threadIdx.x;  // this thread's first vector
