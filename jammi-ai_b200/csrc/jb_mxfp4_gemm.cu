@@ -49,15 +49,19 @@ constexpr int kUnitCols = 64;      // columns of an epilogue warp
 constexpr int kUnitBytes = 4096;   // its box: 32 rows of 128 bytes (64 16-bit or 32 f32 columns)
 constexpr int kSfTile = 512;       // scale bytes of 128 rows x 128 columns
 
-template <int BN>
+// CG = 2: a cluster of two CTAs (two SMs of one TPC) shares a tile of 256 x BN
+// by tcgen05.mma.cta_group::2.  Each CTA holds 128 rows of A and of the
+// accumulator and half of W's rows; both hold the scales of all BN columns.
+template <int BN, int CG>
 struct MxCfg {
+  static constexpr int B_ROWS = BN / CG;
   static constexpr int A_BYTES = kBM * 128;
-  static constexpr int B_BYTES = BN * 128;
+  static constexpr int B_BYTES = B_ROWS * 128;
   // 128-row scale tiles that BN rows of W may touch (tiles start at multiples of BN)
   static constexpr int SFB_TILES = BN > 128 ? 2 : 1;
   static constexpr int SF_BYTES = 2 * kSfTile * (1 + SFB_TILES);
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SF_BYTES;
-  static constexpr int STAGES = BN == 192 ? 4 : BN == 128 ? 5 : 6;
+  static constexpr int STAGES = CG == 2 ? 5 : BN == 128 ? 5 : 6;
   static constexpr int SF_COLS = 8 * (1 + SFB_TILES);  // TMEM columns of a stage's scales
   static constexpr int TMEM_COLS = 512;  // all of it (one CTA per SM): the base is column 0
   static_assert(2 * BN + STAGES * SF_COLS <= TMEM_COLS, "TMEM columns");
@@ -69,8 +73,6 @@ struct MxCfg {
 };
 
 struct MxParams {
-  const uint8_t* a_scale;
-  const uint8_t* w_scale;
   const float* bias;
   int M, N, K;
   int* err;
@@ -81,27 +83,72 @@ enum Out { kBf16, kF16, kF32 };
 
 // D[tmem] (+)= A . B^T over K = 64 e2m1 elements, each block of 32 scaled by
 // the UE8M0 bytes at sfa / sfb.
+template <int CG>
 __device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                          uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-          d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
 }
 // 32 rows of 16 contiguous bytes -> 4 TMEM columns of lanes 0-31, repeated in
-// the other three lane quarters.
+// the other three lane quarters (CG = 2: in both CTAs, each from its own
+// shared memory).
+template <int CG>
 __device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-// Untiled bulk copy, 16-byte aligned, a multiple of 16 bytes.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-      : "memory");
+// Arrive on `bar` (CG = 2: on both CTAs' barriers at that offset) once every
+// tcgen05 operation issued so far by this thread has completed.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 1)
+    mma_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+// A box into this CTA's shared memory; its bytes count on `bar` (CG = 2: the
+// even CTA's barrier, a shared::cluster address).
+template <int CG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (CG == 1)
+    tma_load_2d(dst, map, x, y, bar);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+// The address of CTA 0's copy of a shared-memory variable of the cluster.
+__device__ __forceinline__ uint32_t of_cta0(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Descriptor of a scale tile: 8-row groups of 16-byte rows, 128 bytes apart,
 // no swizzle.
@@ -191,12 +238,13 @@ __device__ __forceinline__ void finish32(const uint32_t (&r)[32], uint32_t bias,
   }
 }
 
-template <int BN, int EPI, Out OUT>
-__global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
+template <int BN, int EPI, Out OUT, int CG>
+__global__ void __launch_bounds__(MxCfg<BN, CG>::THREADS, 1)
     gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                      const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                       const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
                       const MxParams p) {
-  using Cfg = MxCfg<BN>;
+  using Cfg = MxCfg<BN, CG>;
   constexpr bool kRes = EPI == JB_EPI_RESIDUAL;
   constexpr bool F32 = OUT == kF32;
   extern __shared__ uint8_t smem_raw[];
@@ -209,6 +257,7 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
   const uint32_t scales = boxes + Cfg::EPI_WARPS * kUnitBytes;
   const uint32_t biases = scales + Cfg::STAGES * Cfg::SF_BYTES;
   const uint32_t bars = biases + Cfg::EPI_WARPS * kUnitCols * 4;
+  // CG = 2: full and tempty of the even CTA count for the pair
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (Cfg::STAGES + s); };
   auto tfull_bar = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + i); };
@@ -220,8 +269,11 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform to the compiler too
   const int lane = threadIdx.x & 31;
+  int rank = 0;  // this CTA's half of the tile
+  if constexpr (CG == 2) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
   const int n_tiles = (p.N + BN - 1) / BN;
-  const int total = (p.M + kBM - 1) / kBM * n_tiles;
+  const int total = (p.M + CG * kBM - 1) / (CG * kBM) * n_tiles;
   const int kb_count = (p.K + kStageK - 1) / kStageK;
   const int k_tiles = (p.K + 127) / 128;  // scale tiles along K
 
@@ -232,22 +284,34 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull_bar(i), 1);
-      mbar_init(tempty_bar(i), Cfg::EPI_WARPS);
+      mbar_init(tempty_bar(i), CG * Cfg::EPI_WARPS);
     }
     mbar_init(spare, 1);
     for (int w = 0; w < Cfg::EPI_WARPS; ++w) mbar_init(res_bar(w), 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (CG == 1) {
+      tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(Cfg::TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+  }
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&tmA);
     prefetch_tensormap(&tmB);
+    prefetch_tensormap(&tmSA);
+    prefetch_tensormap(&tmSB);
     prefetch_tensormap(&tmC);
     if (kRes) prefetch_tensormap(&tmR);
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
   tc_fence_after();
   constexpr uint32_t tmem_base = 0;
 
@@ -257,41 +321,42 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
   // uniform register.  With one lane in `if (lane == 0)` a product of any width
   // takes about 250 clocks to issue; a 192-column product of K = 64 runs in 96.
   if (warp == 0) {  // ── producer
-    const int w_tiles = (p.N + 127) / 128;  // scale tiles along N
-    int it = 0, filled = 0;  // stages
+    int st = 0, filled = 0;
+    uint32_t ph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      const int mb = t / n_tiles, nb = t % n_tiles;
+    for (int t = first; t < total; t += step) {
+      const int mt = t / n_tiles * CG + rank, nb = t % n_tiles;  // rows in 128s, columns in BNs
       const int wt = nb * BN / 128;
-      const int w_copies = min(Cfg::SFB_TILES, w_tiles - wt);
-      const uint8_t* sfa_src = p.a_scale + static_cast<size_t>(mb) * k_tiles * kSfTile;
-      const uint8_t* sfb_src = p.w_scale + static_cast<size_t>(wt) * k_tiles * kSfTile;
-      for (int kb = 0; kb < kb_count; ++kb, ++it) {
-        const int st = it % Cfg::STAGES;
-        if (ok) ok = warp_mbar_wait(empty_bar(st), ((it / Cfg::STAGES) & 1) ^ 1u, abort_flag);
+#pragma unroll 1
+      for (int kb = 0; kb < kb_count; ++kb) {
+        if (ok) ok = warp_mbar_wait(empty_bar(st), ph ^ 1u, abort_flag);
         const uint32_t sa = base + st * (Cfg::A_BYTES + Cfg::B_BYTES);
         const uint32_t sf = scales + st * Cfg::SF_BYTES;
-        const uint32_t sf_bytes = min(2, k_tiles - 2 * kb) * kSfTile;
+        const uint32_t full = CG == 2 ? of_cta0(full_bar(st)) : full_bar(st);
         if (elect_one() && ok) {
-          mbar_arrive_expect_tx(full_bar(st), Cfg::A_BYTES + Cfg::B_BYTES + sf_bytes * (1 + w_copies));
-          tma_load_2d(sa, &tmA, kb * 128, mb * kBM, full_bar(st));
-          tma_load_2d(sa + Cfg::A_BYTES, &tmB, kb * 128, nb * BN, full_bar(st));
-          bulk_load(sf, sfa_src + 2 * kb * kSfTile, sf_bytes, full_bar(st));
-          bulk_load(sf + 2 * kSfTile, sfb_src + 2 * kb * kSfTile, sf_bytes, full_bar(st));
-          if (w_copies > 1)
-            bulk_load(sf + 4 * kSfTile, sfb_src + (k_tiles + 2 * kb) * static_cast<size_t>(kSfTile), sf_bytes,
-                      full_bar(st));
+          if (CG == 1 || rank == 0) mbar_arrive_expect_tx(full_bar(st), CG * Cfg::STAGE_BYTES);
+          load_box<CG>(sa, &tmA, kb * 128, mt * kBM, full);
+          load_box<CG>(sa + Cfg::A_BYTES, &tmB, kb * 128, nb * BN + rank * Cfg::B_ROWS, full);
+          // two K tiles of scales; past the last one: the next row's, which no product reads
+          load_box<CG>(sf, &tmSA, 0, (mt * k_tiles + 2 * kb) * 4, full);
+#pragma unroll
+          for (int i = 0; i < Cfg::SFB_TILES; ++i)
+            load_box<CG>(sf + 2 * kSfTile * (1 + i), &tmSB, 0, ((wt + i) * k_tiles + 2 * kb) * 4, full);
         }
         __syncwarp();
         filled += ok ? 1 : 0;
+        if (++st == Cfg::STAGES) {
+          st = 0;
+          ph ^= 1u;
+        }
       }
     }
-    if (*abort_flag) {  // copies in flight land before the CTA leaves (bounded)
+    if (*abort_flag && rank == 0) {  // the pair's copies in flight land before a CTA leaves (bounded)
       volatile int no_abort = 0;
       for (int b = max(0, filled - Cfg::STAGES); b < filled; ++b)
         mbar_wait(full_bar(b % Cfg::STAGES), (b / Cfg::STAGES) & 1, &no_abort);
     }
-  } else if (warp == 1) {  // ── MMA issuer
+  } else if (warp == 1) {  // ── MMA issuer (of the even CTA)
     constexpr uint32_t kStageDesc = (Cfg::A_BYTES + Cfg::B_BYTES) >> 4;  // descriptors count 16 bytes
     constexpr uint32_t kTileDesc = kSfTile >> 4;
     const uint64_t da0 = umma_desc_sw128(base), db0 = umma_desc_sw128(base + Cfg::A_BYTES);
@@ -299,7 +364,7 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
     int acc = 0, st = 0;
     uint32_t acc_ph = 0, ph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+    for (int t = rank == 0 ? first : total; t < total; t += step) {
       const uint32_t sf_shift = static_cast<uint32_t>((t % n_tiles) * BN % 128) / 32;
       if (ok) ok = warp_mbar_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag);
       tc_fence_after();
@@ -317,17 +382,17 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             if (2 * c < steps) {
-              tmem_cp_scales(tsa + 4 * c, ds + c * kTileDesc);
+              tmem_cp_scales<CG>(tsa + 4 * c, ds + c * kTileDesc);
 #pragma unroll
               for (int i = 0; i < Cfg::SFB_TILES; ++i)
-                tmem_cp_scales(tsb + 4 * (c * Cfg::SFB_TILES + i), ds + (2 * (1 + i) + c) * kTileDesc);
+                tmem_cp_scales<CG>(tsb + 4 * (c * Cfg::SFB_TILES + i), ds + (2 * (1 + i) + c) * kTileDesc);
             }
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             if (k < steps)
-              mma_mxf4(d_tmem, da + 2u * k, db + 2u * k, mx_idesc(kBM, BN, 2 * (k & 1)), tsa + 4 * (k >> 1),
-                       tsb + 4 * Cfg::SFB_TILES * (k >> 1) + sf_shift, (kb | k) != 0);
+              mma_mxf4<CG>(d_tmem, da + 2u * k, db + 2u * k, mx_idesc(CG * kBM, BN, 2 * (k & 1)), tsa + 4 * (k >> 1),
+                           tsb + 4 * Cfg::SFB_TILES * (k >> 1) + sf_shift, (kb | k) != 0);
         };
         const int steps = (p.K - kb * kStageK + 63) / 64;
         if (elect_one() && ok) {
@@ -335,8 +400,8 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
             products(4);
           else
             products(steps);
-          mma_commit(empty_bar(st));
-          if (kb == kb_count - 1) mma_commit(tfull_bar(acc));
+          commit<CG>(empty_bar(st));
+          if (kb == kb_count - 1) commit<CG>(tfull_bar(acc));
         }
         __syncwarp();
         if (++st == Cfg::STAGES) {
@@ -349,7 +414,7 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
     }
     if (!ok) {  // every MMA issued completes before TMEM is freed (bounded)
       volatile int no_abort = 0;
-      if (elect_one()) mma_commit(spare);
+      if (elect_one()) commit<CG>(spare);
       __syncwarp();
       warp_mbar_wait(spare, 0, &no_abort);
     }
@@ -363,14 +428,14 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
       return p.bias && col < p.N ? __ldg(p.bias + col) : 0.f;
     };
     float b0 = 0.f, b1 = 0.f;
-    if (static_cast<int>(blockIdx.x) < total) {
-      b0 = bias_at(blockIdx.x, lane);
-      b1 = bias_at(blockIdx.x, 32 + lane);
+    if (first < total) {
+      b0 = bias_at(first, lane);
+      b1 = bias_at(first, 32 + lane);
     }
     int acc = 0, loads = 0, waited = 0;  // residual boxes issued / seen
     uint32_t acc_ph = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      const int row0 = t / n_tiles * kBM + quarter * 32;
+    for (int t = first; t < total; t += step) {
+      const int row0 = (t / n_tiles * CG + rank) * kBM + quarter * 32;
       const int col0 = (t % n_tiles) * BN + part * kUnitCols;
       const bool live = col0 < p.N && row0 < p.M;  // warp-uniform
       auto load_res = [&](int c) {
@@ -385,9 +450,9 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
       if (kRes && live) load_res(0);
       asm volatile("st.shared.b32 [%0], %1;" ::"r"(bias + 4 * lane), "f"(b0) : "memory");
       asm volatile("st.shared.b32 [%0], %1;" ::"r"(bias + 4 * (32 + lane)), "f"(b1) : "memory");
-      if (t + static_cast<int>(gridDim.x) < total) {
-        b0 = bias_at(t + gridDim.x, lane);
-        b1 = bias_at(t + gridDim.x, 32 + lane);
+      if (t + step < total) {
+        b0 = bias_at(t + step, lane);
+        b1 = bias_at(t + step, 32 + lane);
       }
       __syncwarp();
       if (!warp_mbar_wait(tfull_bar(acc), acc_ph, abort_flag)) break;
@@ -400,7 +465,10 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(tempty_bar(acc));
+      if (lane == 0) {
+        if constexpr (CG == 2) arrive_cluster(of_cta0(tempty_bar(acc)));
+        else mbar_arrive(tempty_bar(acc));
+      }
       acc ^= 1;
       if (acc == 0) acc_ph ^= 1u;
       if (!live) continue;
@@ -465,11 +533,16 @@ __global__ void __launch_bounds__(MxCfg<BN>::THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // neither CTA leaves while the other one uses its memory
   if (threadIdx.x == 0 && *abort_flag && p.err) atomicOr(p.err, kErrTimeout);
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(*tmem_slot, Cfg::TMEM_COLS);
+    if constexpr (CG == 1)
+      tmem_dealloc(*tmem_slot, Cfg::TMEM_COLS);
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(Cfg::TMEM_COLS)
+                   : "memory");
   }
 }
 
@@ -487,9 +560,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 }
 
 // 2-D map over a dense [rows, cols] buffer with boxes of 128 bytes x box_rows,
-// 128-byte swizzle.
-bool make_map(CUtensorMap* map, CUtensorMapDataType type, int esz, const void* ptr, int rows, int cols,
-              int box_rows) {
+// 128-byte swizzle or none.
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, int esz, const void* ptr, long long rows, int cols,
+              int box_rows, bool swizzled = true) {
   auto enc = encoder();
   if (!enc) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
@@ -497,20 +570,26 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, int esz, const void* p
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / esz), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t estr[2] = {1, 1};
   return enc(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// Scale tiles as rows of 128 bytes, four to a tile, in boxes of two tiles.
+bool make_scale_map(CUtensorMap* map, const uint8_t* scale, int rows, int cols) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, scale, (rows + 127ll) / 128 * ((cols + 127) / 128) * 4, 128, 8,
+                  false);
+}
 
-template <int BN, int EPI, Out OUT>
+template <int BN, int EPI, Out OUT, int CG>
 cudaError_t launch_tile(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
-  using Cfg = MxCfg<BN>;
-  CUtensorMap ma, mb, mc, mr;
+  using Cfg = MxCfg<BN, CG>;
+  CUtensorMap ma, mb, msa, msb, mc, mr;
   const CUtensorMapDataType ct = OUT == kF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : OUT == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int esz = OUT == kF32 ? 4 : 2;
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  bool ok = make_map(&ma, u8, 1, g.aq, g.M, g.K / 2, kBM) && make_map(&mb, u8, 1, g.wq, g.N, g.K / 2, BN) &&
+  bool ok = make_map(&ma, u8, 1, g.aq, g.M, g.K / 2, kBM) && make_map(&mb, u8, 1, g.wq, g.N, g.K / 2, Cfg::B_ROWS) &&
+            make_scale_map(&msa, g.a_scale, g.M, g.K) && make_scale_map(&msb, g.w_scale, g.N, g.K) &&
             make_map(&mc, ct, esz, g.C, g.M, g.N, 32);
   mr = mc;  // unused without a residual
   if (ok && EPI == JB_EPI_RESIDUAL) ok = make_map(&mr, ct, esz, g.resid, g.M, g.N, 32);
@@ -518,7 +597,7 @@ cudaError_t launch_tile(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, 
     if (why) *why = "linear(mxfp4): cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  auto kern = gemm_mxfp4_kernel<BN, EPI, OUT>;
+  auto kern = gemm_mxfp4_kernel<BN, EPI, OUT, CG>;
   int dev = 0;
   cudaGetDevice(&dev);
   // the shared-memory opt-in is a property of each device's context
@@ -528,29 +607,39 @@ cudaError_t launch_tile(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, 
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev].store(1, std::memory_order_release);
   }
-  const long long tiles = ((g.M + kBM - 1ll) / kBM) * ((g.N + BN - 1) / BN);
-  const int grid = static_cast<int>(std::min<long long>(num_sms(dev), tiles));
-  kern<<<grid, Cfg::THREADS, Cfg::SMEM, s>>>(ma, mb, mc, mr, p);
-  return cudaGetLastError();
+  const long long tiles = ((g.M + CG * kBM - 1ll) / (CG * kBM)) * ((g.N + BN - 1) / BN);
+  const int grid = static_cast<int>(std::min<long long>(num_sms(dev) / CG, tiles)) * CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(Cfg::THREADS);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG == 1 ? 0 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, ma, mb, msa, msb, mc, mr, p);
 }
 
-template <int BN, Out OUT>
+template <int BN, Out OUT, int CG>
 cudaError_t launch_epi(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
   switch (g.epi) {
-    case JB_EPI_GELU: return launch_tile<BN, JB_EPI_GELU, OUT>(g, p, s, why);
-    case JB_EPI_QUICK_GELU: return launch_tile<BN, JB_EPI_QUICK_GELU, OUT>(g, p, s, why);
-    case JB_EPI_RESIDUAL: return launch_tile<BN, JB_EPI_RESIDUAL, OUT>(g, p, s, why);
-    default: return launch_tile<BN, JB_EPI_NONE, OUT>(g, p, s, why);
+    case JB_EPI_GELU: return launch_tile<BN, JB_EPI_GELU, OUT, CG>(g, p, s, why);
+    case JB_EPI_QUICK_GELU: return launch_tile<BN, JB_EPI_QUICK_GELU, OUT, CG>(g, p, s, why);
+    case JB_EPI_RESIDUAL: return launch_tile<BN, JB_EPI_RESIDUAL, OUT, CG>(g, p, s, why);
+    default: return launch_tile<BN, JB_EPI_NONE, OUT, CG>(g, p, s, why);
   }
 }
-template <int BN>
+template <int BN, int CG>
 cudaError_t launch_out(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, std::string* why) {
-  if (g.c_dtype == JB_DT_F16) return launch_epi<BN, kF16>(g, p, s, why);
+  if (g.c_dtype == JB_DT_F16) return launch_epi<BN, kF16, CG>(g, p, s, why);
   // f32 outputs hold 64 accumulators and 32 results: more than the 448
   // threads of BN = 192 have registers for
   if constexpr (BN < 192)
-    if (g.c_dtype == JB_DT_F32) return launch_epi<BN, kF32>(g, p, s, why);
-  return launch_epi<BN, kBf16>(g, p, s, why);
+    if (g.c_dtype == JB_DT_F32) return launch_epi<BN, kF32, CG>(g, p, s, why);
+  return launch_epi<BN, kBf16, CG>(g, p, s, why);
 }
 
 }  // namespace
@@ -562,13 +651,13 @@ cudaError_t launch_linear_mxfp4(const MxGemmArgs& g, cudaStream_t s, std::string
     if (why) *why = "linear(mxfp4): too many output tiles";
     return cudaErrorInvalidValue;
   }
-  MxParams p{g.a_scale, g.w_scale, g.bias, g.M, g.N, g.K, g.err};
+  MxParams p{g.bias, g.M, g.N, g.K, g.err};
   int dev = 0;
   cudaGetDevice(&dev);
   const long long sms = num_sms(dev);
-  if (m_tiles * ((g.N + 127) / 128) <= sms) return launch_out<64>(g, p, s, why);
-  if (g.c_dtype == JB_DT_F32 || m_tiles * ((g.N + 191) / 192) <= sms) return launch_out<128>(g, p, s, why);
-  return launch_out<192>(g, p, s, why);
+  if (m_tiles * ((g.N + 127) / 128) <= sms) return launch_out<64, 1>(g, p, s, why);
+  if (g.c_dtype == JB_DT_F32 || m_tiles * ((g.N + 191) / 192) <= sms) return launch_out<128, 1>(g, p, s, why);
+  return launch_out<192, 2>(g, p, s, why);
 }
 
 }  // namespace jb
