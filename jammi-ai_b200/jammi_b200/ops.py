@@ -84,26 +84,30 @@ def layernorm(x: torch.Tensor, gamma, beta, eps: float, residual=None) -> torch.
     return y
 
 
-def _check(name, t, shape=None, dtypes=None, device=None, optional=False):
-    """Raises ValueError unless ``t`` is a contiguous CUDA tensor of ``shape`` and one of
-    ``dtypes`` on ``device``."""
+def _refuse(name, t, shape, dtypes, index):
+    """The ValueError that says what ``_check`` found wrong."""
     if t is None:
-        if optional:
-            return
         raise ValueError(f"{name} is missing")
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise ValueError(f"{name} must be on {device or 'a CUDA device'}, not on {t.device}")
+    if not t.is_cuda or (index is not None and t.get_device() != index):
+        where = "a CUDA device" if index is None else f"cuda:{index}"
+        raise ValueError(f"{name} must be on {where}, not on {t.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    if dtypes is not None and t.dtype not in dtypes:
-        raise ValueError(f"{name}: {t.dtype} is not one of {', '.join(map(str, dtypes))}")
+    raise ValueError(f"{name}: {t.dtype} is not one of {', '.join(map(str, dtypes))}")
+
+
+def _check(name, t, shape, dtypes, index=None):
+    """Raises ValueError unless ``t`` is a contiguous CUDA tensor of ``shape`` (None: any) and one
+    of ``dtypes``, on device ``index`` (None: any)."""
+    if (t is None or t.dtype not in dtypes or not t.is_contiguous() or not t.is_cuda or
+            (shape is not None and t.shape != shape) or (index is not None and t.get_device() != index)):
+        _refuse(name, t, shape, dtypes, index)
 
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _F32 = (torch.float32,)
-
 
 # The current stream's handle without building a Stream object (3 us a call).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -111,40 +115,42 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _entry = {}
 
 
-def _call(name, device, *args):
-    """One library call on ``device`` and its current torch stream."""
+def _call(name, index, *args):
+    """One library call on device ``index`` and its current torch stream."""
     fn = _entry.get(name)
     if fn is None:
         fn = _entry[name] = getattr(lib(), name)
-    index = device.index
     if torch.cuda.current_device() == index:
         status = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             status = fn(*args, _raw_stream(index))
     if status:
         check(status)
 
 
 def _rms_args(x, gamma, residual):
-    if x.dim() != 2:
-        raise ValueError("x must be [rows, cols]")
-    dev = x.device
+    """The device index of a valid call."""
     _check("x", x, None, _FLOATS)
-    _check("gamma", gamma, x.shape[1:], _F32, dev)
-    _check("residual", residual, x.shape, (x.dtype,), dev, optional=True)
+    shape, index = x.shape, x.get_device()
+    if len(shape) != 2:
+        raise ValueError("x must be [rows, cols]")
+    _check("gamma", gamma, shape[1:], _F32, index)
+    if residual is not None:
+        _check("residual", residual, shape, (x.dtype,), index)
+    return index
 
 
 def rmsnorm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=None):
     """RMS norm of ``x`` [R, C] (+ ``residual``): ``s * rsqrt(mean(s^2) + eps) * gamma`` with
     ``s = x + residual`` in f32.  Returns y, or (y, s rounded to x's dtype) when a residual is
     given.  x f32, bf16 or f16; gamma f32 [C]."""
-    _rms_args(x, gamma, residual)
+    index = _rms_args(x, gamma, residual)
     R, C = x.shape
     y = torch.empty_like(x)
     h = None if residual is None else torch.empty_like(x)
     if R:
-        _call("jb_op_rmsnorm", x.device, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), y.data_ptr(),
+        _call("jb_op_rmsnorm", index, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), y.data_ptr(),
               None, None, _DT[x.dtype], R, C, eps)
     return y if h is None else (y, h)
 
@@ -153,13 +159,13 @@ def rmsnorm_quantize(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=
     """``rmsnorm`` with its output as per-row int8: (q int8 [R, C], scale f32 [R]) -- the
     activations of ``linear_s8`` -- and the rounded sum as a third value when a residual is given.
     The unrounded f32 norm is quantised; a row that is not finite has scale NaN and q 0."""
-    _rms_args(x, gamma, residual)
+    index = _rms_args(x, gamma, residual)
     R, C = x.shape
     q = x.new_empty((R, C), dtype=torch.int8)
     scale = x.new_empty((R,), dtype=torch.float32)
     h = None if residual is None else torch.empty_like(x)
     if R:
-        _call("jb_op_rmsnorm", x.device, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), None,
+        _call("jb_op_rmsnorm", index, x.data_ptr(), _p(residual), gamma.data_ptr(), _p(h), None,
               q.data_ptr(), scale.data_ptr(), _DT[x.dtype], R, C, eps)
     return (q, scale) if h is None else (q, scale, h)
 
@@ -169,12 +175,12 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) 
     _check("q", q, None, (torch.int8,))
     if q.dim() != 2:
         raise ValueError("q must be [rows, cols]")
-    _check("scale", scale, q.shape[:1], _F32, q.device)
+    _check("scale", scale, q.shape[:1], _F32, q.get_device())
     if dtype not in _FLOATS:
         raise ValueError(f"{dtype} is not one of {', '.join(map(str, _FLOATS))}")
     y = q.new_empty(q.shape, dtype=dtype)
     if q.shape[0]:
-        _call("jb_op_dequantize_rows", q.device, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype],
+        _call("jb_op_dequantize_rows", q.get_device(), q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype],
               q.shape[0], q.shape[1])
     return y
 
@@ -197,15 +203,15 @@ def quantize_mxfp4(x: torch.Tensor):
     q = x.new_empty((R, C // 2), dtype=torch.uint8)
     scale = q.new_empty(_mx_scale_shape(R, C))
     if R:
-        _call("jb_op_quantize_mxfp4", x.device, x.data_ptr(), _DT[x.dtype], q.data_ptr(), scale.data_ptr(), R, C)
+        _call("jb_op_quantize_mxfp4", x.get_device(), x.data_ptr(), _DT[x.dtype], q.data_ptr(), scale.data_ptr(), R, C)
     return q, scale
 
 
-def _check_mxfp4(name, q, scale, device=None):
-    _check(name, q, None, _U8, device)
+def _check_mxfp4(name, q, scale, index=None):
+    _check(name, q, None, _U8, index)
     if q.dim() != 2 or q.shape[1] % 16 or not q.shape[1]:
         raise ValueError(f"{name} must be [rows, cols / 2] with cols a multiple of 32")
-    _check(name + "'s scale", scale, _mx_scale_shape(q.shape[0], 2 * q.shape[1]), _U8, q.device)
+    _check(name + "'s scale", scale, _mx_scale_shape(q.shape[0], 2 * q.shape[1]), _U8, q.get_device())
 
 
 def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
@@ -216,7 +222,7 @@ def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16)
     R, C = q.shape[0], 2 * q.shape[1]
     y = q.new_empty((R, C), dtype=dtype)
     if R:
-        _call("jb_op_dequantize_mxfp4", q.device, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype], R, C)
+        _call("jb_op_dequantize_mxfp4", q.get_device(), q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype], R, C)
     return y
 
 
@@ -226,18 +232,20 @@ def linear_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w_sc
     ``quantize_mxfp4`` returns them; N a multiple of 8, ``out_dtype`` f32, bf16 or f16 (the
     residual's too), bias f32 [N]."""
     _check_mxfp4("aq", aq, a_scale)
-    dev = aq.device
-    _check_mxfp4("wq", wq, w_scale, dev)
+    index = aq.get_device()
+    _check_mxfp4("wq", wq, w_scale, index)
     if wq.shape[1] != aq.shape[1]:
         raise ValueError("aq and wq must have the same number of columns")
     M, N, K = aq.shape[0], wq.shape[0], 2 * aq.shape[1]
     if out_dtype not in _FLOATS:
         raise ValueError(f"{out_dtype} is not one of {', '.join(map(str, _FLOATS))}")
-    _check("bias", bias, wq.shape[:1], _F32, dev, optional=True)
-    _check("residual", residual, (M, N), (out_dtype,), dev, optional=True)
+    if bias is not None:
+        _check("bias", bias, wq.shape[:1], _F32, index)
+    if residual is not None:
+        _check("residual", residual, (M, N), (out_dtype,), index)
     c = aq.new_empty((M, N), dtype=out_dtype)
     if M:
-        _call("jb_op_linear_mxfp4", dev, aq.data_ptr(), a_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
+        _call("jb_op_linear_mxfp4", index, aq.data_ptr(), a_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
               _p(bias), _p(residual), c.data_ptr(), _DT[out_dtype], M, N, K, epilogue)
     return c
 
@@ -270,7 +278,7 @@ def attention_window(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, ma
     Rows behind ``cu_seqlens[-1]`` are left unwritten."""
     kv_heads = heads if kv_heads is None else kv_heads
     _check("qkv", qkv, None, _FLOATS)
-    _check("cu_seqlens", cu_seqlens, None, (torch.int32,), qkv.device)
+    _check("cu_seqlens", cu_seqlens, None, (torch.int32,), qkv.get_device())
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError("heads must be a positive multiple of kv_heads")
     if qkv.dim() != 2 or not qkv.shape[1] or qkv.shape[1] % (heads + 2 * kv_heads):
@@ -279,7 +287,7 @@ def attention_window(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, ma
         raise ValueError("cu_seqlens must be [batch + 1]")
     T, d = qkv.shape[0], qkv.shape[1] // (heads + 2 * kv_heads)
     ctx = qkv.new_empty((T, heads * d))
-    _call("jb_op_attention_window", qkv.device, qkv.data_ptr(), cu_seqlens.data_ptr(), ctx.data_ptr(),
+    _call("jb_op_attention_window", qkv.get_device(), qkv.data_ptr(), cu_seqlens.data_ptr(), ctx.data_ptr(),
           _DT[qkv.dtype], cu_seqlens.numel() - 1, heads, kv_heads, d, max_len, T, left, right, sinks)
     return ctx
 
