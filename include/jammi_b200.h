@@ -240,6 +240,12 @@ jb_status jb_op_quantize_rows_act(const void* x, int x_dtype, int activation, in
 jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamma,
                           const float* beta, void* y, int dtype, int rows, int cols,
                           float eps, void* stream);
+/* The entry points from here to jb_op_linear_mxfp4, and jb_op_attention_window,
+ * allocate nothing, share no memory between calls (concurrent calls and
+ * replayed graphs do not meet) and can be captured; the first
+ * jb_op_linear_mxfp4 or jb_op_attention_window on a device allocates that
+ * device's error flag, so make it before a capture.  Rows (M, N, batch) are
+ * below 2^31 - 2^20. */
 /* RMS norm over the last dim with the residual's addition: s = x (+ residual)
  * in f32, y = s * rsqrt(mean(s^2) + eps) * gamma.  `sum` (NULL unless a
  * residual is given; NULL: not wanted) receives s rounded to dtype, the next

@@ -555,10 +555,16 @@ jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamm
   });
 }
 
+namespace {
+// The kernels step through rows in 32 bits: a last step past the end must not wrap.
+constexpr int kMaxOpRows = INT32_MAX - (1 << 20);
+}  // namespace
+
 jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma, void* sum, void* y,
                         int8_t* q, float* scale, int dtype, int rows, int cols, float eps, void* stream) {
   return guarded([&] {
-    if (rows < 0 || cols <= 0) jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: rows must be >= 0 and cols > 0");
+    if (rows < 0 || rows > kMaxOpRows || cols <= 0)
+      jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: rows must be in 0 .. 2^31 - 2^20 - 1 and cols > 0");
     if (dtype != JB_DT_F32 && dtype != JB_DT_BF16 && dtype != JB_DT_F16)
       jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: dtype must be f32, bf16 or f16");
     if ((y != nullptr) == (q != nullptr) || (q != nullptr) != (scale != nullptr))
@@ -585,7 +591,8 @@ jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma,
 jb_status jb_op_dequantize_rows(const int8_t* q, const float* scale, void* y, int dtype, int rows, int cols,
                                 void* stream) {
   return guarded([&] {
-    if (rows < 0 || cols <= 0) jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: rows must be >= 0 and cols > 0");
+    if (rows < 0 || rows > kMaxOpRows || cols <= 0)
+      jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: rows must be in 0 .. 2^31 - 2^20 - 1 and cols > 0");
     if (dtype != JB_DT_F32 && dtype != JB_DT_BF16 && dtype != JB_DT_F16)
       jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: dtype must be f32, bf16 or f16");
     if (rows == 0) return;
@@ -602,8 +609,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 void check_mxfp4_rows(const char* op, const void* x, int dtype, const void* q, const void* scale, int rows,
                       int cols) {
   const std::string name = op;
-  if (rows < 0 || cols <= 0 || cols % 32)
-    jb::fail(JB_ERR_INVALID, name + ": rows must be >= 0 and cols a positive multiple of 32");
+  if (rows < 0 || rows > kMaxOpRows || cols <= 0 || cols % 32 || cols > (1 << 30))
+    jb::fail(JB_ERR_INVALID, name + ": rows must be in 0 .. 2^31 - 2^20 - 1 and cols a multiple of 32 up to 2^30");
   if (!is_float_dtype(dtype)) jb::fail(JB_ERR_INVALID, name + ": dtype must be f32, bf16 or f16");
   if (rows == 0) return;
   if (!x || !q || !scale) jb::fail(JB_ERR_INVALID, name + ": null buffer");
@@ -641,9 +648,10 @@ jb_status jb_op_linear_mxfp4(const uint8_t* Aq, const uint8_t* a_scale, const ui
   return guarded([&] {
     if (!is_float_dtype(c_dtype)) jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: C must be f32, bf16 or f16");
     if (epilogue < JB_EPI_NONE || epilogue > JB_EPI_RESIDUAL) jb::fail(JB_ERR_INVALID, "unknown epilogue");
-    if (M < 0 || N <= 0 || K <= 0 || K % 32 || N % 8)
+    if (M < 0 || M > kMaxOpRows || N <= 0 || N > kMaxOpRows || N % 8 || K <= 0 || K > (1 << 30) || K % 32)
       jb::fail(JB_ERR_INVALID,
-               "jb_op_linear_mxfp4: M must be >= 0, N a positive multiple of 8, K a positive multiple of 32");
+               "jb_op_linear_mxfp4: M must be >= 0, N a positive multiple of 8 (both below 2^31 - 2^20), K a multiple "
+               "of 32 up to 2^30");
     if ((epilogue == JB_EPI_RESIDUAL) != (residual != nullptr) && M > 0)
       jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: a residual and JB_EPI_RESIDUAL go together");
     if (M == 0) return;
@@ -718,8 +726,10 @@ jb_status jb_op_attention_window(const void* qkv, const int* cu_seqlens, void* c
                                  int kv_heads, int head_dim, int max_len, int rows, int left, int right, int sinks,
                                  void* stream) {
   return guarded([&] {
-    if (batch < 0 || heads <= 0 || kv_heads <= 0 || max_len < 0 || rows < 0)
-      jb::fail(JB_ERR_INVALID, "jb_op_attention_window: batch, max_len and rows must be >= 0, heads and kv_heads > 0");
+    if (batch < 0 || batch > kMaxOpRows || heads <= 0 || kv_heads <= 0 || max_len < 0 || rows < 0 || rows > kMaxOpRows)
+      jb::fail(JB_ERR_INVALID,
+               "jb_op_attention_window: batch, max_len and rows must be >= 0 (batch and rows below 2^31 - 2^20), heads "
+               "and kv_heads > 0");
     if (heads % kv_heads) jb::fail(JB_ERR_INVALID, "jb_op_attention_window: heads must be a multiple of kv_heads");
     if (!is_float_dtype(dtype)) jb::fail(JB_ERR_INVALID, "jb_op_attention_window: dtype must be f32, bf16 or f16");
     if (head_dim != 8 && head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128)

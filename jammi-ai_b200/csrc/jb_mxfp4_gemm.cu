@@ -647,8 +647,10 @@ cudaError_t launch_out(const MxGemmArgs& g, const MxParams& p, cudaStream_t s, s
 cudaError_t launch_linear_mxfp4(const MxGemmArgs& g, cudaStream_t s, std::string* why) {
   if (g.M == 0) return cudaSuccess;
   const long long m_tiles = (g.M + kBM - 1ll) / kBM;
-  if (m_tiles * ((g.N + 63) / 64) > INT32_MAX / 2) {
-    if (why) *why = "linear(mxfp4): too many output tiles";
+  // tile numbers, and scale rows (four to a scale tile) as TMA coordinates
+  const long long k_tiles = (g.K + 127) / 128;
+  if (m_tiles * ((g.N + 63) / 64) > INT32_MAX / 2 || (std::max<long long>(m_tiles, (g.N + 127ll) / 128) + 2) * k_tiles * 4 > INT32_MAX) {
+    if (why) *why = "linear(mxfp4): more tiles than 32 bits number";
     return cudaErrorInvalidValue;
   }
   MxParams p{g.bias, g.M, g.N, g.K, g.err};

@@ -543,3 +543,131 @@ def test_attention_window_refusals(dev):
     with pytest.raises(JbError):
         ops.attention_window(torch.ones((4, 3 * 24), device=dev), cu, 1, 4, 1, 1)  # head_dim 24
     assert ops.attention_window(qkv[:0], cu[:1], 1, 0, 4, 4).shape == (0, 64)
+
+
+# ── together ────────────────────────────────────────────────────────────────
+
+class Layer:
+    """A pre-norm encoder layer at low precision: x + r -> RMS norm -> int8 rows -> int8 QKV linear ->
+    windowed attention -> MXFP4 output linear added to the sum -> RMS norm -> MXFP4 FFN with GELU."""
+
+    H, HEADS, F = 256, 4, 1024
+
+    def __init__(self, seed):
+        ops, g = _ops(), _gen(seed)
+        H, F = self.H, self.F
+        rand = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+        self.g1, self.g2 = 1 + 0.1 * rand(H), 1 + 0.1 * rand(H)
+        self.qkv = ops.quantize_rows(rand(3 * H, H) / math.sqrt(H))
+        self.out = ops.quantize_mxfp4(rand(H, H) / math.sqrt(H))
+        self.up = ops.quantize_mxfp4(rand(F, H) / math.sqrt(H))
+        self.down = ops.quantize_mxfp4(rand(H, F) / math.sqrt(F))
+        self.b_up, self.b_down = 0.1 * rand(F), 0.1 * rand(H)
+
+    def __call__(self, x, r, cu, longest):
+        from jammi_b200 import _lib as L
+        ops = _ops()
+        q, s, h = ops.rmsnorm_quantize(x, self.g1, EPS, residual=r)
+        qkv = ops.linear_s8(q, s, *self.qkv, out_dtype=torch.bfloat16)
+        ctx = ops.attention_window(qkv, cu, self.HEADS, longest, 64, 64, sinks=1)
+        a = ops.linear_mxfp4(*ops.quantize_mxfp4(ctx), *self.out, residual=h, epilogue=L.EPI_RESIDUAL)
+        y = ops.rmsnorm(a, self.g2, EPS)
+        up = ops.linear_mxfp4(*ops.quantize_mxfp4(y), *self.up, bias=self.b_up, epilogue=L.EPI_GELU)
+        z = ops.linear_mxfp4(*ops.quantize_mxfp4(up), *self.down, bias=self.b_down, residual=a, epilogue=L.EPI_RESIDUAL)
+        return dict(h=h, q=q, s=s, qkv=qkv, ctx=ctx, a=a, y=y, up=up, z=z)
+
+
+def layer_inputs(lens, seed):
+    g = _gen(seed)
+    T = sum(lens)
+    x = torch.randn((T, Layer.H), generator=g, device="cuda").bfloat16()
+    r = torch.randn((T, Layer.H), generator=g, device="cuda").bfloat16()
+    cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
+    return x, r, cu
+
+
+LAYER_LENS = [70, 1, 300, 0, 12, 256]
+
+
+def test_layer_each_stage_on_what_it_got(dev):
+    """The whole run, every stage held to float64 of its own operator on the tensors that reached it."""
+    layer, (x, r, cu) = Layer(1), layer_inputs(LAYER_LENS, 2)
+    t = layer(x, r, cu, max(LAYER_LENS))
+    _ops().sync()
+    s, ref = rms_ref(x, layer.g1, r)
+    amax, rel = ref.abs().amax(1), rms_f32_error(sum_depth(Layer.H))
+    assert ((t["q"].double() - ref * (127 / amax)[:, None]).abs() <= 0.5 + 127 * (2 * rel + 2.0 ** -22)).all()
+    acc = t["q"].double() @ layer.qkv[0].double().T * t["s"].double()[:, None] * layer.qkv[1].double()
+    assert ((t["qkv"].double() - acc).abs() <= (2.0 ** -8 + 2.0 ** -22) * acc.abs()).all()
+    window_check(t["ctx"], t["qkv"], LAYER_LENS, Layer.HEADS, Layer.HEADS, 64, 64, 1, True)
+    value = lambda m: _ops().dequantize_mxfp4(*m, torch.float32).double()  # noqa: E731
+    linear_check(t["a"], mx_ref(t["ctx"])[0], value(layer.out), None, t["h"], "residual", Layer.H)
+    linear_check(t["up"], mx_ref(t["y"])[0], value(layer.up), layer.b_up, None, "gelu", Layer.H)
+    linear_check(t["z"], mx_ref(t["up"])[0], value(layer.down), layer.b_down, t["a"], "residual", Layer.F)
+
+
+def test_layer_captured_replayed_and_on_two_streams(dev):
+    """Two captured runs replayed at once on two streams, on new inputs copied into theirs, give the
+    eager runs' bits: nothing is kept from one call for the next, and nothing is shared."""
+    layer, lens = Layer(3), LAYER_LENS
+    runs = []
+    for k in range(2):
+        static = layer_inputs(lens, 10 + k)
+        layer(*static, max(lens))  # warm-up: attributes, the error flag
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = layer(*static, max(lens))
+        runs.append((static, stream, graph, out))
+    for turn in range(3):
+        fresh = [layer_inputs(lens, 100 + 10 * turn + k) for k in range(2)]
+        want = [layer(*f, max(lens)) for f in fresh]
+        torch.cuda.synchronize()
+        for (static, stream, graph, out), f in zip(runs, fresh):
+            with torch.cuda.stream(stream):
+                for a, b in zip(static, f):
+                    a.copy_(b)
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, _, out), w in zip(runs, want):
+            for k in w:
+                assert torch.equal(out[k], w[k]), k
+    _ops().sync()
+    del runs
+
+
+def test_ops_run_on_the_current_stream(dev):
+    """A call waits for the work before it on its own stream only."""
+    ops = _ops()
+    x = torch.zeros((4096, 1024), device=dev).bfloat16()
+    gamma = torch.ones(1024, device=dev)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            x.add_(1.0)
+        q, s = ops.rmsnorm_quantize(x, gamma, EPS)
+        m = ops.quantize_mxfp4(x)
+        y = ops.dequantize_mxfp4(*m, torch.float32)
+    side.synchronize()
+    assert (q == 127).all() and (y == 16.0).all()  # 20 / 4 = 5 ties to the even code 6: 4 * 4
+
+
+def test_window_two_calls_at_once_on_two_streams(dev):
+    ops = _ops()
+    lens = torch.randint(32, 257, (200,), generator=torch.Generator().manual_seed(1)).tolist()
+    cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32).to(dev)
+    qs = [torch.randn((sum(lens), 3 * 12 * 64), generator=_gen(k), device=dev).bfloat16() for k in range(2)]
+    want = [ops.attention_window(q, cu, 12, 256, 64, 64, sinks=1) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = []
+    for _ in range(5):
+        for st, q in zip(streams, qs):
+            with torch.cuda.stream(st):
+                got.append(ops.attention_window(q, cu, 12, 256, 64, 64, sinks=1))
+    torch.cuda.synchronize()
+    ops.sync()
+    assert all(torch.equal(g, want[k % 2]) for k, g in enumerate(got))

@@ -23,14 +23,14 @@ def rms(**kw):
                    a["rows"], a["cols"], a["eps"], None)
 
 
-@pytest.mark.parametrize("kw", [dict(rows=-1), dict(cols=0), dict(cols=-3), dict(dtype=L.DT_S8), dict(dtype=9), dict(y=None),
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(rows=2 ** 31 - 1), dict(cols=0), dict(cols=-3), dict(dtype=L.DT_S8), dict(dtype=9), dict(y=None),
                                 dict(q=P, scale=P), dict(y=None, q=P), dict(y=None, scale=P), dict(scale=P),
                                 dict(sum=P), dict(eps=-1.0), dict(eps=math.nan), dict(x=None), dict(gamma=None)])
 def test_rmsnorm_refuses(kw):
     assert "rmsnorm" in rms(**kw)
 
 
-@pytest.mark.parametrize("kw", [dict(rows=-1), dict(cols=0), dict(dtype=L.DT_S32), dict(q=None), dict(scale=None),
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(rows=2 ** 31 - 1), dict(cols=0), dict(dtype=L.DT_S32), dict(q=None), dict(scale=None),
                                 dict(y=None)])
 def test_dequantize_rows_refuses(kw):
     a = dict(q=P, scale=P, y=P, dtype=L.DT_F32, rows=2, cols=8) | kw
@@ -38,7 +38,7 @@ def test_dequantize_rows_refuses(kw):
 
 
 @pytest.mark.parametrize("fn", ["jb_op_quantize_mxfp4", "jb_op_dequantize_mxfp4"])
-@pytest.mark.parametrize("kw", [dict(rows=-1), dict(cols=0), dict(cols=48), dict(cols=-32), dict(dtype=L.DT_S8), dict(x=None),
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(rows=2 ** 31 - 1), dict(cols=2 ** 31 - 32), dict(cols=0), dict(cols=48), dict(cols=-32), dict(dtype=L.DT_S8), dict(x=None),
                                 dict(q=None), dict(scale=None), dict(x=P + 8), dict(q=P + 4), dict(scale=P + 2)])
 def test_mxfp4_rows_refuse(fn, kw):
     a = dict(x=P, dtype=L.DT_BF16, q=P, scale=P, rows=4, cols=64) | kw
@@ -46,7 +46,7 @@ def test_mxfp4_rows_refuse(fn, kw):
     assert fn in refused(getattr(L.lib(), fn), *args, a["rows"], a["cols"], None)
 
 
-@pytest.mark.parametrize("kw", [dict(M=-1), dict(N=0), dict(N=12), dict(K=0), dict(K=48), dict(c_dtype=L.DT_S32),
+@pytest.mark.parametrize("kw", [dict(M=-1), dict(M=2 ** 31 - 1), dict(N=2 ** 31 - 8), dict(K=2 ** 31 - 32), dict(N=0), dict(N=12), dict(K=0), dict(K=48), dict(c_dtype=L.DT_S32),
                                 dict(epi=-1), dict(epi=4), dict(epi=L.EPI_RESIDUAL), dict(res=P), dict(aq=None),
                                 dict(ws=None), dict(c=None), dict(aq=P + 8), dict(c=P + 2), dict(asc=P + 1),
                                 dict(epi=L.EPI_RESIDUAL, res=P + 4)])
@@ -62,7 +62,7 @@ def test_mxfp4_scale_bytes():
     assert f(2 ** 31 - 1, 4096) == 2 ** 24 * 32 * 512
 
 
-@pytest.mark.parametrize("kw", [dict(batch=-1), dict(heads=0), dict(kv=0), dict(kv=3), dict(d=24), dict(d=256), dict(d=0),
+@pytest.mark.parametrize("kw", [dict(batch=-1), dict(batch=2 ** 31 - 1), dict(rows=2 ** 31 - 1), dict(heads=0), dict(kv=0), dict(kv=3), dict(d=24), dict(d=256), dict(d=0),
                                 dict(max_len=-1), dict(rows=-1), dict(left=-1), dict(right=-5), dict(sinks=-1),
                                 dict(dtype=L.DT_S8), dict(qkv=None), dict(cu=None), dict(ctx=None), dict(qkv=P + 2),
                                 dict(ctx=P + 8), dict(heads=2 ** 22, kv=2 ** 21)])
