@@ -38,27 +38,31 @@ struct WinParams {
 };
 
 // ── any head width, f32 arithmetic ──────────────────────────────────────────
-// A CTA per (row, head, kSimtQ queries): LANES lanes share a query's
-// dimensions (interleaved by four, so that a warp's reads of a key fall on
-// different banks), each thread works on two queries, so that a key read from
-// shared memory serves both.  FMA-bound: 4 d per (query, key).
+// A CTA per (row, head, QUERIES queries): LANES lanes share a query's
+// dimensions, 16 each (interleaved by four, so that a warp's reads of a key
+// fall on different banks); each thread works on two neighbouring queries, so
+// that a key read from shared memory serves both, and a warp skips the key
+// tiles that none of its consecutive queries sees.  FMA-bound: 4 d per
+// (query, key), two dimensions to an instruction (packed f32x2); f32 tiles are
+// copied asynchronously, one ahead.
 constexpr int kSimtThreads = 128;
-constexpr int kSimtKeys = 32;
 
-template <int D>
+template <typename T, int D>
 struct SimtCfg {
-  static constexpr int LANES = D >= 64 ? D / 32 : D == 32 ? 2 : 1;
+  static constexpr int LANES = D > 16 ? D / 16 : 1;
   static constexpr int DL = D / LANES;          // dimensions per lane
-  static constexpr int GROUPS = kSimtThreads / LANES;
-  static constexpr int QUERIES = 2 * GROUPS;    // queries per CTA
+  static constexpr int QUERIES = 2 * kSimtThreads / LANES;
+  static constexpr int KEYS = D >= 32 ? 2048 / D : 64;  // of a tile
+  static constexpr bool kAsync = sizeof(T) == 4;
+  static constexpr int STAGES = kAsync ? 2 : 1;
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kSimtThreads) window_simt_kernel(WinParams p) {
-  using C = SimtCfg<D>;
+__global__ void __launch_bounds__(kSimtThreads, 4) window_simt_kernel(WinParams p) {
+  using C = SimtCfg<T, D>;
   constexpr int V4 = C::DL / 4;
-  __shared__ __align__(16) float Ks[kSimtKeys][D];
-  __shared__ __align__(16) float Vs[kSimtKeys][D];
+  __shared__ __align__(16) float Ks[C::STAGES][C::KEYS][D];
+  __shared__ __align__(16) float Vs[C::STAGES][C::KEYS][D];
   const int qb = blockIdx.x % p.q_blocks;
   const int h = blockIdx.x / p.q_blocks % p.heads, b = blockIdx.x / p.q_blocks / p.heads;
   const int start = p.cu[b], n = min(p.cu[b + 1], p.rows) - start;  // never past the buffers
@@ -70,107 +74,139 @@ __global__ void __launch_bounds__(kSimtThreads) window_simt_kernel(WinParams p) 
   const T* gk = row + (p.heads + hk) * D;
   const T* gv = gk + p.kv_heads * D;
   const int part = threadIdx.x % C::LANES, group = threadIdx.x / C::LANES;
-  // queries group and group + GROUPS: a short row fills the first half
   int qi[2], lo[2], hi[2];
-  float qv[2][C::DL], o[2][C::DL], m[2], l[2];
+  float2 qv[2][C::DL / 2], o[2][C::DL / 2];
+  float m[2], l[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    qi[u] = q0 + group + u * C::GROUPS;
+    qi[u] = q0 + 2 * group + u;
     lo[u] = qi[u] - min(p.left, qi[u]);
     hi[u] = qi[u] < n ? qi[u] + min(p.right, n - 1 - qi[u]) : -1;  // last visible key
     m[u] = -INFINITY;
     l[u] = 0.f;
 #pragma unroll
-    for (int i = 0; i < V4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = 4 * (i * C::LANES + part) + e;
-        qv[u][4 * i + e] = qi[u] < n ? to_f(row[static_cast<size_t>(qi[u]) * ld + h * D + d]) * p.scale_log2 : 0.f;
-        o[u][4 * i + e] = 0.f;
+    for (int i = 0; i < C::DL / 2; ++i) {
+      const int d = 4 * (i / 2 * C::LANES + part) + 2 * (i & 1);
+      qv[u][i] = o[u][i] = make_float2(0.f, 0.f);
+      if (qi[u] < n) {
+        const T* q = row + static_cast<size_t>(qi[u]) * ld + h * D + d;
+        qv[u][i] = make_float2(to_f(q[0]) * p.scale_log2, to_f(q[1]) * p.scale_log2);
       }
+    }
   }
   const int q_last = min(n, q0 + C::QUERIES) - 1;
   const int k_end = q_last + min(p.right, n - 1 - q_last) + 1;
-  int k_begin = q0 - min(p.left, q0);
+  const int k_begin = q0 - min(p.left, q0);
   const int s_end = min(p.sinks, k_begin);  // sinks behind the block's window
-  // [0, s_end), then [k_begin, k_end)
-  for (int k0 = s_end > 0 ? 0 : k_begin; k0 < k_end;) {
-    const int stop = k0 < s_end ? s_end : k_end;
-    const int kn = min(kSimtKeys, stop - k0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kn * D; i += kSimtThreads) {
-      const size_t at = static_cast<size_t>(k0 + i / D) * ld + i % D;
-      Ks[i / D][i % D] = to_f(gk[at]);
-      Vs[i / D][i % D] = to_f(gv[at]);
+  int see_lo = lo[0], see_hi = max(hi[0], hi[1]);  // of the warp
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) {
+    see_lo = min(see_lo, __shfl_xor_sync(0xffffffffu, see_lo, w));
+    see_hi = max(see_hi, __shfl_xor_sync(0xffffffffu, see_hi, w));
+  }
+  // tiles of [0, s_end), then of [k_begin, k_end)
+  auto stop_of = [&](int k0) { return min(k0 + C::KEYS, k0 < s_end ? s_end : k_end); };
+  auto after = [&](int k1) { return k1 == s_end ? k_begin : k1; };
+  auto load = [&](int k0, int st) {
+    const int kn = stop_of(k0) - k0;
+    if constexpr (C::kAsync) {
+      for (int i = threadIdx.x; i < kn * (D / 4); i += kSimtThreads) {
+        const size_t at = static_cast<size_t>(k0 + i / (D / 4)) * ld + i % (D / 4) * 4;
+        const uint32_t k = smem_u32(&Ks[st][0][0] + 4 * i), v = smem_u32(&Vs[st][0][0] + 4 * i);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(k), "l"(gk + at) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(v), "l"(gv + at) : "memory");
+      }
+    } else {
+      for (int i = threadIdx.x; i < kn * D; i += kSimtThreads) {
+        const size_t at = static_cast<size_t>(k0 + i / D) * ld + i % D;
+        (&Ks[st][0][0])[i] = to_f(gk[at]);
+        (&Vs[st][0][0])[i] = to_f(gv[at]);
+      }
+    }
+  };
+  int k0 = s_end > 0 ? 0 : k_begin, st = 0;
+  if constexpr (C::kAsync) {
+    load(k0, 0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  while (k0 < k_end) {
+    const int k1 = stop_of(k0), next = after(k1), kn = k1 - k0;
+    if constexpr (C::kAsync) {
+      if (next < k_end) load(next, st ^ 1);  // last read in the turn before, behind its barrier
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      load(k0, 0);
     }
     __syncthreads();
-    for (int j0 = 0; j0 < kn; j0 += 4) {
-      float s[2][4];
-      bool seen[2][4];  // a hidden value adds nothing, not even 0 * NaN
+    if (k0 <= see_hi && (k1 > see_lo || k0 < p.sinks)) {
+#pragma unroll 1
+      for (int j0 = 0; j0 < kn; j0 += 4) {
+        float s[2][4];
+        bool seen[2][4];  // a hidden value adds nothing, not even 0 * NaN
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[0][j] = s[1][j] = 0.f;
-        if (j0 + j < kn) {
+        for (int j = 0; j < 4; ++j) {
+          float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          if (j0 + j < kn) {
 #pragma unroll
-          for (int i = 0; i < V4; ++i) {
-            const float4 k4 = *reinterpret_cast<const float4*>(&Ks[j0 + j][4 * (i * C::LANES + part)]);
+            for (int i = 0; i < V4; ++i) {
+              const float4 k4 = *reinterpret_cast<const float4*>(&Ks[st][j0 + j][4 * (i * C::LANES + part)]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              s[u][j] = fmaf(qv[u][4 * i], k4.x, s[u][j]);
-              s[u][j] = fmaf(qv[u][4 * i + 1], k4.y, s[u][j]);
-              s[u][j] = fmaf(qv[u][4 * i + 2], k4.z, s[u][j]);
-              s[u][j] = fmaf(qv[u][4 * i + 3], k4.w, s[u][j]);
+              for (int u = 0; u < 2; ++u) {
+                s2[u] = __ffma2_rn(qv[u][2 * i], make_float2(k4.x, k4.y), s2[u]);
+                s2[u] = __ffma2_rn(qv[u][2 * i + 1], make_float2(k4.z, k4.w), s2[u]);
+              }
             }
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            s[u][j] = s2[u].x + s2[u].y;
+#pragma unroll
+            for (int w = 1; w < C::LANES; w <<= 1) s[u][j] += __shfl_xor_sync(0xffffffffu, s[u][j], w);
           }
         }
 #pragma unroll
-        for (int w = 1; w < C::LANES; w <<= 1) {
-          s[0][j] += __shfl_xor_sync(0xffffffffu, s[0][j], w);
-          s[1][j] += __shfl_xor_sync(0xffffffffu, s[1][j], w);
-        }
-      }
+        for (int u = 0; u < 2; ++u) {
+          float mx = m[u];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float mx = m[u];
+          for (int j = 0; j < 4; ++j) {
+            const int key = k0 + j0 + j;
+            seen[u][j] = j0 + j < kn && key <= hi[u] && (key >= lo[u] || key < p.sinks);
+            if (!seen[u][j]) s[u][j] = -INFINITY;
+            mx = fmaxf(mx, s[u][j]);
+          }
+          const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: p stays 0
+          const float corr = exp2f(m[u] - ref);
+          m[u] = mx;
+          l[u] *= corr;
+#pragma unroll
+          for (int e = 0; e < C::DL / 2; ++e) o[u][e] = __fmul2_rn(o[u][e], f2(corr));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[u][j] = exp2f(s[u][j] - ref);
+            l[u] += s[u][j];
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int key = k0 + j0 + j;
-          seen[u][j] = j0 + j < kn && key <= hi[u] && (key >= lo[u] || key < p.sinks);
-          if (!seen[u][j]) s[u][j] = -INFINITY;
-          mx = fmaxf(mx, s[u][j]);
-        }
-        const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: p stays 0
-        const float corr = exp2f(m[u] - ref);
-        m[u] = mx;
-        l[u] *= corr;
+          if (j0 + j < kn) {
 #pragma unroll
-        for (int e = 0; e < C::DL; ++e) o[u][e] *= corr;
+            for (int i = 0; i < V4; ++i) {
+              const float4 v4 = *reinterpret_cast<const float4*>(&Vs[st][j0 + j][4 * (i * C::LANES + part)]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[u][j] = exp2f(s[u][j] - ref);
-          l[u] += s[u][j];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j0 + j < kn) {
-#pragma unroll
-          for (int i = 0; i < V4; ++i) {
-            const float4 v4 = *reinterpret_cast<const float4*>(&Vs[j0 + j][4 * (i * C::LANES + part)]);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              if (!seen[u][j]) continue;
-              o[u][4 * i] = fmaf(s[u][j], v4.x, o[u][4 * i]);
-              o[u][4 * i + 1] = fmaf(s[u][j], v4.y, o[u][4 * i + 1]);
-              o[u][4 * i + 2] = fmaf(s[u][j], v4.z, o[u][4 * i + 2]);
-              o[u][4 * i + 3] = fmaf(s[u][j], v4.w, o[u][4 * i + 3]);
+              for (int u = 0; u < 2; ++u) {
+                if (!seen[u][j]) continue;
+                o[u][2 * i] = __ffma2_rn(f2(s[u][j]), make_float2(v4.x, v4.y), o[u][2 * i]);
+                o[u][2 * i + 1] = __ffma2_rn(f2(s[u][j]), make_float2(v4.z, v4.w), o[u][2 * i + 1]);
+              }
             }
           }
         }
       }
     }
-    k0 += kn;
-    if (k0 == s_end) k0 = k_begin;
+    __syncthreads();  // the tile may be overwritten
+    k0 = next;
+    if constexpr (C::kAsync) st ^= 1;
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -178,16 +214,18 @@ __global__ void __launch_bounds__(kSimtThreads) window_simt_kernel(WinParams p) 
       const float inv = 1.f / l[u];
       T* out = static_cast<T*>(p.ctx) + (static_cast<size_t>(start + qi[u]) * p.heads + h) * D;
 #pragma unroll
-      for (int i = 0; i < V4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[4 * (i * C::LANES + part) + e] = from_f<T>(o[u][4 * i + e] * inv);
+      for (int i = 0; i < C::DL / 2; ++i) {
+        const int d = 4 * (i / 2 * C::LANES + part) + 2 * (i & 1);
+        out[d] = from_f<T>(o[u][i].x * inv);
+        out[d + 1] = from_f<T>(o[u][i].y * inv);
+      }
     }
   }
 }
 
 template <typename T, int D>
 cudaError_t launch_simt_d(WinParams p, int batch, int max_len, cudaStream_t s, std::string* why) {
-  p.q_blocks = (max_len + SimtCfg<D>::QUERIES - 1) / SimtCfg<D>::QUERIES;
+  p.q_blocks = (max_len + SimtCfg<T, D>::QUERIES - 1) / SimtCfg<T, D>::QUERIES;
   const long long grid = static_cast<long long>(p.q_blocks) * p.heads * batch;
   if (grid > INT32_MAX) {
     if (why) *why = "attention_window: too many (row, head, query block) triples";
