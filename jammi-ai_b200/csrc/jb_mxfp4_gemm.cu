@@ -8,17 +8,18 @@
 // elements, scale_vec::2X): the tensor core multiplies the scales in, exact
 // products accumulated in f32 in TMEM, four times the bf16 rate.
 //
-// One persistent CTA per SM, output tiles of 128 x BN, K in stages of 256
-// elements (one 128-byte swizzled row of codes):
-//   warp 0     TMA producer: codes of A and W by tiled copies, their scale
-//              tiles (contiguous by construction) by plain bulk copies
-//   warp 1     TMEM allocator and single-thread MMA issuer: per stage the
-//              scale tiles go from shared memory to TMEM (tcgen05.cp
-//              32x128b.warpx4: 128 rows x 4 blocks into 4 columns), then four
-//              K = 64 products.  Each stage has its own TMEM columns for the
-//              scales, so a copy never meets a product that still reads them:
-//              the stage's shared memory, and with it its TMEM columns, comes
-//              back only after the commit of its products.
+// Persistent CTAs, one per SM, output tiles of 128 x 64 or 128 x 128, or of
+// 256 x 192 by pairs of CTAs; K in stages of 256 elements (one 128-byte
+// swizzled row of codes):
+//   warp 0     TMA producer: codes of A and W, and their scale tiles as rows of
+//              128 bytes, by tiled copies (what lies past the end arrives as 0)
+//   warp 1     TMEM allocator and MMA issuer: per stage the scale tiles go from
+//              shared memory to TMEM (tcgen05.cp 32x128b.warpx4: 128 rows x 4
+//              blocks into 4 columns), then four K = 64 products.  Each stage
+//              has its own TMEM columns for the scales, so a copy never meets a
+//              product that still reads them: the stage's shared memory, and
+//              with it its TMEM columns, comes back only after the commit of
+//              its products.
 //   warps 2..  epilogue, one warp per 32 rows x 64 columns of the tile: the
 //              accumulators go to registers at once (tcgen05.ld) and are
 //              released before any arithmetic; bias, activation and residual
@@ -26,10 +27,21 @@
 //              accumulators) in f32, one rounding, one TMA store of the box.
 // The accumulator is double-buffered (2 x BN columns).
 //
-// BN = 192: the widest tile whose two accumulators leave TMEM columns for the
-// scales (384 + 4 stages x 24).  Its odd tiles start 64 rows into a scale
+// What bounds it.  A K = 64 product reads 32 bytes of each of its rows from
+// shared memory, at 128 bytes a clock: 128 x 192 by one SM would take 80
+// clocks of reading (and more than that to fill) beside 96 of arithmetic, and
+// did not get past 217 us at 8192^3.  A pair (cta_group::2) gives each SM half
+// of W: 188 us, 5.8 PFLOP/s, 89% of four times the measured bf16 rate.
+// BN = 192 is the widest tile whose two accumulators leave TMEM columns for
+// the scales (384 + 5 stages x 24).  Its odd tiles start 64 rows into a scale
 // tile of W: the scale address of the product starts two columns (2 x 32
 // rows) later.
+//
+// Measured (bf16 in and out unless said, without the quantisation of A):
+//   20479 x 4096 x 1024, GELU         58.9 us  2.9 PFLOP/s  epilogue: 84 M GELUs
+//   20479 x 1024 x 4096, residual     45.7 us  3.8 PFLOP/s  7 waves of tiles, the last one part full
+//   1777 x 1536 x 384, f16             5.0 us               launch, one tile's latency
+//   12 x 2304 x 768                    3.6 us               launch, one tile's latency
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -649,7 +661,8 @@ cudaError_t launch_linear_mxfp4(const MxGemmArgs& g, cudaStream_t s, std::string
   const long long m_tiles = (g.M + kBM - 1ll) / kBM;
   // tile numbers, and scale rows (four to a scale tile) as TMA coordinates
   const long long k_tiles = (g.K + 127) / 128;
-  if (m_tiles * ((g.N + 63) / 64) > INT32_MAX / 2 || (std::max<long long>(m_tiles, (g.N + 127ll) / 128) + 2) * k_tiles * 4 > INT32_MAX) {
+  if (m_tiles * ((g.N + 63) / 64) > INT32_MAX / 2 ||
+      (std::max<long long>(m_tiles, (g.N + 127ll) / 128) + 2) * k_tiles * 4 > INT32_MAX) {
     if (why) *why = "linear(mxfp4): more tiles than 32 bits number";
     return cudaErrorInvalidValue;
   }
@@ -657,8 +670,21 @@ cudaError_t launch_linear_mxfp4(const MxGemmArgs& g, cudaStream_t s, std::string
   int dev = 0;
   cudaGetDevice(&dev);
   const long long sms = num_sms(dev);
-  if (m_tiles * ((g.N + 127) / 128) <= sms) return launch_out<64, 1>(g, p, s, why);
-  if (g.c_dtype == JB_DT_F32 || m_tiles * ((g.N + 191) / 192) <= sms) return launch_out<128, 1>(g, p, s, why);
+  // Width of the tile.  One wave of 128 x 64 tiles, when it holds them all, is
+  // the shortest way through (12 x 2304 x 768: 3.6 us, 3.9 with 128 columns; 777 x
+  // 1024 x 4096: 6.9, 7.8); two waves of it are not (1777 x 1024 x 4096: 10.7, 8.0).
+  if (m_tiles * ((g.N + 63) / 64) <= sms) return launch_out<64, 1>(g, p, s, why);
+  // Pairs do more per wave, and cost more per wave and to start.  In units of
+  // the time of a K column in a 128 x 128 tile, waves measured at K = 384 to
+  // 4096 take max(K, 640) + 576 and, by pairs, max(K, 640) + 1024 with 600 once.
+  // 128 columns against pairs: 5000 x 768 x 768 5.5 us, 6.7; 3000 x 2304 x 768
+  // 6.6, 7.1; 9000 x 2304 x 768 13.8, 13.0; 3000 x 1024 x 4096 12.1, 9.2; 20479 x
+  // 4096 x 1024 53.7, 47.1.
+  const long long k = std::max<long long>(g.K, 640);
+  auto waves = [](long long tiles, long long slots) { return (tiles + slots - 1) / slots; };
+  const long long one = waves(m_tiles * ((g.N + 127) / 128), sms) * (k + 576);
+  const long long two = waves((m_tiles + 1) / 2 * ((g.N + 191) / 192), sms / 2) * (k + 1024) + 600;
+  if (g.c_dtype == JB_DT_F32 || one <= two) return launch_out<128, 1>(g, p, s, why);
   return launch_out<192, 2>(g, p, s, why);
 }
 
