@@ -37,6 +37,11 @@ struct WinParams {
   float scale_log2;
 };
 
+// Tokens of row b that lie inside the buffers, whatever the offsets hold.
+__device__ __forceinline__ int row_tokens(const WinParams& p, int b, int start) {
+  return start < 0 ? 0 : max(0, min(p.cu[b + 1], p.rows)) - start;
+}
+
 // ── any head width, f32 arithmetic ──────────────────────────────────────────
 // A CTA per (row, head, QUERIES queries): LANES lanes share a query's
 // dimensions, 16 each (interleaved by four, so that a warp's reads of a key
@@ -65,9 +70,9 @@ __global__ void __launch_bounds__(kSimtThreads, 4) window_simt_kernel(WinParams 
   __shared__ __align__(16) float Vs[C::STAGES][C::KEYS][D];
   const int qb = blockIdx.x % p.q_blocks;
   const int h = blockIdx.x / p.q_blocks % p.heads, b = blockIdx.x / p.q_blocks / p.heads;
-  const int start = p.cu[b], n = min(p.cu[b + 1], p.rows) - start;  // never past the buffers
+  const int start = p.cu[b], n = row_tokens(p, b, start);
   const int q0 = qb * C::QUERIES;
-  if (start < 0 || q0 >= n) return;
+  if (q0 >= n) return;
   const int hk = h / (p.heads / p.kv_heads);
   const int ld = (p.heads + 2 * p.kv_heads) * D;
   const T* row = static_cast<const T*>(p.qkv) + static_cast<size_t>(start) * ld;
@@ -275,7 +280,8 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 // A masked value contributes 0 * v, which is not 0 when v is not finite.  V
 // rows behind the item's last key are zeroed in shared memory; for the rest
 // outputs that are not finite are computed again, by their thread, over the
-// visible keys only (window_row_exact).
+// visible keys only (window_row_exact; a row of an item of several blocks only
+// if a hidden value is the cause, so that no visible one makes a long row slow).
 //
 // Items are numbered over the query blocks that exist (a prefix sum of the
 // rows' blocks in shared memory, for batches of up to kPrefixRows) and dealt
@@ -356,8 +362,8 @@ __host__ __device__ constexpr uint32_t p_col(int k) {
   return static_cast<uint32_t>((piece < 6 ? 32 * piece : 32 * (piece - 6) + 16) + 8 * (k & 1));
 }
 
-// Output columns [c0, c1) of one query row over its visible keys
-// only, in f32 from global memory: rows whose tensor-core output is not finite.
+// Output columns [c0, c1) of one query row over its visible keys only, in f32
+// from global memory.
 template <typename T, int D>
 __device__ __noinline__ void window_row_exact(const WinParams& p, int start, int n, int h, int qi, int c0, int c1) {
   const int ld = (p.heads + 2 * p.kv_heads) * D;
@@ -368,23 +374,46 @@ __device__ __noinline__ void window_row_exact(const WinParams& p, int start, int
   T* out = static_cast<T*>(p.ctx) + (static_cast<size_t>(start + qi) * p.heads + h) * D;
   const int lo = qi - min(p.left, qi), hi = qi + min(p.right, n - 1 - qi);
   const int behind = min(p.sinks, lo);  // sinks in front of the window
-  auto score = [&](int j) {
-    float s = 0.f;
-    for (int d = 0; d < D; ++d) s = fmaf(to_f(q[d]), to_f(k[static_cast<size_t>(j) * ld + d]), s);
-    return s * p.scale_log2;
-  };
-  float m = -INFINITY;
-  for (int j = behind > 0 ? 0 : lo; j <= hi; j = j + 1 == behind ? lo : j + 1) m = fmaxf(m, score(j));
-  if (m == -INFINITY) m = 0.f;
-  for (int c = c0; c < c1; c += 16) {  // 16 output columns a pass
-    float o[16] = {}, l = 0.f;
-    for (int j = behind > 0 ? 0 : lo; j <= hi; j = j + 1 == behind ? lo : j + 1) {
-      const float e = exp2f(score(j) - m);
-      l += e;
-      for (int d = 0; d < 16; ++d) o[d] = fmaf(e, to_f(v[static_cast<size_t>(j) * ld + c + d]), o[d]);
+  for (int c = c0; c < c1; c += 16) {   // 16 output columns a pass
+    float o[16] = {}, l = 0.f, m = -INFINITY;
+    bool lost = false;  // every output is NaN and stays so
+    for (int j = behind > 0 ? 0 : lo; j <= hi && !lost; j = j + 1 == behind ? lo : j + 1) {
+      float s = 0.f;
+      for (int d = 0; d < D; ++d) s = fmaf(to_f(q[d]), to_f(k[static_cast<size_t>(j) * ld + d]), s);
+      s *= p.scale_log2;
+      if (s == -INFINITY) continue;  // weighs nothing, not even 0 * NaN
+      const float top = fmaxf(m, s), corr = exp2f(m - top), e = exp2f(s - top);
+      m = top;
+      l = l * corr + e;
+      lost = true;
+      for (int d = 0; d < 16; ++d) {
+        // (o is 0 until the first key: the scale from -infinity is 0)
+        o[d] = fmaf(e, to_f(v[static_cast<size_t>(j) * ld + c + d]), o[d] * corr);
+        lost &= o[d] != o[d];
+      }
     }
     for (int d = 0; d < 16; ++d) out[c + d] = from_f<T>(o[d] / l);
   }
+}
+
+// Whether an item of several blocks held a value that is not finite and that
+// the row does not see, in columns [c0, c1): the keys of the item's range on
+// both sides of the row's window, and those that pad the sinks.
+template <typename T, int D>
+__device__ __noinline__ bool hidden_not_finite(const WinParams& p, int start, int n, int h, int qi, int k_begin, int nw,
+                                               int s_end, int c0, int c1) {
+  const int ld = (p.heads + 2 * p.kv_heads) * D;
+  const T* v = static_cast<const T*>(p.qkv) + static_cast<size_t>(start) * ld +
+               (p.heads + p.kv_heads + h / (p.heads / p.kv_heads)) * D;
+  auto any = [&](int j, int stop) {
+    float zero = 0.f;
+    for (; j < stop; ++j)
+      for (int c = c0; c < c1; ++c) zero = fmaf(to_f(v[static_cast<size_t>(j) * ld + c]), 0.f, zero);
+    return zero != 0.f;
+  };
+  const int lo = qi - min(p.left, qi), hi = qi + min(p.right, n - 1 - qi);
+  return any(max(k_begin, min(p.sinks, lo)), lo) || any(hi + 1, k_begin + nw) ||
+         any(s_end, min(ceil16(s_end), p.rows - start));
 }
 
 // Descriptor of a K-major (or, for V, MN-major) tile of 64- or 128-byte
@@ -436,8 +465,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       int blocks = 0;
       if (b0 + lane < p.batch) {
-        const int start = w.cu[b0 + lane], n = min(w.cu[b0 + lane + 1], w.rows) - start;  // never past the buffers
-        if (start >= 0 && n > 0) blocks = (min(n, w.q_blocks * p.kq) + p.kq - 1) / p.kq;
+        const int n = row_tokens(w, b0 + lane, w.cu[b0 + lane]);
+        if (n > 0) blocks = (min(n, w.q_blocks * p.kq) + p.kq - 1) / p.kq;
       }
       int incl = blocks;
 #pragma unroll
@@ -502,9 +531,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         q0 = qb * p.kq;
         start = w.cu[b];
-        n = min(w.cu[b + 1], w.rows) - start;  // never past the buffers
+        // (rows that overlap could have more blocks than 32 bits count)
+        n = qb >= 0 && qb < w.q_blocks ? row_tokens(w, b, start) : 0;
       }
-      unsigned todo = __ballot_sync(0xffffffffu, f < items && start >= 0 && q0 < n);
+      unsigned todo = __ballot_sync(0xffffffffu, f < items && q0 < n);
       while (todo && ok) {
         const int src = __ffs(todo) - 1;
         todo &= todo - 1;
@@ -701,7 +731,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // sees: bf16 P has f32's range, so any reference within 2^100 of the
           // maximum gives the same relative rounding, and no maximum is needed.
           // Both warps of a row read it.
-          // (p beyond f32 makes the outputs not finite: window_row_exact.)
+          // (p beyond f32 makes the sum or the outputs infinite: window_row_exact.)
           const int d0 = q0 + 32 * quarter - k_begin;  // lane 0's own column
           const int col = min(d0, 256 - 32);           // inside the slot's columns
           uint32_t s[32];
@@ -742,10 +772,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mx = fmaxf(mx, xm[32 * (half ^ 1)]);
           const float mb = mx * w.scale_log2;
           if (j == 0) {
-            mref = mb == -INFINITY ? 0.f : mb;  // nothing visible yet: p stays 0
+            mref = mb;
           } else {
             // both threads of a row decide alike; each rescales its half of O
-            const bool up = mb > mref + kRescale;
+            const bool up = mb > mref + kRescale;  // always behind scores of -infinity only
             if (__any_sync(0xffffffffu, up)) {
               const float alpha = up ? ex2_approx(mref - mb) : 1.f;
               l *= alpha;
@@ -765,6 +795,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (active) {
           float2 l2 = make_float2(0.f, 0.f);
+          const float ref = mref == -INFINITY ? 0.f : mref;  // nothing seen so far: p stays 0
 #pragma unroll 1
           for (int c = 32 * half; c < v1 - v0; c += 64) {
             const uint32_t bits = visible(v0 + c);
@@ -779,7 +810,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
                 float2 z = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
-                                      f2(w.scale_log2), f2(-mref));
+                                      f2(w.scale_log2), f2(-ref));
                 // (a second, unmasked copy of this code is slower: it does not fit
                 // the instruction cache beside the rest)
                 if (!(bits >> i & 1)) z.x = -INFINITY;
@@ -879,9 +910,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       __syncwarp();
-      // a sum that is NaN has a NaN score in it: the outputs are NaN.  Else a
-      // value that the row does not see may be the one that is not finite.
-      if (mine && !(zero2.x + zero2.y == 0.f) && l_row == l_row) window_row_exact<T, D>(w, start, n, h, qi, half * (D / 2), (half + 1) * (D / 2));
+      // An infinite sum (the row's own score lies far below another one) hides in
+      // outputs of 0.  A sum that is NaN has a NaN score in it: the outputs are NaN.
+      // Else a value that the row does not see may be the one that is not finite;
+      // long ranges are computed again only if there is one.
+      // A reference of -infinity (the row's own score is) says nothing about the others.
+      const bool unsafe = !(zero2.x + zero2.y == 0.f && l_row < INFINITY) || (nb == 1 && mref == -INFINITY);
+      if (mine && unsafe && l_row == l_row) {
+        const int c0 = half * (D / 2), c1 = c0 + D / 2;
+        if (nb == 1 || hidden_not_finite<T, D>(w, start, n, h, qi, k_begin, nw, s_end, c0, c1))
+          window_row_exact<T, D>(w, start, n, h, qi, c0, c1);
+      }
     }
   }
   tc_fence_before();

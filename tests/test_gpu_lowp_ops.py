@@ -271,7 +271,7 @@ def gelu64(z):
 
 
 LIN_SHAPES = [(1, 8, 32), (12, 2304, 768), (3, 72, 64), (127, 200, 96), (129, 264, 160), (64, 1024, 4096), (300, 1536, 384),
-              (2000, 1160, 288), (5000, 768, 768), (4100, 1000, 1056)]
+              (2000, 1160, 288), (5000, 768, 768), (4100, 1000, 1056), (2850, 1000, 1056)]
 
 
 @pytest.mark.parametrize("out", DTYPES)
@@ -337,6 +337,26 @@ def test_linear_mxfp4(dev, M, N, K, epi, out):
     linear_check(c, mx_ref(a)[0], mx_ref(w)[0], bias, res, epi, K)
 
 
+@pytest.mark.parametrize("epi", ["gelu", "quick_gelu"])
+def test_linear_mxfp4_activations_over_their_range(dev, epi):
+    """Weights of zero: the bias is what the activation gets.  Its error is the 1e-6 max(1, |z|) that
+    the framework's other linears keep to."""
+    from jammi_b200 import _lib as L
+    z = torch.cat([torch.linspace(-20, 20, 8192), torch.tensor([0.0, -0.0, 1e30, -1e30, 3e38, -3e38, 1e-30, -1e-30]),
+                   torch.tensor([math.inf, -math.inf, math.nan, 40.0, -40.0, 90.0, -90.0, 1e4])]).to(dev)
+    aq = _ops().quantize_mxfp4(torch.ones((2, 32), device=dev))
+    wq = _ops().quantize_mxfp4(torch.zeros((z.numel(), 32), device=dev))
+    c = _ops().linear_mxfp4(*aq, *wq, bias=z, epilogue=L.EPI_GELU if epi == "gelu" else L.EPI_QUICK_GELU,
+                            out_dtype=torch.float32)
+    _ops().sync()
+    assert torch.equal(torch.nan_to_num(c[0], nan=-7.0), torch.nan_to_num(c[1], nan=-7.0))
+    z, y = z.double(), c[0].double()
+    assert y[z.isnan()].isnan().all() and (y[z == math.inf] == math.inf).all()
+    fin = z.isfinite()
+    want = (gelu64(z) if epi == "gelu" else z * torch.sigmoid(1.702 * z))[fin]
+    assert ((y[fin] - want).abs() <= 1e-6 * z[fin].abs().clamp(min=1)).all()
+
+
 def test_linear_mxfp4_residual_in_place_and_nan_rows(dev):
     from jammi_b200 import _lib as L
     ops, g = _ops(), _gen(8)
@@ -390,8 +410,9 @@ def test_mxfp4_refusals(dev):
 
 # ── windowed attention ──────────────────────────────────────────────────────
 
-def window_ref(qkv, lens, h, hk, left, right, sinks):
-    """Float64, row by row; also sum_j p_j |v_j| / sum_j p_j and max |q k| / sqrt(d) for the error bound."""
+def window_ref(qkv, lens, h, hk, left, right, sinks, hide=None):
+    """Float64, row by row; also sum_j p_j |v_j| / sum_j p_j and max |q k| / sqrt(d) for the error bound.
+    ``hide`` [tokens]: keys with p = 0."""
     d = qkv.shape[1] // (h + 2 * hk)
     x = qkv.double()
     out, mag = torch.zeros((qkv.shape[0], h * d), dtype=torch.float64, device=qkv.device), None
@@ -404,6 +425,8 @@ def window_ref(qkv, lens, h, hk, left, right, sinks):
             v = v.reshape(n, hk, d).transpose(0, 1).repeat_interleave(h // hk, 0)
             i, j = torch.arange(n, device=x.device)[:, None], torch.arange(n, device=x.device)[None]
             seen = (j <= i + right) & ((j >= i - left) | (j < sinks))
+            if hide is not None:
+                seen = seen & ~hide[at:at + n]
             s = (q @ k.transpose(1, 2) / math.sqrt(d)).masked_fill(~seen, -math.inf)
             top = max(top, (q.abs() @ k.abs().transpose(1, 2)).max().item() / math.sqrt(d))
             p = torch.softmax(s, -1)
@@ -413,13 +436,13 @@ def window_ref(qkv, lens, h, hk, left, right, sinks):
     return out, mag, top
 
 
-def window_check(got, qkv, lens, h, hk, left, right, sinks, tensor_cores, first=0):
+def window_check(got, qkv, lens, h, hk, left, right, sinks, tensor_cores, first=0, hide=None):
     """An output is sum p v / sum p.  Scores: d products and sums in f32, off by (d + 4) 2^-24 of
     sum |q k| / sqrt(d) =: top, so p is off by that share (and 2^-21 for the exponential and its
     argument's rounding at |argument| <= 2 top log2 e).  On tensor cores each p is also rounded to
     the rows' 16-bit type (u), against an unrounded sum.  The sums over up to n keys in f32 add
     n 2^-24.  All of it is a share of sum p |v| / sum p; the store rounds once."""
-    ref, mag, top = window_ref(qkv, lens, h, hk, left, right, sinks)
+    ref, mag, top = window_ref(qkv, lens, h, hk, left, right, sinks, hide)
     d = qkv.shape[1] // (h + 2 * hk)
     u = torch.finfo(qkv.dtype).eps / 2
     share = 2 * ((d + 8) * 2.0 ** -24 * top + 2.0 ** -21) + max(lens, default=0) * 2.0 ** -23 + (u if tensor_cores else 0)
@@ -522,6 +545,76 @@ def test_attention_window_leaves_other_rows(dev, dt):
     full = torch.where(torch.arange(n + 70, device=dev)[:, None] < n, ctx, torch.zeros_like(ctx))
     window_check(full, clean, [n], h, h, 64, 64, 2, dt == "bf16", first=200)
     assert ctx[5:100].isnan().all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("left,right", [(64, 64), (300, 20)])
+@pytest.mark.parametrize("gap", [60, 100, 123, 125, 127, 129, 200, 2000])
+def test_attention_window_own_score_far_below_the_others(dev, gap, left, right, dt):
+    """Every other query's score with its own key lies ``gap`` powers of two below those of half of
+    the keys it sees."""
+    t, n, d, g = DTYPES[dt], 500, 64, _gen(gap)
+    qkv = torch.zeros((n, 3 * d), device=dev)
+    qkv[:, 0] = 8.0
+    qkv[::2, d] = gap * math.log(2)  # 8 k / sqrt(64) log2(e) = gap
+    qkv[:, 2 * d:] = torch.randn((n, d), generator=g, device=dev)
+    qkv = qkv.to(t)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    got = _ops().attention_window(qkv, cu, 1, n, left, right)
+    _ops().sync()
+    window_check(got, qkv, [n], 1, 1, left, right, 0, t != torch.float32)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("left,right,sinks", [(64, 64, 0), (300, 300, 0), (300, 20, 3)])
+def test_attention_window_scores_of_minus_infinity(dev, left, right, sinks, d, dt):
+    """Keys at minus infinity, a query's own and whole leading blocks among them, weigh nothing."""
+    t, n, g = DTYPES[dt], 700, _gen(d + left)
+    qkv = torch.randn((n, 3 * d), generator=g, device=dev)
+    hide = torch.arange(n, device=dev) % 2 == 1
+    if left == 300 and not sinks:
+        hide[:200] = True
+    root = math.sqrt(d)
+    qkv[:, 0] = root / 2
+    qkv[:, d] = torch.where(hide, -math.inf, -28.0)  # visible keys: scores near -14
+    qkv = qkv.to(t)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    got = _ops().attention_window(qkv, cu, 1, n, left, right, sinks=sinks)
+    _ops().sync()
+    clean = qkv.clone()
+    clean[hide, d] = -28.0
+    window_check(got, clean, [n], 1, 1, left, right, sinks, t != torch.float32, hide=hide)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("left,right,sinks", [(64, 64, 1), (300, 20, 3), (10 ** 6, 0, 0)])
+def test_attention_window_infinite_value(dev, left, right, sinks, dt):
+    """An infinite value reaches the queries that see it, in its column, and nothing else."""
+    t, n, d, key, g = DTYPES[dt], 900, 64, 400, _gen(left)
+    qkv = torch.randn((n, 3 * d), generator=g, device=dev).to(t)
+    clean = qkv.clone()
+    qkv[key, 2 * d + 5] = math.inf
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    got = _ops().attention_window(qkv, cu, 1, n, left, right, sinks=sinks)
+    _ops().sync()
+    i = torch.arange(n, device=dev)
+    sees = (key <= i + right) & (key >= i - left)
+    assert (got[sees, 5] == math.inf).all()
+    got[sees, 5] = window_ref(clean, [n], 1, 1, left, right, sinks)[0].to(t)[sees, 5]
+    window_check(got, clean, [n], 1, 1, left, right, sinks, t != torch.float32)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_attention_window_values_of_nan_alone(dev, dt):
+    """No query waits long for a long row without one finite value."""
+    n, d = 40000, 64
+    qkv = torch.randn((n, 3 * d), generator=_gen(1), device=dev).to(DTYPES[dt])
+    qkv[:, 2 * d:] = math.nan
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    got = _ops().attention_window(qkv, cu, 1, n, n, n)
+    _ops().sync()
+    assert got.isnan().all()
 
 
 def test_attention_window_refusals(dev):
