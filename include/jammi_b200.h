@@ -256,8 +256,9 @@ jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamm
  *   of jb_op_linear_s8).  A row whose y holds a NaN or an infinity has scale
  *   NaN and q 0.
  * dtype F32, BF16 or F16; gamma f32 [cols]; any cols >= 1 (cols that are a
- * multiple of 16 bytes, up to 2048 16-byte vectors, with 16-byte aligned
- * buffers take the vectorised kernels).  sum and y may replace x or residual.
+ * multiple of 16 bytes, up to 4096 16-byte vectors, with 16-byte aligned
+ * buffers take the vectorised kernels).  The squares are summed in f32: rows
+ * whose sum of squares passes its range come out as 0.  sum and y may replace x or residual.
  * No counterpart in the reference (its encoders use LayerNorm). */
 jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma, void* sum,
                         void* y, int8_t* q, float* scale, int dtype, int rows, int cols,

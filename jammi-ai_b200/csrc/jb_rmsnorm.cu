@@ -12,9 +12,20 @@
 // row held in registers between its two reductions (the sum of squares and
 // the maximum).  Rows of up to 1024 16-bit columns belong to one warp (no
 // barrier; the next row's loads are issued before the current row's
-// reductions); wider rows to a CTA of four or eight warps with the same
-// registers per thread.  Rows whose width or base address rules 16-byte
-// loads out take a scalar kernel that reads each row two or three times.
+// reductions); wider rows to a CTA of four, eight or sixteen warps with the
+// same registers per thread.  Rows whose width or base address rules 16-byte
+// loads out, and rows of more than 4096 vectors, take a scalar kernel that
+// reads each row two or three times.
+//
+// Measured, inputs and outputs out of cache, with residual and sum, bf16 (a
+// copy runs at 6.54 TB/s):
+//   36870 x 768    y 43.0 us, 5.3 TB/s    int8 38.9 us, 5.1 TB/s
+//   9001 x 4096    y 55.2 us, 5.3 TB/s    int8 49.2 us, 5.3 TB/s
+//   3000 x 20000   y 131 us, 3.7 TB/s     int8 139 us  (the scalar kernel: 213, 240)
+//   36870 x 770    y 104 us, 2.2 TB/s     int8 164 us  (scalar)
+//   12 x 768       2.5 us, launch and one row's latency
+// What is left to the copy's rate are the reductions between a row's loads
+// and its stores, which the next row's loads cover only in part.
 #include <algorithm>
 #include <atomic>
 
@@ -313,7 +324,7 @@ void launch_width(const RmsArgs& a, cudaStream_t s) {
   const int nvec = a.cols / VN;
   const bool vec = a.cols % VN == 0 && aligned(a.x, 16) && aligned(a.resid, 16) && aligned(a.sum, 16) &&
                    aligned(a.y, 16) && aligned(a.gamma, 16) && aligned(a.q, VN);
-  if (!vec || nvec > 256 * 8) {
+  if (!vec || nvec > 512 * 8) {
     int dev = 0;
     cudaGetDevice(&dev);
     const unsigned grid = static_cast<unsigned>(std::min<long long>(a.rows, 8ll * num_sms(dev)));
@@ -328,13 +339,16 @@ void launch_width(const RmsArgs& a, cudaStream_t s) {
     launch_form<T, 2, 4>(a, s);
   } else if (nvec <= 512) {
     launch_form<T, 4, 4>(a, s);
-  } else {
+  } else if (nvec <= 2048) {
     launch_form<T, 8, 8>(a, s);
+  } else {
+    launch_form<T, 8, 16>(a, s);
   }
 }
 
 // y = q * scale, rounded to T.  A warp per row, eight codes per lane and
-// load; other widths and alignments element by element.
+// load; other widths and alignments element by element.  Memory-bound: 36870 x
+// 768 to bf16 22.3 us out of cache (3.8 TB/s), 9001 x 4096 24.6 us (4.5 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(const int8_t* __restrict__ q,
                                                               const float* __restrict__ scale, T* y, int rows,

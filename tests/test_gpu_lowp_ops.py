@@ -56,7 +56,7 @@ def sum_depth(cols):
 
 
 RMS_SHAPES = [(1, 1), (1, 8), (3, 7), (12, 768), (5, 33), (257, 384), (1000, 1024), (9, 1032), (130, 1536), (33, 2056),
-              (17, 4096), (5, 4100), (3, 16384), (2, 16392), (2, 20001)]
+              (17, 4096), (5, 4100), (3, 16384), (2, 16392), (2, 20001), (700, 16400), (3, 32768), (2, 32776)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
