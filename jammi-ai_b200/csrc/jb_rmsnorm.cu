@@ -14,16 +14,15 @@
 // barrier; the next row's loads are issued before the current row's
 // reductions); wider rows to a CTA of four, eight or sixteen warps with the
 // same registers per thread.  Rows whose width or base address rules 16-byte
-// loads out, and rows of more than 4096 vectors, take a scalar kernel that
-// reads each row two or three times.
+// loads out, and rows of more than 4096 vectors, are read element by element.
 //
 // Measured, inputs and outputs out of cache, with residual and sum, bf16 (a
 // copy runs at 6.54 TB/s):
 //   36870 x 768    y 43.0 us, 5.3 TB/s    int8 38.9 us, 5.1 TB/s
 //   9001 x 4096    y 55.2 us, 5.3 TB/s    int8 49.2 us, 5.3 TB/s
 //   3000 x 20000   y 131 us, 3.7 TB/s     int8 139 us  (the scalar kernel: 213, 240)
-//   36870 x 770    y 104 us, 2.2 TB/s     int8 164 us  (scalar)
-//   12 x 768       2.5 us, launch and one row's latency
+//   36870 x 770    y 80 us, 2.8 TB/s      int8 94 us   (single elements)
+//   12 x 768       2.1 us, int8 2.4: launch and one row's latency
 // What is left to the copy's rate are the reductions between a row's loads
 // and its stores, which the next row's loads cover only in part.
 #include <algorithm>
@@ -239,9 +238,68 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) rmsnorm_kernel(RmsArgs 
   }
 }
 
-// Any width and alignment: a CTA per row, each element read again in every
-// pass and every output written in the last one (so outputs may replace
-// inputs element for element).
+// Narrow rows of any width and alignment: a warp per row with single elements,
+// E of them per lane.  Up to 1024 columns (36870 x 770 bf16 with residual 80 us,
+// int8 94; f32 without residual 64, int8 74; the form below, a CTA per row, takes
+// 104, 164, 100, 150), but 256 of f32 with a residual, where the misaligned
+// lines of two wide rows do not stay in L1 from one warp access to the next
+// (36870 x 770: 215 us, int8 219; below 103 and 152).
+template <typename T, int E>
+__global__ void __launch_bounds__(256) rmsnorm_ragged_kernel(RmsArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int row = blockIdx.x * 8 + warp; row < a.rows; row += gridDim.x * 8) {
+    const size_t off = static_cast<size_t>(row) * a.cols;
+    const T* x = static_cast<const T*>(a.x) + off;
+    float v[E];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = lane + 32 * i < a.cols ? to_f(x[lane + 32 * i]) : 0.f;
+    if (a.resid) {
+      const T* r = static_cast<const T*>(a.resid) + off;
+      T t[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (lane + 32 * i < a.cols) t[i] = r[lane + 32 * i];
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (lane + 32 * i < a.cols) v[i] += to_f(t[i]);
+      if (a.sum) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (lane + 32 * i < a.cols) static_cast<T*>(a.sum)[off + lane + 32 * i] = from_f<T>(v[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
+    const float rstd = 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(a.cols) + a.eps);
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int c = lane + 32 * i;
+      if (c < a.cols) {
+        v[i] = v[i] * rstd * __ldg(a.gamma + c);
+        top = max(top, abs_bits(v[i]));
+        if (a.y) static_cast<T*>(a.y)[off + c] = from_f<T>(v[i]);
+      }
+    }
+    if (a.q) {
+      const RowQuant rq = row_quant(__reduce_max_sync(0xffffffffu, top));
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int c = lane + 32 * i;
+        if (c < a.cols)
+          a.q[off + c] = static_cast<int8_t>(rint_byte(rq.up == 0.f ? 0.f : v[i] * rq.up, rq.inv) & 0xffu);
+      }
+      if (lane == 0) a.scale[row] = rq.scale;
+    }
+  }
+}
+
+// Wider rows of any width and alignment: a CTA per row, each element read
+// again (mostly out of L1) in every pass and every output written in the last
+// one (so outputs may replace inputs element for element).  9001 x 4095 bf16
+// with residual 90 us, int8 101 us; with the row in registers 96 to 113 us
+// (fewer loads in flight).
 template <typename T>
 __global__ void __launch_bounds__(256) rmsnorm_scalar_kernel(RmsArgs a) {
   __shared__ float red[8];
@@ -266,7 +324,7 @@ __global__ void __launch_bounds__(256) rmsnorm_scalar_kernel(RmsArgs a) {
     RowQuant rq{1.f, 0.f, 0.f};
     if (a.q) {
       unsigned top = 0;
-      for (int c = threadIdx.x; c < a.cols; c += 256) top = max(top, abs_bits(s_at(c) * rstd * a.gamma[c]));
+      for (int c = threadIdx.x; c < a.cols; c += 256) top = max(top, abs_bits(s_at(c) * rstd * __ldg(a.gamma + c)));
       top = __reduce_max_sync(0xffffffffu, top);
       if (lane == 0) redm[warp] = top;
       __syncthreads();
@@ -276,7 +334,7 @@ __global__ void __launch_bounds__(256) rmsnorm_scalar_kernel(RmsArgs a) {
     }
     for (int c = threadIdx.x; c < a.cols; c += 256) {
       const float s = s_at(c);
-      const float y = s * rstd * a.gamma[c];
+      const float y = s * rstd * __ldg(a.gamma + c);
       if (a.sum) static_cast<T*>(a.sum)[off + c] = from_f<T>(s);
       if (a.q)
         a.q[off + c] = static_cast<int8_t>(rint_byte(rq.up == 0.f ? 0.f : y * rq.up, rq.inv) & 0xffu);
@@ -318,6 +376,11 @@ void launch_form(const RmsArgs& a, cudaStream_t s) {
   else
     a.resid ? launch_rows<T, MAXV, W, true, false>(a, s) : launch_rows<T, MAXV, W, false, false>(a, s);
 }
+template <typename T, int E>
+void launch_ragged(const RmsArgs& a, cudaStream_t s) {
+  constexpr auto kern = rmsnorm_ragged_kernel<T, E>;
+  kern<<<wave<kern>(256, (a.rows + 7ll) / 8), 256, 0, s>>>(a);
+}
 template <typename T>
 void launch_width(const RmsArgs& a, cudaStream_t s) {
   constexpr int VN = Row<T>::N;
@@ -325,10 +388,13 @@ void launch_width(const RmsArgs& a, cudaStream_t s) {
   const bool vec = a.cols % VN == 0 && aligned(a.x, 16) && aligned(a.resid, 16) && aligned(a.sum, 16) &&
                    aligned(a.y, 16) && aligned(a.gamma, 16) && aligned(a.q, VN);
   if (!vec || nvec > 512 * 8) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const unsigned grid = static_cast<unsigned>(std::min<long long>(a.rows, 8ll * num_sms(dev)));
-    rmsnorm_scalar_kernel<T><<<grid, 256, 0, s>>>(a);
+    if (a.cols <= 256) {
+      launch_ragged<T, 8>(a, s);
+    } else if (a.cols <= 1024 && (sizeof(T) == 2 || !a.resid)) {
+      launch_ragged<T, 32>(a, s);
+    } else {
+      rmsnorm_scalar_kernel<T><<<wave<rmsnorm_scalar_kernel<T>>(256, a.rows), 256, 0, s>>>(a);
+    }
   } else if (nvec <= 32) {
     launch_form<T, 1, 1>(a, s);
   } else if (nvec <= 96) {

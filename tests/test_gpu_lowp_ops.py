@@ -56,7 +56,7 @@ def sum_depth(cols):
 
 
 RMS_SHAPES = [(1, 1), (1, 8), (3, 7), (12, 768), (5, 33), (257, 384), (1000, 1024), (9, 1032), (130, 1536), (33, 2056),
-              (17, 4096), (5, 4100), (3, 16384), (2, 16392), (2, 20001), (700, 16400), (3, 32768), (2, 32776)]
+              (17, 4096), (5, 4100), (3, 16384), (2, 16392), (2, 20001), (700, 16400), (3, 32768), (2, 32776), (1300, 201), (30, 1501), (5, 4095), (3, 256), (3, 1023), (7, 2049), (70, 225), (33, 226), (40, 993), (40, 994), (9, 2017), (9, 2018), (11, 4065), (11, 4066)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
