@@ -351,6 +351,12 @@ __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
 }
+__device__ __forceinline__ float tmem_ld_1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  tmem_wait_ld();
+  return __uint_as_float(r);
+}
 template <bool H16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if constexpr (H16) {
@@ -372,6 +378,20 @@ __device__ __forceinline__ uint32_t low_bits(int c) {
 __host__ __device__ constexpr uint32_t p_col(int k) {
   const int piece = k >> 1;
   return static_cast<uint32_t>((piece < 6 ? 32 * piece : 32 * (piece - 6) + 16) + 8 * (k & 1));
+}
+
+// The score column of a single-block item that a warp's rows take as their
+// reference: a key of the window near the middle of the warp's own ones
+// (`near`), else a sink.  Its column is one that P never overwrites (the second
+// half of a piece, of pieces 2 to 5 where 6 and 7 put P into 0 and 1), since
+// the two warps of a row read it at different times.  (Items of 16 columns have
+// one piece, and one warp that uses the reference.)
+__device__ __forceinline__ int ref_col(int nw, int nw16, int nv, int s_end, int near) {
+  if (nw > 16 && (nv <= 192 || nw > 80)) {
+    const int piece = min(near >> 5, (nw - 17) >> 5);  // its column 16 is a key
+    return 32 * (nv > 192 ? max(piece, 2) : piece) + 16;
+  }
+  return nv > 192 ? 144 : s_end > 0 ? nw16 : 0;  // nw <= 80, nv > 192: columns 80 to 176 are sinks
 }
 
 // Output columns [c0, c1) of one query row over its visible keys only, in f32
@@ -739,26 +759,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!warp_mbar_wait(sfull, bc & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         if (active && !H16 && nb == 1) {
-          // The reference is the row's score with its own key, which it always
-          // sees: bf16 P has f32's range, so any reference within 2^100 of the
+          // The reference is the row's score with one key of the item (see ref_col):
+          // bf16 P has f32's range, so any reference within 2^100 of the row's
           // maximum gives the same relative rounding, and no maximum is needed.
-          // Both warps of a row read it.
-          // (p beyond f32 makes the sum or the outputs infinite: window_row_exact.)
-          const int d0 = q0 + 32 * quarter - k_begin;  // lane 0's own column
-          const int col = min(d0, 256 - 32);           // inside the slot's columns
-          uint32_t s[32];
-          tmem_ld_32x32b_x32(trow + col, s);
-          const int at = min(lane + d0 - col, 31);
-          tmem_wait_ld();
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-            for (int i = 0; i < o; ++i) s[i] = at & o ? s[i + o] : s[i];
-          mref = mine ? __uint_as_float(s[0]) * w.scale_log2 : 0.f;
-          // the column may lie in a piece that the other warp overwrites with P
-          tc_fence_before();
-          if (!meet()) { ok = false; break; }
-          tc_fence_after();
+          // (A sum outside that range: window_row_exact.)
+          mref = tmem_ld_1(trow + ref_col(nw, nw16, nv, s_end, q0 + 32 * quarter - k_begin + 16)) * w.scale_log2;
         } else if (active) {
           float mx = -INFINITY;
 #pragma unroll 1
@@ -922,13 +927,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       __syncwarp();
-      // An infinite sum (the row's own score lies far below another one) hides in
-      // outputs of 0.  A sum that is NaN has a NaN score in it: the outputs are NaN.
-      // Else a value that the row does not see may be the one that is not finite;
-      // long ranges are computed again only if there is one.
-      // A reference of -infinity (the row's own score is) says nothing about the others.
-      const bool unsafe = !(zero2.x + zero2.y == 0.f && l_row < INFINITY) || (nb == 1 && mref == -INFINITY);
-      if (mine && unsafe && l_row == l_row) {
+      // One block: a sum far from 1 has a reference far from the row's maximum (its
+      // outputs may even be 0), one that is NaN perhaps a hidden one.  Several
+      // blocks: a NaN sum has a NaN score in it, and the outputs are NaN; else a
+      // value that the row does not see may be the one that is not finite.
+      const bool sound = zero2.x + zero2.y == 0.f && l_row < INFINITY;
+      if (mine && !(sound && (nb > 1 || l_row > 0x1p-100f)) && (nb == 1 || l_row == l_row)) {
         const int c0 = half * (D / 2), c1 = c0 + D / 2;
         if (nb == 1 || hidden_not_finite<T, D>(w, start, n, h, qi, k_begin, nw, s_end, c0, c1))
           window_row_exact<T, D>(w, start, n, h, qi, c0, c1);

@@ -549,14 +549,15 @@ def test_attention_window_leaves_other_rows(dev, dt):
 
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("left,right", [(64, 64), (300, 20)])
-@pytest.mark.parametrize("gap", [60, 100, 123, 125, 127, 129, 200, 2000])
-def test_attention_window_own_score_far_below_the_others(dev, gap, left, right, dt):
-    """Every other query's score with its own key lies ``gap`` powers of two below those of half of
-    the keys it sees."""
+@pytest.mark.parametrize("gap", [60, 100, 123, 125, 127, 129, 200, 2000, -100, -2000])
+@pytest.mark.parametrize("at,of", [(0, 2), (1, 2), (16, 32), (5, 32), (48, 500), (200, 500)])
+def test_attention_window_scores_far_apart(dev, gap, at, of, left, right, dt):
+    """A query's scores with some of the keys that it sees, or that its neighbours see, lie ``gap``
+    powers of two above the others."""
     t, n, d, g = DTYPES[dt], 500, 64, _gen(gap)
     qkv = torch.zeros((n, 3 * d), device=dev)
     qkv[:, 0] = 8.0
-    qkv[::2, d] = gap * math.log(2)  # 8 k / sqrt(64) log2(e) = gap
+    qkv[at::of, d] = gap * math.log(2)  # 8 k / sqrt(64) log2(e) = gap
     qkv[:, 2 * d:] = torch.randn((n, d), generator=g, device=dev)
     qkv = qkv.to(t)
     cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
