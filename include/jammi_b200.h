@@ -321,8 +321,8 @@ jb_status jb_op_attention_rows(const void* qkv, const int* cu_seqlens, void* ctx
  * of qkv behind cu_seqlens[batch] are not read and of ctx not written.  left,
  * right: 0 .. 2^31 - 1 (anything >= the row's length: unbounded).  dtype F32,
  * BF16 or F16; head_dim 8, 16, 32, 64 or 128; heads a multiple of kv_heads;
- * max_len bounds every row's length, rows >= cu_seqlens[batch]; qkv and ctx
- * 16-byte aligned.  No counterpart in the reference (its ModernBERT layers
+ * max_len bounds every row's length (of a longer row the first max_len tokens
+ * are a row), rows >= cu_seqlens[batch]; qkv and ctx 16-byte aligned.  No counterpart in the reference (its ModernBERT layers
  * attend to the whole row, crates/jammi-encoders/src/modernbert.rs). */
 jb_status jb_op_attention_window(const void* qkv, const int* cu_seqlens, void* ctx, int dtype,
                                  int batch, int heads, int kv_heads, int head_dim, int max_len,

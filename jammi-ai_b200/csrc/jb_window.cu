@@ -32,14 +32,15 @@ struct WinParams {
   void* ctx;
   int heads, kv_heads;
   int rows;      // rows that qkv and ctx hold
+  int max_len;   // of a row
   int q_blocks;  // query blocks of the longest row
   int left, right, sinks;
   float scale_log2;
 };
 
-// Tokens of row b that lie inside the buffers, whatever the offsets hold.
+// Tokens of row b that lie inside the buffers and max_len, whatever the offsets hold.
 __device__ __forceinline__ int row_tokens(const WinParams& p, int b, int start) {
-  return start < 0 ? 0 : max(0, min(p.cu[b + 1], p.rows)) - start;
+  return start < 0 ? 0 : min(max(0, min(p.cu[b + 1], p.rows)) - start, p.max_len);
 }
 
 // ── any head width, f32 arithmetic ──────────────────────────────────────────
@@ -256,18 +257,22 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 // ── tcgen05, 16-bit rows with head_dim 32, 64 or 128 ────────────────────────
 // A persistent CTA per SM runs two independent slots, each on its own items
 // (row, head, kq-query block) with its own shared memory and half of TMEM:
-//   TMA warp      publishes the slot's items in a two-entry ring and loads
+//   TMA warp      publishes the slot's items in a ring of four and loads
 //                 each one's Q and then, per key block, K and V.
 //   MMA warp      S = Q K^T (M = 128, N = the block's keys) into columns
-//                 [0, N), then O (+)= P V with P read from TMEM.
+//                 [0, N), then O (+)= P V with P read from TMEM.  The next
+//                 item's S comes right behind, before O is read, unless it
+//                 is so wide that it would overwrite it.
 //   8 softmax     two threads per query row, which take the block's 32-key
-//   warps         pieces in turn (even / odd) and exchange their maxima and
-//                 sums.  Two passes over the scores in TMEM (maximum;
-//                 exponentials and sum); a warp skips the pieces that none of
+//   warps         pieces in turn (even / odd).  Two passes over the scores in
+//                 TMEM (maximum, which the two exchange; exponentials and sum),
+//                 or one (see ref_col); a warp skips the pieces that none of
 //                 its 32 queries sees.  P (16-bit pairs) overwrites the
 //                 scores of its own piece: no thread writes where the other
-//                 one still reads.  O / sum goes out through shared memory in
-//                 whole row segments.
+//                 one still reads.
+// and four warps for both slots' outputs: O / sum goes out through shared
+// memory in whole row segments while the softmax warps are at the next item
+// (256 x [32,256]: 75 us with the softmax warps writing them, 69 us).
 // The keys of an item are its window [k_begin, k_end), padded to 16, then the
 // first keys [0, s_end) that the window has left behind, padded to 16.  With
 // head_dim 32 or 64, an item of up to 256 keys is ONE block: no running maximum, no
@@ -290,22 +295,30 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 // graphs share nothing.
 //
 // Measured, bf16 unless said, window 64 + 64 (out of cache):
-//   256 rows of 32 to 256 tokens, 12 heads of 64, 1 sink   75 us  3.0 TB/s
-//   8 rows of 4000 to 8192, 16 heads of 64                110 us  3.4 TB/s, f16 114 us
-//   64 x 512 tokens, 12 heads of 32                         51 us
-//   64 x 512 tokens, 6 heads of 128, 3 key heads            61 us
-//   64 x 512 tokens, 12 heads of 64, unbounded             150 us  344 TFLOP/s
-//   one row of 12 tokens                                   6.5 us
-// What bounds it is the chain of an item (load, S, P, O, store) at two items
-// per SM: without the exponentials and masks it took 15% less, without the
-// stores 7%, without P V 8%.  f16 makes the maximum pass that bf16 saves.
+//   256 rows of 32 to 256 tokens, 12 heads of 64, 1 sink   67 us  3.3 TB/s
+//   8 rows of 4000 to 8192, 16 heads of 64                100 us  3.7 TB/s, f16 109 us
+//   64 x 512 tokens, 12 heads of 32                         45 us
+//   64 x 512 tokens, 6 heads of 128, 3 key heads            55 us
+//   64 x 512 tokens, 12 heads of 64, unbounded             144 us  357 TFLOP/s
+//   one row of 12 tokens                                   4.8 us from its first instruction to its last
+// What bounds it: an item's chain P -> O -> next S leaves the softmax warps
+// idle for a third of its 6300 clocks; their exponentials take half of them,
+// 16 a clock (two slots' at once).  More code in any role costs more than it
+// saves (a second, unmasked copy of the exponentials: 69 -> 71 us; P V in two
+// parts, the first behind half of P: 69 -> 72 us; an unmasked copy of the
+// maximum: 67 -> 69 us): the roles' loops share small instruction caches.
+// Items dealt by equal cost in contiguous runs instead of in turn: 69 -> 83 us
+// (neighbouring heads of a token are then not read at the same time).  f16
+// makes the maximum pass that bf16 saves.
 //
 // Every wait is bounded; on a timeout each role stops, copies and MMAs in
 // flight are waited for (bounded), the error flag is set and TMEM is freed.
-constexpr int kTcWarps = 20;      // 2 TMA, 2 MMA, 16 softmax
+constexpr int kTcWarps = 24;      // 2 TMA, 2 MMA, 16 softmax, 4 output
 constexpr int kTcThreads = 32 * kTcWarps;
 constexpr int kGroupWarps = 8;    // softmax warps of a slot
+constexpr int kSlotBars = 128;    // bytes of a slot's barriers
 constexpr int kPrefixRows = 2048;
+constexpr int kRounds = (kPrefixRows + kTcThreads - 1) / kTcThreads;
 constexpr float kRescale = 8.f;   // lazy-rescaling threshold, log2 units
 
 template <int D>
@@ -318,10 +331,10 @@ struct TcCfg {
   static constexpr int KV_BYTES = HALVES * KEYS * ROW;
   static constexpr int SLOT_BYTES = Q_BYTES + 2 * KV_BYTES;
   static constexpr int O_COL = 256 - D;                    // O's columns of a slot
-  static constexpr int SEG = D == 64 ? 64 : 32;            // bytes of a row that a warp stores at once
-  static constexpr int STAGE_BYTES = 2 * kGroupWarps * 32 * SEG;
-  static constexpr int XCH_BYTES = 2 * (2 + 1) * 4 * 2 * 32 * 4;  // [slot][max 0, max 1, sum][quarter][half][lane]
-  static constexpr int META_BYTES = 512;
+  static constexpr int SEG = D == 32 ? 64 : 128;           // bytes of a row that an output warp stores at once
+  static constexpr int STAGE_BYTES = 4 * 32 * SEG;
+  static constexpr int XCH_BYTES = 2 * 4 * 4 * 2 * 32 * 4;  // [slot][max 0, max 1, sum 0, sum 1][quarter][half][lane]
+  static constexpr int META_BYTES = 640;
   static constexpr int USED = 1024 + 2 * SLOT_BYTES + STAGE_BYTES + XCH_BYTES + (kPrefixRows + 4) * 4 + META_BYTES;
   // more than half of an SM's: two CTAs cannot share its TMEM
   static constexpr int SMEM = USED > 120 * 1024 ? USED : 120 * 1024;
@@ -473,51 +486,76 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   float* xch = reinterpret_cast<float*>(smem_raw + (staging + C::STAGE_BYTES - raw));
   int* prefix = reinterpret_cast<int*>(xch) + C::XCH_BYTES / 4;  // [batch + 1] query blocks before each row
   uint8_t* meta = reinterpret_cast<uint8_t*>(prefix + kPrefixRows + 4);
-  const int g = warp < 4 ? warp & 1 : (warp - 4) / kGroupWarps;  // this warp's slot
+  const int g = warp < 4 ? warp & 1 : (warp - 4) / kGroupWarps & 1;  // this warp's slot
   const uint32_t sQ = base + g * C::SLOT_BYTES, sK = sQ + C::Q_BYTES, sV = sK + C::KV_BYTES;
-  const uint32_t bars = smem_u32(meta) + g * 112;
+  const uint32_t bars = smem_u32(meta) + g * kSlotBars;
   const uint32_t ifull = bars;         // [2] an item is published
   const uint32_t kfull = bars + 16;    // K (and Q) of a block loaded
   const uint32_t vfull = bars + 24;
   const uint32_t sfull = bars + 32;    // S written: K (and Q) read
   const uint32_t pfull = bars + 40;    // P written
   const uint32_t ofull = bars + 48;    // P V done: V read
-  const uint32_t sfree = bars + 56;    // O read: the slot's TMEM is free
+  const uint32_t sfree = bars + 56;    // O read
   const uint32_t spare = bars + 64;
   const uint32_t pairs = bars + 72;    // [4] the two warps of a lane quarter meet
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(meta + 224);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 228);
-  volatile TcItem* ring = reinterpret_cast<volatile TcItem*>(meta + 256) + 2 * g;
-  static_assert(256 + 4 * sizeof(TcItem) <= C::META_BYTES, "meta layout");
+  const uint32_t odone = bars + 104;   // an item's last P V done
+  const uint32_t lfull = bars + 112;   // [2] an item's sums written
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(meta + 2 * kSlotBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 2 * kSlotBars + 4);
+  volatile int* ends = reinterpret_cast<volatile int*>(meta + 2 * kSlotBars + 8);  // [2] a slot's number of items
+  // four items a slot: the TMA warp is up to two ahead of the output warps
+  volatile TcItem* rings = reinterpret_cast<volatile TcItem*>(meta + 2 * kSlotBars + 16);
+  volatile TcItem* ring = rings + 4 * g;
+  static_assert(2 * kSlotBars + 16 + 8 * sizeof(TcItem) <= C::META_BYTES, "meta layout");
   const WinParams& w = p.w;
   const bool counted = p.batch <= kPrefixRows;
 
-  if (warp == 0 && counted) {  // query blocks before each row
-    int sum = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+  if (warp == 1 && lane == 0) {
+    prefetch_tensormap(&tm64);
+    prefetch_tensormap(&tm16);
+  }
+  // Query blocks before each row: a scan by all warps, kTcThreads rows a round.
+  int incl[kRounds], mine_blocks[kRounds];
+  if (counted) {
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int b = i * kTcThreads + threadIdx.x;
       int blocks = 0;
-      if (b0 + lane < p.batch) {
-        const int n = row_tokens(w, b0 + lane, w.cu[b0 + lane]);
-        if (n > 0) blocks = (min(n, w.q_blocks * p.kq) + p.kq - 1) / p.kq;
+      if (b < p.batch) {
+        const int n = row_tokens(w, b, w.cu[b]);
+        if (n > 0) blocks = (n + p.kq - 1) / p.kq;
       }
-      int incl = blocks;
+      mine_blocks[i] = blocks;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
+        const int up = __shfl_up_sync(0xffffffffu, blocks, o);
+        if (lane >= o) blocks += up;
       }
-      if (b0 + lane < p.batch) prefix[b0 + lane] = sum + incl - blocks;
-      sum += __shfl_sync(0xffffffffu, incl, 31);
+      incl[i] = blocks;
+      if (lane == 31) reinterpret_cast<int*>(xch)[i * kTcWarps + warp] = blocks;
     }
-    if (lane == 0) prefix[p.batch] = sum;
+    __syncthreads();
+    int before = 0, at = 0;  // blocks of the warps before this one
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      if (i * kTcThreads < p.batch || i == 0) {
+        for (; at < i * kTcWarps + warp; ++at) before += reinterpret_cast<int*>(xch)[at];
+        const int b = i * kTcThreads + threadIdx.x;
+        if (b < p.batch) prefix[b] = before + incl[i] - mine_blocks[i];
+        if (b == p.batch - 1) prefix[p.batch] = before + incl[i];
+      }
+    }
   }
   if (threadIdx.x == 64) {
     for (int s = 0; s < 2; ++s) {
-      const uint32_t b = smem_u32(meta) + s * 112;
-      for (int i = 0; i < 9; ++i) mbar_init(b + 8 * i, i == 5 || i == 7 ? kGroupWarps : 1);  // 5: pfull, 7: sfree
+      const uint32_t b = smem_u32(meta) + s * kSlotBars;
+      for (int i = 0; i < 9; ++i) mbar_init(b + 8 * i, i == 5 ? kGroupWarps : i == 7 ? 4 : 1);  // 5: pfull, 7: sfree
       for (int i = 9; i < 13; ++i) mbar_init(b + 8 * i, 2);
+      mbar_init(b + 104, 1);
+      for (int i = 14; i < 16; ++i) mbar_init(b + 8 * i, kGroupWarps);
     }
     *abort_flag = 0;
+    ends[0] = ends[1] = -1;
     fence_barrier_init();
   }
   if (warp == 3) tmem_alloc(smem_u32(tslot), 512);  // all of it (one CTA per SM): the base is column 0
@@ -536,7 +574,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // registers (see jb_mxfp4_gemm.cu).
   if (warp < 2) {  // ── TMA
     const long long items =
-        (counted ? static_cast<long long>(prefix[p.batch]) : static_cast<long long>(p.batch) * w.q_blocks) * w.heads;
+        counted ? min(static_cast<long long>(prefix[p.batch]) * w.heads, static_cast<long long>(INT32_MAX))
+                : static_cast<long long>(p.batch) * w.q_blocks * w.heads;
     const long long stride = 2ll * gridDim.x;
     int bc = 0, m = 0;  // blocks loaded, items published
     bool ok = true;
@@ -545,10 +584,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const long long f = f0 + lane * stride;
       int start = 0, n = 0, h = 0, q0 = 0;  // this lane's candidate
       if (f < items) {
-        h = static_cast<int>(f % w.heads);
-        const long long bq = f / w.heads;
         int b, qb;
         if (counted) {
+          const int bq = static_cast<int>(f) / w.heads;
+          h = static_cast<int>(f) - bq * w.heads;
           int lo = 0, hi = p.batch;  // prefix[lo] <= bq < prefix[hi]
           while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -556,8 +595,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             else hi = mid;
           }
           b = lo;
-          qb = static_cast<int>(bq) - prefix[lo];
+          qb = bq - prefix[lo];
         } else {
+          const long long bq = f / w.heads;
+          h = static_cast<int>(f - bq * w.heads);
           b = static_cast<int>(bq / w.q_blocks);
           qb = static_cast<int>(bq % w.q_blocks);
         }
@@ -608,7 +649,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int boxes = (min(it.n - it.q0, p.kq) + 63) >> 6;
           if (elect_one()) {
             if (j == 0) {
-              volatile TcItem& e = ring[m & 1];
+              volatile TcItem& e = ring[m & 3];
               e.live = 1; e.start = it.start; e.n = it.n; e.h = it.h; e.q0 = it.q0;
               e.k_begin = it.k_begin; e.nw = it.nw; e.s_end = it.s_end; e.nb = it.nb;
               mbar_arrive(ifull + 8 * (m & 1));
@@ -641,7 +682,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     if (lane == 0) {
       if (ok && (bc == 0 || mbar_wait(sfull, (bc - 1) & 1, abort_flag))) {  // no more items
-        ring[m & 1].live = 0;
+        ring[m & 3].live = 0;
         mbar_arrive(ifull + 8 * (m & 1));
         mbar_arrive(kfull);
       }
@@ -658,14 +699,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool ok = true;
     for (int m = 0; ok; ++m) {
       if (!warp_mbar_wait(kfull, bc & 1, abort_flag)) { ok = false; break; }
-      const volatile TcItem& e = ring[m & 1];
-      if (!e.live) break;
+      const volatile TcItem& e = ring[m & 3];
+      if (!e.live) {  // the output warps may go, once all of them have seen the last item
+        if (m > 0 && !warp_mbar_wait(sfree, (m - 1) & 1, abort_flag)) ok = false;
+        if (ok && lane == 0) {
+          ends[g] = m;
+          mbar_arrive(odone);
+        }
+        break;
+      }
       const int nv = __shfl_sync(0xffffffffu, ceil16(e.nw) + ceil16(e.s_end), 0);
       const int nb = __shfl_sync(0xffffffffu, e.nb, 0);
-      if (m > 0 && !warp_mbar_wait(sfree, (m - 1) & 1, abort_flag)) { ok = false; break; }
       for (int j = 0; j < nb; ++j, ++bc) {
         int v0, v1;
         block_of(nv, nb, j, v0, v1);
+        // The first S replaces the P of the item before, which P V has read, and,
+        // where it is wide, that item's O.
+        if (j == 0 && m > 0 &&
+            !(v1 - v0 <= C::O_COL ? warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag)
+                                  : warp_mbar_wait(sfree, (m - 1) & 1, abort_flag))) {
+          ok = false;
+          break;
+        }
         // S_j replaces P_{j-1}, which P V has read
         if (j > 0 &&
             (!warp_mbar_wait(kfull, bc & 1, abort_flag) || !warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag))) {
@@ -685,7 +740,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mma_commit(sfull);
         }
         __syncwarp();
-        if (!warp_mbar_wait(pfull, bc & 1, abort_flag) || !warp_mbar_wait(vfull, bc & 1, abort_flag)) {
+        // (P comes last)
+        if ((j == 0 && m > 0 && !warp_mbar_wait(sfree, (m - 1) & 1, abort_flag)) ||
+            !warp_mbar_wait(vfull, bc & 1, abort_flag) || !warp_mbar_wait(pfull, bc & 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -702,6 +759,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             (j > 0 || c > 0) ? 1u : 0u);
           }
           mma_commit(ofull);
+          if (j == nb - 1) mma_commit(odone);
         }
         __syncwarp();
       }
@@ -712,28 +770,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       __syncwarp();
       warp_mbar_wait(spare, 0, &no_abort);
     }
-  } else {  // ── softmax
+  } else if (warp < 4 + 2 * kGroupWarps) {  // ── softmax
     const int quarter = warp & 3, half = ((warp - 4) >> 2) & 1;
     const int r = 32 * quarter + lane;
     const uint32_t trow = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
     const uint32_t pair = pairs + 8 * quarter;
-    // [3] max (by block parity), sum; then [half][lane]
-    float* xq = xch + ((g * 3) * 4 + quarter) * 64 + lane;
+    // [4] max (by block parity), sum (by item parity); then [half][lane]
+    float* xq = xch + ((g * 4) * 4 + quarter) * 64 + lane;
     int meets = 0;
     auto meet = [&]() -> bool {  // what both warps wrote before is visible to both
       __syncwarp();
       if (lane == 0) mbar_arrive(pair);
       return warp_mbar_wait(pair, (meets++) & 1, abort_flag);
     };
-    const uint32_t stage = staging + static_cast<uint32_t>(warp - 4) * 32 * C::SEG;
     int bc = 0;
     bool ok = true;
     for (int m = 0; ok; ++m) {
       if (!warp_mbar_wait(ifull + 8 * (m & 1), (m >> 1) & 1, abort_flag)) break;
-      const volatile TcItem& e = ring[m & 1];
+      const volatile TcItem& e = ring[m & 3];
       if (!e.live) break;
-      const int start = e.start, n = e.n, h = e.h, q0 = e.q0, k_begin = e.k_begin, nw = e.nw, s_end = e.s_end,
-                nb = e.nb;
+      const int n = e.n, q0 = e.q0, k_begin = e.k_begin, nw = e.nw, s_end = e.s_end, nb = e.nb;
       const int nw16 = ceil16(nw), nv = nw16 + ceil16(s_end);
       const int qi = q0 + r;
       const int rows = min(p.kq, n - q0) - 32 * quarter;  // rows of this warp's quarter (32 and more: all)
@@ -773,15 +829,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             uint32_t s[32];
             tmem_ld_32x32b_x32(trow + c, s);
             tmem_wait_ld();
-            if (__all_sync(0xffffffffu, bits == 0xffffffffu)) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 2)
-                mx = fmaxf(mx, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (bits >> i & 1) mx = fmaxf(mx, __uint_as_float(s[i]));
-            }
+            for (int i = 0; i < 32; ++i)
+              if (bits >> i & 1) mx = fmaxf(mx, __uint_as_float(s[i]));
           }
           float* xm = xq + (bc & 1) * 256;
           xm[32 * half] = mx;
@@ -828,8 +878,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int i = 0; i < 32; i += 2) {
                 float2 z = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
                                       f2(w.scale_log2), f2(-ref));
-                // (a second, unmasked copy of this code is slower: it does not fit
-                // the instruction cache beside the rest)
                 if (!(bits >> i & 1)) z.x = -INFINITY;
                 if (!(bits >> (i + 1) & 1)) z.y = -INFINITY;
                 const float2 e2 = make_float2(ex2_approx(z.x), ex2_approx(z.y));
@@ -860,56 +908,83 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive(pfull);
       }
       if (!ok) break;
-      float inv = 0.f, l_row = 0.f;
-      if (active) {
-        float* xs = xq + 2 * 256;
-        xs[32 * half] = l;
-        if (!meet()) break;
-        l_row = l + xs[32 * (half ^ 1)];
-        inv = 1.f / l_row;
+      xq[(2 + (m & 1)) * 256 + 32 * half] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(lfull + 8 * (m & 1));
+    }
+  } else {  // ── output, of both slots: whichever has an item done
+    const int quarter = warp & 3;
+    const uint32_t stage = staging + static_cast<uint32_t>(quarter) * 32 * C::SEG;
+    int done[2] = {0, 0};
+    bool more[2] = {true, true};
+    while (more[0] || more[1]) {
+      int s = -1;
+      uint64_t t0 = 0;
+#pragma unroll 1
+      for (int i = 0; s < 0; ++i) {
+        const bool a = more[0] && mbar_test_wait(smem_u32(meta) + 104, done[0] & 1);
+        const bool b = more[1] && mbar_test_wait(smem_u32(meta) + kSlotBars + 104, done[1] & 1);
+        if (__all_sync(0xffffffffu, a)) s = 0;
+        else if (__all_sync(0xffffffffu, b)) s = 1;
+        else if ((i & 63) == 63) {
+          bool late = *abort_flag != 0;
+          if (t0 == 0) t0 = global_timer_ns();
+          else if (global_timer_ns() - t0 > kWaitLimitNs) *abort_flag = 1, late = true;
+          if (__any_sync(0xffffffffu, late)) break;
+        }
       }
-      if (!warp_mbar_wait(ofull, (bc - 1) & 1, abort_flag)) break;
+      if (s < 0) break;
+      const int m = s ? done[1] : done[0];
+      if (s) ++done[1]; else ++done[0];
+      if (ends[s] == m) {
+        if (s) more[1] = false; else more[0] = false;
+        continue;
+      }
+      const uint32_t sbars = smem_u32(meta) + s * kSlotBars;
+      if (!warp_mbar_wait(sbars + 112 + 8 * (m & 1), (m >> 1) & 1, abort_flag)) break;
+      const volatile TcItem& e = rings[4 * s + (m & 3)];
       tc_fence_after();
-      // this thread's D / 2 columns, up to 32 at a time
-      constexpr int kCols = D / 2 < 32 ? D / 2 : 32;
+      const int start = e.start, n = e.n, h = e.h, q0 = e.q0, nb = e.nb;
+      const int rows = min(p.kq, n - q0) - 32 * quarter;  // rows of this warp's quarter (32 and more: all)
+      const uint32_t to = s * 256u + (static_cast<uint32_t>(32 * quarter) << 16) + C::O_COL;
+      const float* xs = xch + ((s * 4 + 2 + (m & 1)) * 4 + quarter) * 64 + lane;
+      const float l_row = xs[0] + xs[32], inv = 1.f / l_row;
       T* out = static_cast<T*>(w.ctx) + (static_cast<size_t>(start + q0 + 32 * quarter) * w.heads + h) * D;
       float2 zero2 = make_float2(0.f, 0.f);  // sum of o * 0: NaN if any output is not finite
+      constexpr int kSlots = C::SEG / 16, kShift = kSlots == 4 ? 1 : 0;  // 16-byte slots of a staged row
+      constexpr int kRowsPerIns = 32 / kSlots;
+      auto slot_at = [&](int row, int q) {
+        return stage + row * C::SEG + ((q ^ ((row >> kShift) & (kSlots - 1))) << 4);
+      };
 #pragma unroll
-      for (int c = 0; c < D / 2; c += kCols) {
-        uint32_t o[kCols];
-        if (active) {
-          if constexpr (kCols == 16) tmem_ld_32x32b_x16(trow + C::O_COL + half * (D / 2) + c, o);
-          else tmem_ld_32x32b_x32(trow + C::O_COL + half * (D / 2) + c, o);
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (rows > 0) {
+          tmem_ld_32x32b_x32(to + c, o);
           tmem_wait_ld();
         }
-        if (c + kCols == D / 2) {  // the slot's TMEM may be overwritten
+        if (c + 32 == D) {  // the slot's O may be overwritten
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(sfree);
+          if (lane == 0) mbar_arrive(sbars + 56);
         }
-        if (active) {
-          constexpr int kSlots = C::SEG / 16, kShift = kSlots == 4 ? 1 : 2;  // 16-byte slots of a staged row
-          constexpr int kRowsPerIns = 32 / kSlots;
-          auto slot_at = [&](int row, int q) {
-            return stage + row * C::SEG + ((q ^ ((row >> kShift) & (kSlots - 1))) << 4);
-          };
+        if (rows > 0) {
+          if (c % (C::SEG / 2) == 0) __syncwarp();  // the staged rows before have been read
 #pragma unroll
-          for (int c1 = 0; c1 < kCols; c1 += C::SEG / 2) {  // columns staged at once
-            __syncwarp();  // the staged rows before have been read
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[4];
 #pragma unroll
-            for (int q = 0; q < kSlots; ++q) {
-              uint32_t pk[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 y = __fmul2_rn(make_float2(__uint_as_float(o[c1 + 8 * q + 2 * i]),
-                                                        __uint_as_float(o[c1 + 8 * q + 2 * i + 1])), f2(inv));
-                zero2 = __ffma2_rn(y, make_float2(0.f, 0.f), zero2);
-                pk[i] = pack16<H16>(y.x, y.y);
-              }
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot_at(lane, q)), "r"(pk[0]), "r"(pk[1]),
-                           "r"(pk[2]), "r"(pk[3])
-                           : "memory");
+            for (int i = 0; i < 4; ++i) {
+              const float2 y = __fmul2_rn(make_float2(__uint_as_float(o[8 * q + 2 * i]),
+                                                      __uint_as_float(o[8 * q + 2 * i + 1])), f2(inv));
+              zero2 = __ffma2_rn(y, make_float2(0.f, 0.f), zero2);
+              pk[i] = pack16<H16>(y.x, y.y);
             }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot_at(lane, c % (C::SEG / 2) / 8 + q)),
+                         "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3])
+                         : "memory");
+          }
+          if ((c + 32) % (C::SEG / 2) == 0) {
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < kSlots; ++i) {
@@ -920,7 +995,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                            : "r"(slot_at(row, q))
                            : "memory");
               if (row < rows)
-                *reinterpret_cast<uint4*>(out + static_cast<size_t>(row) * w.heads * D + half * (D / 2) + c + c1 + 8 * q) =
+                *reinterpret_cast<uint4*>(out + static_cast<size_t>(row) * w.heads * D + c + 32 - C::SEG / 2 + 8 * q) =
                     make_uint4(v0, v1, v2, v3);
             }
           }
@@ -932,10 +1007,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // blocks: a NaN sum has a NaN score in it, and the outputs are NaN; else a
       // value that the row does not see may be the one that is not finite.
       const bool sound = zero2.x + zero2.y == 0.f && l_row < INFINITY;
-      if (mine && !(sound && (nb > 1 || l_row > 0x1p-100f)) && (nb == 1 || l_row == l_row)) {
-        const int c0 = half * (D / 2), c1 = c0 + D / 2;
-        if (nb == 1 || hidden_not_finite<T, D>(w, start, n, h, qi, k_begin, nw, s_end, c0, c1))
-          window_row_exact<T, D>(w, start, n, h, qi, c0, c1);
+      if (lane < rows && !(sound && (nb > 1 || l_row > 0x1p-100f)) && (nb == 1 || l_row == l_row)) {
+        const int qi = q0 + 32 * quarter + lane;
+        if (nb == 1 || hidden_not_finite<T, D>(w, start, n, h, qi, e.k_begin, e.nw, e.s_end, 0, D))
+          window_row_exact<T, D>(w, start, n, h, qi, 0, D);
       }
     }
   }
@@ -1021,6 +1096,7 @@ cudaError_t launch_attention_window(const WindowArgs& a, cudaStream_t s, std::st
   p.heads = a.heads;
   p.kv_heads = a.kv_heads;
   p.rows = a.rows;
+  p.max_len = a.max_len;
   p.q_blocks = 0;
   p.left = a.left;
   p.right = a.right;

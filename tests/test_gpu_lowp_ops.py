@@ -606,6 +606,29 @@ def test_attention_window_infinite_value(dev, left, right, sinks, dt):
     window_check(got, clean, [n], 1, 1, left, right, sinks, t != torch.float32)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("cu", [[0, 300, 300, 900], [0, 5, -7, 20, 2 ** 31 - 1], [600, 20, -(2 ** 31), 40, 900]])
+def test_attention_window_offsets_that_do_not_fit(dev, cu, dt):
+    """Rows longer than max_len are cut; offsets that go back, are negative or lie behind the
+    buffer make rows of what is inside it."""
+    t, n, d, longest = DTYPES[dt], 800, 64, 250
+    qkv = torch.randn((n, 3 * d), generator=_gen(len(cu)), device=dev).to(t)
+    ctx = torch.full((n, d), 7.0, device=dev, dtype=t)
+    from jammi_b200 import _lib as L
+    offsets = torch.tensor(cu, dtype=torch.int32, device=dev)
+    L.check(L.lib().jb_op_attention_window(qkv.data_ptr(), offsets.data_ptr(), ctx.data_ptr(), {"f32": L.DT_F32, "bf16": L.DT_BF16,
+                                           "f16": L.DT_F16}[dt], len(cu) - 1, 1, 1, d, longest, n, 64, 64, 1,
+                                           torch.cuda.current_stream().cuda_stream))
+    _ops().sync()
+    rows = [(a, min(b, n, a + longest)) for a, b in zip(cu, cu[1:]) if a >= 0]
+    written = torch.zeros(n, dtype=torch.bool, device=dev)
+    for a, b in rows:
+        if b > a:
+            written[a:b] = True
+            window_check(ctx[a:b], qkv[a:b], [b - a], 1, 1, 64, 64, 1, t != torch.float32)
+    assert (ctx[~written] == 7.0).all()
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 def test_attention_window_values_of_nan_alone(dev, dt):
     """No query waits long for a long row without one finite value."""
