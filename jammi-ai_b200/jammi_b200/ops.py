@@ -112,6 +112,7 @@ _F32 = (torch.float32,)
 # The current stream's handle without building a Stream object (3 us a call).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _entry = {}
 
 
@@ -120,7 +121,7 @@ def _call(name, index, *args):
     fn = _entry.get(name)
     if fn is None:
         fn = _entry[name] = getattr(lib(), name)
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -130,7 +131,7 @@ def _call(name, index, *args):
 
 
 def _rms_args(x, gamma, residual):
-    """The device index of a valid call."""
+    """The device index and the shape of a valid call."""
     _check("x", x, None, _FLOATS)
     shape, index = x.shape, x.get_device()
     if len(shape) != 2:
@@ -138,15 +139,14 @@ def _rms_args(x, gamma, residual):
     _check("gamma", gamma, shape[1:], _F32, index)
     if residual is not None:
         _check("residual", residual, shape, (x.dtype,), index)
-    return index
+    return index, shape
 
 
 def rmsnorm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=None):
     """RMS norm of ``x`` [R, C] (+ ``residual``): ``s * rsqrt(mean(s^2) + eps) * gamma`` with
     ``s = x + residual`` in f32.  Returns y, or (y, s rounded to x's dtype) when a residual is
     given.  x f32, bf16 or f16; gamma f32 [C]."""
-    index = _rms_args(x, gamma, residual)
-    R, C = x.shape
+    index, (R, C) = _rms_args(x, gamma, residual)
     y = torch.empty_like(x)
     h = None if residual is None else torch.empty_like(x)
     if R:
@@ -159,8 +159,7 @@ def rmsnorm_quantize(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=
     """``rmsnorm`` with its output as per-row int8: (q int8 [R, C], scale f32 [R]) -- the
     activations of ``linear_s8`` -- and the rounded sum as a third value when a residual is given.
     The unrounded f32 norm is quantised; a row that is not finite has scale NaN and q 0."""
-    index = _rms_args(x, gamma, residual)
-    R, C = x.shape
+    index, (R, C) = _rms_args(x, gamma, residual)
     q = x.new_empty((R, C), dtype=torch.int8)
     scale = x.new_empty((R,), dtype=torch.float32)
     h = None if residual is None else torch.empty_like(x)
@@ -188,41 +187,45 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) 
 _U8 = (torch.uint8,)
 
 
-def _mx_scale_shape(rows, cols):
-    return ((rows + 127) // 128, (cols + 127) // 128, 512)
-
-
 def quantize_mxfp4(x: torch.Tensor):
     """MXFP4 form of ``x`` [R, C] (f32, bf16 or f16; C a multiple of 32): codes uint8 [R, C / 2],
     the even column in the low half, and scale bytes uint8 [ceil(R / 128), ceil(C / 128), 512] in
     the order ``linear_mxfp4`` reads (``jb_op_quantize_mxfp4``)."""
     _check("x", x, None, _FLOATS)
-    if x.dim() != 2 or x.shape[1] % 32 or not x.shape[1]:
+    shape = x.shape
+    if len(shape) != 2 or shape[1] % 32 or not shape[1]:
         raise ValueError("x must be [rows, cols] with cols a multiple of 32")
-    R, C = x.shape
+    R, C = shape
     q = x.new_empty((R, C // 2), dtype=torch.uint8)
-    scale = q.new_empty(_mx_scale_shape(R, C))
+    scale = q.new_empty(((R + 127) // 128, (C + 127) // 128, 512))
     if R:
         _call("jb_op_quantize_mxfp4", x.get_device(), x.data_ptr(), _DT[x.dtype], q.data_ptr(), scale.data_ptr(), R, C)
     return q, scale
 
 
 def _check_mxfp4(name, q, scale, index=None):
+    """Raises ValueError unless q and scale are MXFP4 rows on device ``index`` (None: any); their
+    device, rows and columns."""
     _check(name, q, None, _U8, index)
-    if q.dim() != 2 or q.shape[1] % 16 or not q.shape[1]:
+    shape, index = q.shape, q.get_device()
+    if len(shape) != 2 or shape[1] % 16 or not shape[1]:
         raise ValueError(f"{name} must be [rows, cols / 2] with cols a multiple of 32")
-    _check(name + "'s scale", scale, _mx_scale_shape(q.shape[0], 2 * q.shape[1]), _U8, q.get_device())
+    R, C = shape[0], 2 * shape[1]
+    tiles = ((R + 127) // 128, (C + 127) // 128, 512)
+    if (scale is None or scale.shape != tiles or scale.dtype is not torch.uint8 or not scale.is_contiguous() or
+            scale.get_device() != index):
+        _refuse(name + "'s scale", scale, tiles, _U8, index)
+    return index, R, C
 
 
 def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
     """The values [R, C] that ``quantize_mxfp4``'s codes and scales stand for, in ``dtype``."""
-    _check_mxfp4("q", q, scale)
+    index, R, C = _check_mxfp4("q", q, scale)
     if dtype not in _FLOATS:
         raise ValueError(f"{dtype} is not one of {', '.join(map(str, _FLOATS))}")
-    R, C = q.shape[0], 2 * q.shape[1]
     y = q.new_empty((R, C), dtype=dtype)
     if R:
-        _call("jb_op_dequantize_mxfp4", q.get_device(), q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype], R, C)
+        _call("jb_op_dequantize_mxfp4", index, q.data_ptr(), scale.data_ptr(), y.data_ptr(), _DT[dtype], R, C)
     return y
 
 
@@ -231,16 +234,14 @@ def linear_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w_sc
     """``epi(a @ w.T + bias)`` [M, N] of MXFP4 activations [M, K] and weights [N, K], both as
     ``quantize_mxfp4`` returns them; N a multiple of 8, ``out_dtype`` f32, bf16 or f16 (the
     residual's too), bias f32 [N]."""
-    _check_mxfp4("aq", aq, a_scale)
-    index = aq.get_device()
-    _check_mxfp4("wq", wq, w_scale, index)
-    if wq.shape[1] != aq.shape[1]:
+    index, M, K = _check_mxfp4("aq", aq, a_scale)
+    _, N, columns = _check_mxfp4("wq", wq, w_scale, index)
+    if columns != K:
         raise ValueError("aq and wq must have the same number of columns")
-    M, N, K = aq.shape[0], wq.shape[0], 2 * aq.shape[1]
     if out_dtype not in _FLOATS:
         raise ValueError(f"{out_dtype} is not one of {', '.join(map(str, _FLOATS))}")
     if bias is not None:
-        _check("bias", bias, wq.shape[:1], _F32, index)
+        _check("bias", bias, (N,), _F32, index)
     if residual is not None:
         _check("residual", residual, (M, N), (out_dtype,), index)
     c = aq.new_empty((M, N), dtype=out_dtype)
@@ -281,14 +282,15 @@ def attention_window(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, ma
     _check("cu_seqlens", cu_seqlens, None, (torch.int32,), qkv.get_device())
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError("heads must be a positive multiple of kv_heads")
-    if qkv.dim() != 2 or not qkv.shape[1] or qkv.shape[1] % (heads + 2 * kv_heads):
+    shape, offsets = qkv.shape, cu_seqlens.shape
+    if len(shape) != 2 or not shape[1] or shape[1] % (heads + 2 * kv_heads):
         raise ValueError("qkv must be [tokens, (heads + 2 * kv_heads) * head_dim]")
-    if cu_seqlens.dim() != 1 or not cu_seqlens.numel():
+    if len(offsets) != 1 or not offsets[0]:
         raise ValueError("cu_seqlens must be [batch + 1]")
-    T, d = qkv.shape[0], qkv.shape[1] // (heads + 2 * kv_heads)
+    T, d = shape[0], shape[1] // (heads + 2 * kv_heads)
     ctx = qkv.new_empty((T, heads * d))
     _call("jb_op_attention_window", qkv.get_device(), qkv.data_ptr(), cu_seqlens.data_ptr(), ctx.data_ptr(),
-          _DT[qkv.dtype], cu_seqlens.numel() - 1, heads, kv_heads, d, max_len, T, left, right, sinks)
+          _DT[qkv.dtype], offsets[0] - 1, heads, kv_heads, d, max_len, T, left, right, sinks)
     return ctx
 
 
