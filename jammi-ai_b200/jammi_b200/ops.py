@@ -106,6 +106,13 @@ def _check(name, t, shape, dtypes, index=None):
         _refuse(name, t, shape, dtypes, index)
 
 
+_INT_MAX = 2 ** 31 - 1  # ctypes would pass what lies beyond it by its low 32 bits
+
+
+def _too_large():
+    raise ValueError("sizes must be below 2^31")
+
+
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _F32 = (torch.float32,)
 
@@ -136,6 +143,8 @@ def _rms_args(x, gamma, residual):
     shape, index = x.shape, x.get_device()
     if len(shape) != 2:
         raise ValueError("x must be [rows, cols]")
+    if shape[0] > _INT_MAX or shape[1] > _INT_MAX:
+        _too_large()
     _check("gamma", gamma, shape[1:], _F32, index)
     if residual is not None:
         _check("residual", residual, shape, (x.dtype,), index)
@@ -174,6 +183,8 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) 
     _check("q", q, None, (torch.int8,))
     if q.dim() != 2:
         raise ValueError("q must be [rows, cols]")
+    if max(q.shape) > _INT_MAX:
+        _too_large()
     _check("scale", scale, q.shape[:1], _F32, q.get_device())
     if dtype not in _FLOATS:
         raise ValueError(f"{dtype} is not one of {', '.join(map(str, _FLOATS))}")
@@ -196,6 +207,8 @@ def quantize_mxfp4(x: torch.Tensor):
     if len(shape) != 2 or shape[1] % 32 or not shape[1]:
         raise ValueError("x must be [rows, cols] with cols a multiple of 32")
     R, C = shape
+    if R > _INT_MAX or C > _INT_MAX:
+        _too_large()
     q = x.new_empty((R, C // 2), dtype=torch.uint8)
     scale = q.new_empty(((R + 127) // 128, (C + 127) // 128, 512))
     if R:
@@ -211,6 +224,8 @@ def _check_mxfp4(name, q, scale, index=None):
     if len(shape) != 2 or shape[1] % 16 or not shape[1]:
         raise ValueError(f"{name} must be [rows, cols / 2] with cols a multiple of 32")
     R, C = shape[0], 2 * shape[1]
+    if R > _INT_MAX or C > _INT_MAX:
+        _too_large()
     tiles = ((R + 127) // 128, (C + 127) // 128, 512)
     if (scale is None or scale.shape != tiles or scale.dtype is not torch.uint8 or not scale.is_contiguous() or
             scale.get_device() != index):
@@ -244,6 +259,8 @@ def linear_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w_sc
         _check("bias", bias, (N,), _F32, index)
     if residual is not None:
         _check("residual", residual, (M, N), (out_dtype,), index)
+    if epilogue > _INT_MAX or epilogue < -_INT_MAX:
+        _too_large()
     c = aq.new_empty((M, N), dtype=out_dtype)
     if M:
         _call("jb_op_linear_mxfp4", index, aq.data_ptr(), a_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
@@ -288,6 +305,9 @@ def attention_window(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, ma
     if len(offsets) != 1 or not offsets[0]:
         raise ValueError("cu_seqlens must be [batch + 1]")
     T, d = shape[0], shape[1] // (heads + 2 * kv_heads)
+    if (max(T, d, offsets[0], max_len, left, right, sinks) > _INT_MAX or
+            min(max_len, left, right, sinks) < -_INT_MAX):
+        _too_large()
     ctx = qkv.new_empty((T, heads * d))
     _call("jb_op_attention_window", qkv.get_device(), qkv.data_ptr(), cu_seqlens.data_ptr(), ctx.data_ptr(),
           _DT[qkv.dtype], offsets[0] - 1, heads, kv_heads, d, max_len, T, left, right, sinks)

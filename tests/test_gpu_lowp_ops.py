@@ -500,6 +500,16 @@ def test_attention_window_many_rows(dev, batch, lo, hi, left, right, sinks, h, h
     window_check(got, qkv, lens, h, hk, left, right, sinks, t != torch.float32)
 
 
+@pytest.mark.parametrize("batch", [1, 31, 33, 767, 768, 769, 1536, 1537, 2048, 2049])
+@pytest.mark.parametrize("longest", [1, 30, 200])
+def test_attention_window_batches_around_the_offset_scan(dev, batch, longest):
+    """Row offsets are scanned 768 at a time, up to 2048 rows."""
+    lens = torch.randint(0, longest + 1, (batch,), generator=torch.Generator().manual_seed(batch + longest)).tolist()
+    lens[-1] = longest
+    qkv, got = run_window(dev, lens, 2, 1, 64, torch.bfloat16, 20, 20, 2, batch)
+    window_check(got, qkv, lens, 2, 1, 20, 20, 2, True)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 def test_attention_window_long_rows_and_large_scores(dev, dt):
     t, lens = DTYPES[dt], [5000, 17, 2049]
@@ -660,6 +670,29 @@ def test_attention_window_refusals(dev):
     with pytest.raises(JbError):
         ops.attention_window(torch.ones((4, 3 * 24), device=dev), cu, 1, 4, 1, 1)  # head_dim 24
     assert ops.attention_window(qkv[:0], cu[:1], 1, 0, 4, 4).shape == (0, 64)
+
+
+def test_sizes_beyond_32_bits_are_refused(dev):
+    """What ctypes would cut to its low 32 bits."""
+    ops = _ops()
+    qkv, cu = torch.ones((10, 3 * 64), device=dev), torch.tensor([0, 10], dtype=torch.int32, device=dev)
+    for i in range(4):
+        for beyond in (2 ** 31, 2 ** 32, 2 ** 40 + 3, -2 ** 32):
+            a = [10, 4, 4, 0]
+            a[i] = beyond
+            with pytest.raises(ValueError):
+                ops.attention_window(qkv, cu, 1, *a[:3], sinks=a[3])
+    long = torch.empty((2 ** 31 + 8, 1), dtype=torch.int8, device=dev)
+    one = torch.ones((1,), device=dev)
+    with pytest.raises(ValueError):
+        ops.rmsnorm(long.bfloat16(), one, EPS)
+    with pytest.raises(ValueError):
+        ops.dequantize_rows(long, one)
+    q, s = ops.quantize_mxfp4(torch.ones((4, 64), device=dev))
+    w, ws = ops.quantize_mxfp4(torch.ones((16, 64), device=dev))
+    with pytest.raises(ValueError):
+        ops.linear_mxfp4(q, s, w, ws, epilogue=2 ** 32)
+    assert ops.attention_window(qkv, cu, 1, 10, 2 ** 31 - 1, 2 ** 31 - 1, sinks=2 ** 31 - 1).isfinite().all()
 
 
 # ── together ────────────────────────────────────────────────────────────────
