@@ -245,7 +245,7 @@ jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamm
  * replayed graphs do not meet) and can be captured; the first
  * jb_op_linear_mxfp4 or jb_op_attention_window on a device allocates that
  * device's error flag, so make it before a capture.  Rows (M, N, batch) are
- * below 2^31 - 2^20. */
+ * below 2^31 - 2^20, columns (cols, K) at most 2^30. */
 /* RMS norm over the last dim with the residual's addition: s = x (+ residual)
  * in f32, y = s * rsqrt(mean(s^2) + eps) * gamma.  `sum` (NULL unless a
  * residual is given; NULL: not wanted) receives s rounded to dtype, the next
@@ -255,7 +255,7 @@ jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamm
  *   int8 of the unrounded y, as jb_op_quantize_rows defines it (the operands
  *   of jb_op_linear_s8).  A row whose y holds a NaN or an infinity has scale
  *   NaN and q 0.
- * dtype F32, BF16 or F16; gamma f32 [cols]; any cols >= 1 (cols that are a
+ * dtype F32, BF16 or F16; gamma f32 [cols]; any cols in 1 .. 2^30 (cols that are a
  * multiple of 16 bytes, up to 4096 16-byte vectors, with 16-byte aligned
  * buffers take the vectorised kernels).  The squares are summed in f32: rows
  * whose sum of squares passes its range come out as 0.  sum and y may replace x or residual.

@@ -556,15 +556,16 @@ jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamm
 }
 
 namespace {
-// The kernels step through rows in 32 bits: a last step past the end must not wrap.
+// The kernels step through rows, and through a row's columns, in 32 bits: a last step past the end must not wrap.
 constexpr int kMaxOpRows = INT32_MAX - (1 << 20);
+constexpr int kMaxOpCols = 1 << 30;
 }  // namespace
 
 jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma, void* sum, void* y,
                         int8_t* q, float* scale, int dtype, int rows, int cols, float eps, void* stream) {
   return guarded([&] {
-    if (rows < 0 || rows > kMaxOpRows || cols <= 0)
-      jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: rows must be in 0 .. 2^31 - 2^20 - 1 and cols > 0");
+    if (rows < 0 || rows > kMaxOpRows || cols <= 0 || cols > kMaxOpCols)
+      jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: rows must be in 0 .. 2^31 - 2^20 - 1 and cols in 1 .. 2^30");
     if (dtype != JB_DT_F32 && dtype != JB_DT_BF16 && dtype != JB_DT_F16)
       jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: dtype must be f32, bf16 or f16");
     if ((y != nullptr) == (q != nullptr) || (q != nullptr) != (scale != nullptr))
@@ -591,8 +592,8 @@ jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma,
 jb_status jb_op_dequantize_rows(const int8_t* q, const float* scale, void* y, int dtype, int rows, int cols,
                                 void* stream) {
   return guarded([&] {
-    if (rows < 0 || rows > kMaxOpRows || cols <= 0)
-      jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: rows must be in 0 .. 2^31 - 2^20 - 1 and cols > 0");
+    if (rows < 0 || rows > kMaxOpRows || cols <= 0 || cols > kMaxOpCols)
+      jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: rows must be in 0 .. 2^31 - 2^20 - 1 and cols in 1 .. 2^30");
     if (dtype != JB_DT_F32 && dtype != JB_DT_BF16 && dtype != JB_DT_F16)
       jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: dtype must be f32, bf16 or f16");
     if (rows == 0) return;
@@ -609,7 +610,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 void check_mxfp4_rows(const char* op, const void* x, int dtype, const void* q, const void* scale, int rows,
                       int cols) {
   const std::string name = op;
-  if (rows < 0 || rows > kMaxOpRows || cols <= 0 || cols % 32 || cols > (1 << 30))
+  if (rows < 0 || rows > kMaxOpRows || cols <= 0 || cols % 32 || cols > kMaxOpCols)
     jb::fail(JB_ERR_INVALID, name + ": rows must be in 0 .. 2^31 - 2^20 - 1 and cols a multiple of 32 up to 2^30");
   if (!is_float_dtype(dtype)) jb::fail(JB_ERR_INVALID, name + ": dtype must be f32, bf16 or f16");
   if (rows == 0) return;
@@ -648,7 +649,7 @@ jb_status jb_op_linear_mxfp4(const uint8_t* Aq, const uint8_t* a_scale, const ui
   return guarded([&] {
     if (!is_float_dtype(c_dtype)) jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: C must be f32, bf16 or f16");
     if (epilogue < JB_EPI_NONE || epilogue > JB_EPI_RESIDUAL) jb::fail(JB_ERR_INVALID, "unknown epilogue");
-    if (M < 0 || M > kMaxOpRows || N <= 0 || N > kMaxOpRows || N % 8 || K <= 0 || K > (1 << 30) || K % 32)
+    if (M < 0 || M > kMaxOpRows || N <= 0 || N > kMaxOpRows || N % 8 || K <= 0 || K > kMaxOpCols || K % 32)
       jb::fail(JB_ERR_INVALID,
                "jb_op_linear_mxfp4: M must be >= 0, N a positive multiple of 8 (both below 2^31 - 2^20), K a multiple "
                "of 32 up to 2^30");

@@ -71,3 +71,12 @@ def test_attention_window_refuses(kw):
              sinks=0) | kw
     refused(L.lib().jb_op_attention_window, a["qkv"], a["cu"], a["ctx"], a["dtype"], a["batch"], a["heads"], a["kv"],
             a["d"], a["max_len"], a["rows"], a["left"], a["right"], a["sinks"], None)
+
+
+@pytest.mark.parametrize("cols", [2 ** 30 + 1, 2 ** 31 - 256, 2 ** 31 - 1])
+def test_columns_that_32_bit_steps_would_pass_are_refused(cols):
+    """A row's last step past its end must not wrap to a negative column."""
+    for kw in (dict(), dict(y=None, q=P, scale=P), dict(dtype=L.DT_F32), dict(r=P, sum=P)):
+        assert "cols" in rms(cols=cols, **kw)
+    for dtype in (L.DT_F32, L.DT_BF16, L.DT_F16):
+        assert "cols" in refused(L.lib().jb_op_dequantize_rows, P, P, P, dtype, 1, cols, None)
