@@ -257,8 +257,10 @@ jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamm
  *   NaN and q 0.
  * dtype F32, BF16 or F16; gamma f32 [cols]; any cols in 1 .. 2^30 (cols that are a
  * multiple of 16 bytes, up to 4096 16-byte vectors, with 16-byte aligned
- * buffers take the vectorised kernels).  The squares are summed in f32: rows
- * whose sum of squares passes its range come out as 0.  sum and y may replace x or residual.
+ * buffers take the vectorised kernels).  The squares are summed in f32; a row
+ * whose squares leave its range (|s| near 1e19 and up, or eps below 1e-27 and
+ * |s| as small) is summed again scaled by a power of two.  A row of zeros with
+ * eps 0 is NaN.  sum and y may replace x or residual.
  * No counterpart in the reference (its encoders use LayerNorm). */
 jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma, void* sum,
                         void* y, int8_t* q, float* scale, int dtype, int rows, int cols,

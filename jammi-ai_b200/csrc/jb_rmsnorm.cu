@@ -91,6 +91,21 @@ template <> struct Row<float> {
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 constexpr unsigned kInfBits = 0x7f800000u;
 
+// mean(s^2) + eps as summed, unless the squares left f32's range (infinite, or
+// so small that they lost bits): then a row's sum is taken again of s * c.  The
+// test costs ordinary rows nothing up to 1024 columns (36870 x 768 bf16 41.3 us
+// with and without it), 1% at 4096 and 4 to 6% in the wider kernels, where it
+// keeps the next pass's loads behind the statistics (3000 x 20000 125 -> 130.5
+// us, int8 of 9001 x 4095 97 -> 104 us).
+__device__ __forceinline__ bool in_range(float var) { return var >= 0x1p-90f && var < INFINITY; }
+// c = 2^-floor(log2(max(|s| of the row, sqrt(eps)))): s * c and eps * c^2 are
+// below 4.  0: the row holds a NaN or an infinity, whose statistics stand.
+__device__ __forceinline__ float range_scale(unsigned top, float eps) {
+  if (top >= kInfBits) return 0.f;
+  const int field = static_cast<int>(max(top, __float_as_uint(sqrtf(eps))) >> 23);
+  return __uint_as_float(static_cast<uint32_t>(max(254 - field, 1)) << 23);
+}
+
 // The row's quantiser from the bits of its largest |y|: q = rint(y * up * inv).
 // `up` is 1 except in rows so small that 127 / a would overflow.  A row with a
 // NaN or an infinity has scale NaN and q 0.
@@ -185,7 +200,44 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) rmsnorm_kernel(RmsArgs 
 #pragma unroll
       for (int w = 0; w < W; ++w) total += red[w];
     }
-    const float rstd = 1.0f / sqrtf(total / static_cast<float>(a.cols) + a.eps);
+    float var = total / static_cast<float>(a.cols) + a.eps;
+    if (!in_range(var)) {  // uniform over the row
+      unsigned big = 0;
+#pragma unroll
+      for (int i = 0; i < MAXV; ++i)
+        if (at + i * kLanes < nvec)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) big = max(big, abs_bits(v[i * VN + e]));
+      big = __reduce_max_sync(0xffffffffu, big);
+      if constexpr (W > 1) {
+        if (lane == 0) red[W + warp] = __uint_as_float(big);
+        __syncthreads();  // and the sums of `red`'s first half have been read
+#pragma unroll
+        for (int w = 0; w < W; ++w) big = max(big, __float_as_uint(red[W + w]));
+      }
+      const float c = range_scale(big, a.eps);
+      if (c != 0.f) {
+        float again = 0.f;
+#pragma unroll
+        for (int i = 0; i < MAXV; ++i)
+          if (at + i * kLanes < nvec)
+#pragma unroll
+            for (int e = 0; e < VN; ++e) {
+              v[i * VN + e] *= c;
+              again = fmaf(v[i * VN + e], v[i * VN + e], again);
+            }
+        again = warp_sum(again);
+        if constexpr (W > 1) {
+          if (lane == 0) red[warp] = again;
+          __syncthreads();
+          again = 0.f;
+#pragma unroll
+          for (int w = 0; w < W; ++w) again += red[w];
+        }
+        var = again / static_cast<float>(a.cols) + a.eps * c * c;
+      }
+    }
+    const float rstd = 1.0f / sqrtf(var);
     unsigned top = 0;
 #pragma unroll
     for (int i = 0; i < MAXV; ++i) {
@@ -271,7 +323,23 @@ __global__ void __launch_bounds__(256) rmsnorm_ragged_kernel(RmsArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
-    const float rstd = 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(a.cols) + a.eps);
+    float var = warp_sum(ss) / static_cast<float>(a.cols) + a.eps;
+    if (!in_range(var)) {  // uniform over the row
+      unsigned big = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) big = max(big, abs_bits(v[i]));
+      const float c = range_scale(__reduce_max_sync(0xffffffffu, big), a.eps);
+      if (c != 0.f) {
+        ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          v[i] *= c;
+          ss = fmaf(v[i], v[i], ss);
+        }
+        var = warp_sum(ss) / static_cast<float>(a.cols) + a.eps * c * c;
+      }
+    }
+    const float rstd = 1.0f / sqrtf(var);
     unsigned top = 0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -298,7 +366,7 @@ __global__ void __launch_bounds__(256) rmsnorm_ragged_kernel(RmsArgs a) {
 // Wider rows of any width and alignment: a CTA per row, each element read
 // again (mostly out of L1) in every pass and every output written in the last
 // one (so outputs may replace inputs element for element).  9001 x 4095 bf16
-// with residual 90 us, int8 101 us; with the row in registers 96 to 113 us
+// with residual 90 us, int8 104 us; with the row in registers 96 to 113 us
 // (fewer loads in flight).
 template <typename T>
 __global__ void __launch_bounds__(256) rmsnorm_scalar_kernel(RmsArgs a) {
@@ -310,21 +378,40 @@ __global__ void __launch_bounds__(256) rmsnorm_scalar_kernel(RmsArgs a) {
     const T* x = static_cast<const T*>(a.x) + off;
     const T* r = a.resid ? static_cast<const T*>(a.resid) + off : nullptr;
     auto s_at = [&](int c) { return r ? to_f(x[c]) + to_f(r[c]) : to_f(x[c]); };
-    float ss = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += 256) {
-      const float s = s_at(c);
-      ss = fmaf(s, s, ss);
+    float scale = 1.f;  // of s in the statistics and y, see in_range
+    auto mean_square = [&] {
+      float ss = 0.f;
+      for (int c = threadIdx.x; c < a.cols; c += 256) {
+        const float s = s_at(c) * scale;
+        ss = fmaf(s, s, ss);
+      }
+      ss = warp_sum(ss);
+      if (lane == 0) red[warp] = ss;
+      __syncthreads();
+      float total = 0.f;
+      for (int w = 0; w < 8; ++w) total += red[w];
+      return total / static_cast<float>(a.cols);
+    };
+    float var = mean_square() + a.eps;
+    if (!in_range(var)) {  // uniform over the row
+      unsigned big = 0;
+      for (int c = threadIdx.x; c < a.cols; c += 256) big = max(big, abs_bits(s_at(c)));
+      big = __reduce_max_sync(0xffffffffu, big);
+      if (lane == 0) redm[warp] = big;
+      __syncthreads();  // and `red` has been read
+      for (int w = 0; w < 8; ++w) big = max(big, redm[w]);
+      const float c = range_scale(big, a.eps);
+      if (c != 0.f) {
+        scale = c;
+        var = mean_square() + a.eps * c * c;
+      }
+      __syncthreads();  // redm has been read
     }
-    ss = warp_sum(ss);
-    if (lane == 0) red[warp] = ss;
-    __syncthreads();
-    float total = 0.f;
-    for (int w = 0; w < 8; ++w) total += red[w];
-    const float rstd = 1.0f / sqrtf(total / static_cast<float>(a.cols) + a.eps);
+    const float rstd = 1.0f / sqrtf(var);
     RowQuant rq{1.f, 0.f, 0.f};
     if (a.q) {
       unsigned top = 0;
-      for (int c = threadIdx.x; c < a.cols; c += 256) top = max(top, abs_bits(s_at(c) * rstd * __ldg(a.gamma + c)));
+      for (int c = threadIdx.x; c < a.cols; c += 256) top = max(top, abs_bits(s_at(c) * scale * rstd * __ldg(a.gamma + c)));
       top = __reduce_max_sync(0xffffffffu, top);
       if (lane == 0) redm[warp] = top;
       __syncthreads();
@@ -334,7 +421,7 @@ __global__ void __launch_bounds__(256) rmsnorm_scalar_kernel(RmsArgs a) {
     }
     for (int c = threadIdx.x; c < a.cols; c += 256) {
       const float s = s_at(c);
-      const float y = s * rstd * __ldg(a.gamma + c);
+      const float y = s * scale * rstd * __ldg(a.gamma + c);
       if (a.sum) static_cast<T*>(a.sum)[off + c] = from_f<T>(s);
       if (a.q)
         a.q[off + c] = static_cast<int8_t>(rint_byte(rq.up == 0.f ? 0.f : y * rq.up, rq.inv) & 0xffu);

@@ -127,6 +127,51 @@ def test_rmsnorm_quantize_special_rows(dev, cols):
     assert (y[0] == 0).all() and y[1].isnan().all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("res", [False, True])
+@pytest.mark.parametrize("cols", [8, 200, 201, 768, 771, 1024, 1536, 4096, 4100, 16384, 20001, 32768, 40000])
+def test_rmsnorm_of_rows_whose_squares_leave_f32(dev, cols, res, dt):
+    """Magnitudes whose squares overflow, underflow or lose bits, with eps of the same size or 0;
+    ordinary rows between them keep their values."""
+    t, g, ops = DTYPES[dt], _gen(cols + res), _ops()
+    size = torch.tensor([1.0, 1e25, 1.0, 3e37, 1e18, 2e19, 1e-25, 1.0, 1e-38, 1e-19, 1e-22], device=dev)
+    x = torch.randn((size.numel(), cols), generator=g, device=dev).clamp(-4, 4)
+    x[:, 0] = 1.0  # no row is 0 throughout
+    x = (x * size[:, None]).to(t)
+    r = (torch.randn((size.numel(), cols), generator=g, device=dev).clamp(-4, 4) * size[:, None]).to(t) if res else None
+    gamma = 1 + 0.2 * torch.rand((cols,), generator=g, device=dev)
+    u, rel = torch.finfo(t).eps / 2, rms_f32_error(sum_depth(cols))
+    s = x.double() + (r.double() if res else 0)
+    assert s.abs().max() < 3.4e38
+    for eps in (0.0, 1e-6, 1e-37, 1e-43):
+        ref = s / torch.sqrt(s.square().mean(1, keepdim=True) + torch.tensor(eps).double().item()) * gamma.double()
+        y = ops.rmsnorm(x, gamma, eps, residual=r)
+        y = (y[0] if res else y).double()
+        # a result below f32's normal range is off by units of its last place
+        off = ((y - ref).abs() - (rel + u) * ref.abs() * (1 + u) - 2.0 ** -130).amax(1)
+        assert (off <= 0).all(), (eps, off)
+        q, scale = ops.rmsnorm_quantize(x, gamma, eps, residual=r)[:2]
+        amax = ref.abs().amax(1)
+        assert ((scale.double() - amax / 127).abs() <= (rel + 2.0 ** -23) * amax / 127 + 2.0 ** -148).all(), eps
+        big = amax > 1e-30  # (scale itself keeps its bits)
+        code = (q.double() - ref * (127 / amax)[:, None])[big].abs()
+        assert code.max() <= 0.5 + 127 * (2 * rel + 2.0 ** -22), (eps, code.max())
+
+
+def test_rmsnorm_of_zeros_without_eps(dev):
+    """0 / 0: NaN, as the formula has it; with a NaN or an infinity in the row too."""
+    for cols in (64, 771, 4096, 5001):
+        x = torch.zeros((4, cols), device=dev)
+        x[1, 3], x[2, 3], x[3, 3] = math.nan, math.inf, 2.0
+        gamma = torch.ones(cols, device=dev)
+        y = _ops().rmsnorm(x, gamma, 0.0)
+        assert y[0].isnan().all() and y[1].isnan().all()
+        assert y[2, 3].isnan() and (y[2, :3] == 0).all() and (y[2, 4:] == 0).all()
+        assert y[3].isfinite().all()
+        q, scale = _ops().rmsnorm_quantize(x, gamma, 0.0)
+        assert scale[:3].isnan().all() and (q[:3] == 0).all() and q[3, 3] == 127
+
+
 @pytest.mark.parametrize("cols", [768, 2048, 770])
 def test_rmsnorm_in_place(dev, cols):
     """sum may replace x or the residual, y may replace the other."""
