@@ -324,8 +324,11 @@ jb_status jb_op_attention_rows(const void* qkv, const int* cu_seqlens, void* ctx
  * right: 0 .. 2^31 - 1 (anything >= the row's length: unbounded).  dtype F32,
  * BF16 or F16; head_dim 8, 16, 32, 64 or 128; heads a multiple of kv_heads;
  * max_len bounds every row's length (of a longer row the first max_len tokens
- * are a row), rows >= cu_seqlens[batch]; qkv and ctx 16-byte aligned.  No counterpart in the reference (its ModernBERT layers
- * attend to the whole row, crates/jammi-encoders/src/modernbert.rs). */
+ * are a row, and ctx keeps what it held for the others); it may be loose (F32,
+ * and head_dim 8 or 16: batch * heads * ceil(max_len / 32) below 2^31).  rows
+ * >= cu_seqlens[batch]; qkv and ctx 16-byte aligned.  No counterpart in the
+ * reference (its ModernBERT layers attend to the whole row,
+ * crates/jammi-encoders/src/modernbert.rs). */
 jb_status jb_op_attention_window(const void* qkv, const int* cu_seqlens, void* ctx, int dtype,
                                  int batch, int heads, int kv_heads, int head_dim, int max_len,
                                  int rows, int left, int right, int sinks, void* stream);

@@ -290,9 +290,10 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 // if a hidden value is the cause, so that no visible one makes a long row slow).
 //
 // Items are numbered over the query blocks that exist (a prefix sum of the
-// rows' blocks in shared memory, for batches of up to kPrefixRows) and dealt
-// to the slots in turn; no counter in global memory, so calls and replayed
-// graphs share nothing.
+// rows' blocks in shared memory; beyond kPrefixRows rows an entry stands for a
+// group of them, and an item's row is found by a walk through its group) and
+// dealt to the slots in turn; no counter in global memory, so calls and
+// replayed graphs share nothing.
 //
 // Measured, bf16 unless said, window 64 + 64 (out of cache):
 //   256 rows of 32 to 256 tokens, 12 heads of 64, 1 sink   67 us  3.3 TB/s
@@ -347,8 +348,17 @@ struct TcItem {
 struct TcParams {
   WinParams w;
   int batch;
-  int kq;    // queries per item
+  int group;  // rows of an entry of the table of query blocks
+  int kq;     // queries per item
   int* err;
+};
+
+// A row's tokens and query blocks.
+struct TcRow {
+  int start, n, blocks;
+  __device__ __forceinline__ TcRow(const TcParams& p, int b) : start(p.w.cu[b]), n(row_tokens(p.w, b, start)), blocks(0) {
+    if (n > 0) blocks = (n + p.kq - 1) / p.kq;
+  }
 };
 
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -484,7 +494,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t staging = base + 2 * C::SLOT_BYTES;
   float* xch = reinterpret_cast<float*>(smem_raw + (staging + C::STAGE_BYTES - raw));
-  int* prefix = reinterpret_cast<int*>(xch) + C::XCH_BYTES / 4;  // [batch + 1] query blocks before each row
+  unsigned* prefix = reinterpret_cast<unsigned*>(xch) + C::XCH_BYTES / 4;  // [entries + 1] query blocks before each group of rows
   uint8_t* meta = reinterpret_cast<uint8_t*>(prefix + kPrefixRows + 4);
   const int g = warp < 4 ? warp & 1 : (warp - 4) / kGroupWarps & 1;  // this warp's slot
   const uint32_t sQ = base + g * C::SLOT_BYTES, sK = sQ + C::Q_BYTES, sV = sK + C::KV_BYTES;
@@ -508,41 +518,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   volatile TcItem* ring = rings + 4 * g;
   static_assert(2 * kSlotBars + 16 + 8 * sizeof(TcItem) <= C::META_BYTES, "meta layout");
   const WinParams& w = p.w;
-  const bool counted = p.batch <= kPrefixRows;
+  const int entries = (p.batch + p.group - 1) / p.group;
 
   if (warp == 1 && lane == 0) {
     prefetch_tensormap(&tm64);
     prefetch_tensormap(&tm16);
   }
-  // Query blocks before each row: a scan by all warps, kTcThreads rows a round.
-  int incl[kRounds], mine_blocks[kRounds];
-  if (counted) {
+  // Query blocks before each group of rows: a scan by all warps, kTcThreads entries
+  // a round.  (Unsigned: overlapping rows could have more than 32 bits count.)
+  unsigned incl[kRounds], mine_blocks[kRounds];
 #pragma unroll
-    for (int i = 0; i < kRounds; ++i) {
-      const int b = i * kTcThreads + threadIdx.x;
-      int blocks = 0;
-      if (b < p.batch) {
-        const int n = row_tokens(w, b, w.cu[b]);
-        if (n > 0) blocks = (n + p.kq - 1) / p.kq;
-      }
-      mine_blocks[i] = blocks;
+  for (int i = 0; i < kRounds; ++i) {
+    const int at = i * kTcThreads + threadIdx.x;
+    unsigned blocks = 0;
+    if (at < entries)
+      for (int b = at * p.group, stop = min(p.batch, b + p.group); b < stop; ++b) blocks += TcRow(p, b).blocks;
+    mine_blocks[i] = blocks;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, blocks, o);
-        if (lane >= o) blocks += up;
-      }
-      incl[i] = blocks;
-      if (lane == 31) reinterpret_cast<int*>(xch)[i * kTcWarps + warp] = blocks;
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, blocks, o);
+      if (lane >= o) blocks += up;
     }
-    __syncthreads();
-    int before = 0, at = 0;  // blocks of the warps before this one
+    incl[i] = blocks;
+    if (lane == 31) reinterpret_cast<unsigned*>(xch)[i * kTcWarps + warp] = blocks;
+  }
+  __syncthreads();
+  {
+    unsigned before = 0;  // blocks of the warps before this one
+    int w0 = 0;
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
-      if (i * kTcThreads < p.batch || i == 0) {
-        for (; at < i * kTcWarps + warp; ++at) before += reinterpret_cast<int*>(xch)[at];
-        const int b = i * kTcThreads + threadIdx.x;
-        if (b < p.batch) prefix[b] = before + incl[i] - mine_blocks[i];
-        if (b == p.batch - 1) prefix[p.batch] = before + incl[i];
+      if (i * kTcThreads < entries || i == 0) {
+        for (; w0 < i * kTcWarps + warp; ++w0) before += reinterpret_cast<unsigned*>(xch)[w0];
+        const int at = i * kTcThreads + threadIdx.x;
+        if (at < entries) prefix[at] = before + incl[i] - mine_blocks[i];
+        if (at == entries - 1) prefix[entries] = before + incl[i];
       }
     }
   }
@@ -573,9 +583,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // each group of instructions, so that the operands stay in uniform
   // registers (see jb_mxfp4_gemm.cu).
   if (warp < 2) {  // ── TMA
-    const long long items =
-        counted ? min(static_cast<long long>(prefix[p.batch]) * w.heads, static_cast<long long>(INT32_MAX))
-                : static_cast<long long>(p.batch) * w.q_blocks * w.heads;
+    const long long items = min(static_cast<long long>(prefix[entries]) * w.heads, static_cast<long long>(INT32_MAX));
     const long long stride = 2ll * gridDim.x;
     int bc = 0, m = 0;  // blocks loaded, items published
     bool ok = true;
@@ -584,28 +592,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const long long f = f0 + lane * stride;
       int start = 0, n = 0, h = 0, q0 = 0;  // this lane's candidate
       if (f < items) {
-        int b, qb;
-        if (counted) {
-          const int bq = static_cast<int>(f) / w.heads;
-          h = static_cast<int>(f) - bq * w.heads;
-          int lo = 0, hi = p.batch;  // prefix[lo] <= bq < prefix[hi]
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (prefix[mid] <= bq) lo = mid;
-            else hi = mid;
-          }
-          b = lo;
-          qb = bq - prefix[lo];
-        } else {
-          const long long bq = f / w.heads;
-          h = static_cast<int>(f - bq * w.heads);
-          b = static_cast<int>(bq / w.q_blocks);
-          qb = static_cast<int>(bq % w.q_blocks);
+        unsigned qb = static_cast<unsigned>(f) / w.heads;
+        h = static_cast<int>(f) - static_cast<int>(qb) * w.heads;
+        int lo = 0, hi = entries;  // prefix[lo] <= qb < prefix[hi]
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (prefix[mid] <= qb) lo = mid;
+          else hi = mid;
         }
-        q0 = qb * p.kq;
-        start = w.cu[b];
-        // (rows that overlap could have more blocks than 32 bits count)
-        n = qb >= 0 && qb < w.q_blocks ? row_tokens(w, b, start) : 0;
+        qb -= prefix[lo];
+        int b = lo * p.group;
+        const int stop = min(p.batch, b + p.group);
+        TcRow row(p, b);
+        while (qb >= static_cast<unsigned>(row.blocks) && ++b < stop) {
+          qb -= row.blocks;
+          row = TcRow(p, b);
+        }
+        if (qb < static_cast<unsigned>(row.blocks)) {  // always, unless the count above wrapped
+          q0 = static_cast<int>(qb) * p.kq;
+          start = row.start;
+          n = row.n;
+        }
       }
       unsigned todo = __ballot_sync(0xffffffffu, f < items && q0 < n);
       while (todo && ok) {
@@ -1078,6 +1085,7 @@ cudaError_t launch_tc(const WindowArgs& a, WinParams w, cudaStream_t s, std::str
   w.q_blocks = (a.max_len + p.kq - 1) / p.kq;
   p.w = w;
   p.batch = a.batch;
+  p.group = (a.batch + kPrefixRows - 1) / kPrefixRows;
   p.err = a.err;
   const long long most = static_cast<long long>(a.batch) * w.q_blocks * a.heads;
   const int grid = static_cast<int>(std::min<long long>(num_sms(dev), most));

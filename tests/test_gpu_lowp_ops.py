@@ -555,6 +555,30 @@ def test_attention_window_batches_around_the_offset_scan(dev, batch, longest):
     window_check(got, qkv, lens, 2, 1, 20, 20, 2, True)
 
 
+@pytest.mark.parametrize("batch,longest", [(2049, 3), (4095, 9), (4097, 0), (30000, 5), (300000, 1), (6145, 200), (2000000, 3)])
+@pytest.mark.parametrize("left,right,sinks", [(2, 1, 1), (10 ** 9, 10 ** 9, 0)])
+def test_attention_window_batches_of_any_size(dev, batch, longest, left, right, sinks):
+    """More rows than the table of offsets, a max_len that says nothing, empty rows among them and
+    one long one: the work follows the tokens, not batch * max_len."""
+    lens = torch.randint(0, longest + 1, (batch,), generator=torch.Generator().manual_seed(batch))
+    lens[batch // 2], lens[0], lens[-1] = 1000, 0, 0
+    T, d, t = int(lens.sum()), 64, torch.bfloat16
+    qkv = torch.randn((T + 2, 3 * d), generator=_gen(batch), device=dev).to(t)
+    cu = torch.zeros(batch + 1, dtype=torch.int32)
+    cu[1:] = lens.cumsum(0)
+    got = _ops().attention_window(qkv, cu.to(dev), 1, 2 ** 31 - 1, left, right, sinks=sinks)
+    _ops().sync()
+    kept = lens[lens > 0]
+    some = torch.randperm(kept.numel(), generator=torch.Generator().manual_seed(1))[:400]
+    at = torch.cat([torch.zeros(1, dtype=torch.long), kept.cumsum(0)])
+    picks = sorted(set(some.tolist()) | {0, kept.numel() - 1, int(kept.argmax())})
+    index = torch.cat([torch.arange(at[i], at[i + 1]) for i in picks]).to(dev)
+    window_check(got[index], qkv[index], [int(kept[i]) for i in picks], 1, 1, left, right, sinks, True)
+    if longest == 1:  # rows of one token give their value
+        one = torch.repeat_interleave(kept == 1, kept).to(dev)
+        assert torch.equal(got[:T][one], qkv[:T][one][:, 2 * d:])
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 def test_attention_window_long_rows_and_large_scores(dev, dt):
     t, lens = DTYPES[dt], [5000, 17, 2049]
