@@ -285,9 +285,8 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 //
 // A masked value contributes 0 * v, which is not 0 when v is not finite.  V
 // rows behind the item's last key are zeroed in shared memory; for the rest
-// outputs that are not finite are computed again, by their thread, over the
-// visible keys only (window_row_exact; a row of an item of several blocks only
-// if a hidden value is the cause, so that no visible one makes a long row slow).
+// outputs that are not finite are computed again, behind the CTA's last item,
+// over the visible keys only (window_rows_exact).
 //
 // Items are numbered over the query blocks that exist (a prefix sum of the
 // rows' blocks in shared memory; beyond kPrefixRows rows an entry stands for a
@@ -342,13 +341,11 @@ struct TcCfg {
   static_assert(SMEM <= 232448, "shared memory");
 };
 
-struct TcItem {
-  int live, start, n, h, q0, k_begin, nw, s_end, nb;
-};
+__host__ __device__ constexpr int ceil16(int v) { return (v + 15) & ~15; }
 struct TcParams {
   WinParams w;
   int batch;
-  int group;  // rows of an entry of the table of query blocks
+  int entries, group;  // of the table of query blocks, and the rows of each
   int kq;     // queries per item
   int* err;
 };
@@ -359,6 +356,53 @@ struct TcRow {
   __device__ __forceinline__ TcRow(const TcParams& p, int b) : start(p.w.cu[b]), n(row_tokens(p.w, b, start)), blocks(0) {
     if (n > 0) blocks = (n + p.kq - 1) / p.kq;
   }
+};
+// Item f: its row, head and first query (n = 0: there is none).
+struct TcPlace {
+  int start = 0, n = 0, h = 0, q0 = 0;
+  __device__ __forceinline__ TcPlace() {}
+  __device__ __forceinline__ TcPlace(const TcParams& p, const unsigned* prefix, int f) {
+    unsigned qb = static_cast<unsigned>(f) / p.w.heads;
+    h = f - static_cast<int>(qb) * p.w.heads;
+    int lo = 0, hi = p.entries;  // prefix[lo] <= qb < prefix[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= qb) lo = mid;
+      else hi = mid;
+    }
+    qb -= prefix[lo];
+    int b = lo * p.group;
+    const int stop = min(p.batch, b + p.group);
+    TcRow row(p, b);
+    while (qb >= static_cast<unsigned>(row.blocks) && ++b < stop) {
+      qb -= row.blocks;
+      row = TcRow(p, b);
+    }
+    if (qb < static_cast<unsigned>(row.blocks)) {  // always, unless the count of blocks wrapped
+      q0 = static_cast<int>(qb) * p.kq;
+      start = row.start;
+      n = row.n;
+    }
+  }
+};
+// Its keys: the window's [k_begin, k_begin + nw), the sinks [0, s_end) behind it, in nb blocks.
+struct TcKeys {
+  int k_begin, nw, s_end, nb;
+  __device__ __forceinline__ TcKeys(const WinParams& w, int kq, int n, int q0, int block_keys) {
+    const int q_last = min(n, q0 + kq) - 1;
+    const int k_end = q_last + min(w.right, n - 1 - q_last) + 1;
+    k_begin = q0 - min(w.left, q0);
+    // no gap between sinks and window, or a row short enough to read whole
+    if (w.sinks >= k_begin || (w.sinks > 0 && k_end <= block_keys)) k_begin = 0;
+    s_end = min(w.sinks, k_begin);
+    nw = k_end - k_begin;
+    const int nv = ceil16(nw) + ceil16(s_end);
+    nb = nv <= block_keys ? 1 : (nv + 127) / 128;
+  }
+};
+// A published item.
+struct TcItem {
+  int live, start, n, h, q0, k_begin, nw, s_end, nb;
 };
 
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -390,7 +434,6 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
-__host__ __device__ constexpr int ceil16(int v) { return (v + 15) & ~15; }
 // bits [0, c) of 32, c clamped to 0 .. 32
 __device__ __forceinline__ uint32_t low_bits(int c) {
   return c <= 0 ? 0u : c >= 32 ? 0xffffffffu : (1u << c) - 1u;
@@ -417,58 +460,114 @@ __device__ __forceinline__ int ref_col(int nw, int nw16, int nv, int s_end, int 
   return nv > 192 ? 144 : s_end > 0 ? nw16 : 0;  // nw <= 80, nv > 192: columns 80 to 176 are sinks
 }
 
-// Output columns [c0, c1) of one query row over its visible keys only, in f32
-// from global memory.
+// The items of a CTA's slot, [it.x, it.y], hold outputs that are not finite: a
+// masked value contributed 0 * v, the softmax reference was far from the row's
+// scores (those rows were set to NaN), or they are so.  All warps of the CTA
+// take the rows in turn, behind its last item, so that nothing waits for them.
+// The columns of a row that are not finite are computed again from global
+// memory, in f32, over the visible keys only: a key per lane for 32 scores at
+// once, then lane c the columns c, c + 32, .. of their values.  In a row of
+// several blocks only a NaN can be wrong, and only if one of its item's hidden
+// values is the cause or, in f16, a visible infinity whose weight was rounded
+// to 0; and a row ends early where every column it needs is NaN, so that long
+// rows of visible values that are not finite cost little.
+// Causal row of 8192 tokens, 16 heads of 64, one column infinite: 38 ms (0.41 ms
+// without it).
 template <typename T, int D>
-__device__ __noinline__ void window_row_exact(const WinParams& p, int start, int n, int h, int qi, int c0, int c1) {
+__device__ __forceinline__ void window_rows_exact(const TcParams& tp, const unsigned* prefix, int slot, int2 its) {
+  const WinParams& p = tp.w;
+  constexpr int CL = D / 32;  // columns of a lane
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ld = (p.heads + 2 * p.kv_heads) * D;
-  const T* row = static_cast<const T*>(p.qkv) + static_cast<size_t>(start) * ld;
-  const T* q = row + static_cast<size_t>(qi) * ld + h * D;
-  const T* k = row + (p.heads + h / (p.heads / p.kv_heads)) * D;
-  const T* v = k + p.kv_heads * D;
-  T* out = static_cast<T*>(p.ctx) + (static_cast<size_t>(start + qi) * p.heads + h) * D;
-  const int lo = qi - min(p.left, qi), hi = qi + min(p.right, n - 1 - qi);
-  const int behind = min(p.sinks, lo);  // sinks in front of the window
-  for (int c = c0; c < c1; c += 16) {   // 16 output columns a pass
-    float o[16] = {}, l = 0.f, m = -INFINITY;
-    bool lost = false;  // every output is NaN and stays so
-    for (int j = behind > 0 ? 0 : lo; j <= hi && !lost; j = j + 1 == behind ? lo : j + 1) {
-      float s = 0.f;
-      for (int d = 0; d < D; ++d) s = fmaf(to_f(q[d]), to_f(k[static_cast<size_t>(j) * ld + d]), s);
-      s *= p.scale_log2;
-      if (s == -INFINITY) continue;  // weighs nothing, not even 0 * NaN
-      const float top = fmaxf(m, s), corr = exp2f(m - top), e = exp2f(s - top);
-      m = top;
-      l = l * corr + e;
-      lost = true;
-      for (int d = 0; d < 16; ++d) {
-        // (o is 0 until the first key: the scale from -infinity is 0)
-        o[d] = fmaf(e, to_f(v[static_cast<size_t>(j) * ld + c + d]), o[d] * corr);
-        lost &= o[d] != o[d];
-      }
+  for (long long at = its.x * 128ll + warp; at < (its.y + 1) * 128ll; at += kTcWarps) {
+    const TcPlace it(tp, prefix, static_cast<int>(slot * gridDim.x + blockIdx.x + (at >> 7) * 2 * gridDim.x));
+    const int qi = it.q0 + static_cast<int>(at & 127), n = it.n, start = it.start;
+    if ((at & 127) >= tp.kq || qi >= n) continue;
+    const T* row = static_cast<const T*>(p.qkv) + static_cast<size_t>(start) * ld;
+    const T* q = row + static_cast<size_t>(qi) * ld + it.h * D;
+    const T* k = row + (p.heads + it.h / (p.heads / p.kv_heads)) * D;
+    const T* v = k + p.kv_heads * D + lane;
+    T* out = static_cast<T*>(p.ctx) + (static_cast<size_t>(start + qi) * p.heads + it.h) * D + lane;
+    const TcKeys keys_of(p, tp.kq, n, it.q0, TcCfg<D>::KEYS);
+    bool need[CL], any = false;
+#pragma unroll
+    for (int i = 0; i < CL; ++i) {
+      const float y = to_f(out[32 * i]);
+      any |= need[i] = y != y || (keys_of.nb == 1 && fabsf(y) == INFINITY);
     }
-    for (int d = 0; d < 16; ++d) out[c + d] = from_f<T>(o[d] / l);
+    if (!__any_sync(0xffffffffu, any)) continue;
+    const int lo = qi - min(p.left, qi), hi = qi + min(p.right, n - 1 - qi);
+    const int behind = min(p.sinks, lo);  // sinks in front of the window
+    const int keys = behind + hi - lo + 1;
+    if (keys_of.nb > 1) {  // the item's hidden keys: on both sides of the row's window, and those that pad the sinks
+      float zero[CL] = {};
+      auto add = [&](int j, int stop) {
+        for (; j < stop; ++j)
+#pragma unroll
+          for (int i = 0; i < CL; ++i) zero[i] = fmaf(to_f(v[static_cast<size_t>(j) * ld + 32 * i]), 0.f, zero[i]);
+      };
+      add(max(keys_of.k_begin, min(p.sinks, lo)), lo);
+      add(hi + 1, keys_of.k_begin + keys_of.nw);
+      add(keys_of.s_end, min(ceil16(keys_of.s_end), p.rows - start));
+      bool cause = false;
+#pragma unroll
+      for (int i = 0; i < CL; ++i) cause |= need[i] && zero[i] != 0.f;
+      cause = __any_sync(0xffffffffu, cause);
+      if constexpr (sizeof(T) == 2 && !std::is_same<T, bf16>::value) {
+        for (int t0 = 0; t0 < keys && !cause; t0 += 32) {
+#pragma unroll 8
+          for (int t = t0; t < min(t0 + 32, keys); ++t) {
+            const T* vj = v + static_cast<size_t>(t < behind ? t : lo + (t - behind)) * ld;
+#pragma unroll
+            for (int i = 0; i < CL; ++i) cause |= need[i] && fabsf(to_f(vj[32 * i])) == INFINITY;
+          }
+          cause = __any_sync(0xffffffffu, cause);
+        }
+      }
+      if (!cause) continue;
+    }
+    float o[CL] = {}, l = 0.f, m = -INFINITY;
+    bool lost = false;  // every column that is needed is NaN and stays so
+    for (int t0 = 0; t0 < keys && !lost; t0 += 32) {
+      const int t = min(t0 + lane, keys - 1);
+      const int j = t < behind ? t : lo + (t - behind);
+      const uint4* kj = reinterpret_cast<const uint4*>(k + static_cast<size_t>(j) * ld);
+      const uint4* q4 = reinterpret_cast<const uint4*>(q);
+      float s = 0.f;
+#pragma unroll 2
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 a = q4[c], b = kj[c];
+        const T* x = reinterpret_cast<const T*>(&a);
+        const T* y = reinterpret_cast<const T*>(&b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(to_f(x[e]), to_f(y[e]), s);
+      }
+      s = t0 + lane < keys ? s * p.scale_log2 : -INFINITY;
+      const float top = fmaxf(m, warp_max(s)), ref = top == -INFINITY ? 0.f : top;
+      const float corr = exp2f(m - ref), e = exp2f(s - ref);
+      m = top;
+      l = l * corr + warp_sum(e);
+#pragma unroll
+      for (int i = 0; i < CL; ++i) o[i] *= corr;
+      const unsigned weighs = __ballot_sync(0xffffffffu, s != -INFINITY);  // the others not even 0 * NaN
+#pragma unroll 4
+      for (int i = 0; i < 32; ++i) {
+        const float ei = __shfl_sync(0xffffffffu, e, i);
+        const int ji = __shfl_sync(0xffffffffu, j, i);
+        if (weighs >> i & 1) {
+#pragma unroll
+          for (int c = 0; c < CL; ++c) o[c] = fmaf(ei, to_f(v[static_cast<size_t>(ji) * ld + 32 * c]), o[c]);
+        }
+      }
+      bool nan = true;
+#pragma unroll
+      for (int i = 0; i < CL; ++i) nan &= !need[i] || o[i] != o[i];
+      lost = __all_sync(0xffffffffu, nan);
+    }
+#pragma unroll
+    for (int i = 0; i < CL; ++i)
+      if (need[i]) out[32 * i] = from_f<T>(o[i] / l);
   }
-}
-
-// Whether an item of several blocks held a value that is not finite and that
-// the row does not see, in columns [c0, c1): the keys of the item's range on
-// both sides of the row's window, and those that pad the sinks.
-template <typename T, int D>
-__device__ __noinline__ bool hidden_not_finite(const WinParams& p, int start, int n, int h, int qi, int k_begin, int nw,
-                                               int s_end, int c0, int c1) {
-  const int ld = (p.heads + 2 * p.kv_heads) * D;
-  const T* v = static_cast<const T*>(p.qkv) + static_cast<size_t>(start) * ld +
-               (p.heads + p.kv_heads + h / (p.heads / p.kv_heads)) * D;
-  auto any = [&](int j, int stop) {
-    float zero = 0.f;
-    for (; j < stop; ++j)
-      for (int c = c0; c < c1; ++c) zero = fmaf(to_f(v[static_cast<size_t>(j) * ld + c]), 0.f, zero);
-    return zero != 0.f;
-  };
-  const int lo = qi - min(p.left, qi), hi = qi + min(p.right, n - 1 - qi);
-  return any(max(k_begin, min(p.sinks, lo)), lo) || any(hi + 1, k_begin + nw) ||
-         any(s_end, min(ceil16(s_end), p.rows - start));
 }
 
 // Descriptor of a K-major (or, for V, MN-major) tile of 64- or 128-byte
@@ -483,7 +582,7 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t smem_addr) {
 
 template <int D, bool H16>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    window_tc_kernel(const TcParams p, const __grid_constant__ CUtensorMap tm64,
+    window_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUtensorMap tm64,
                      const __grid_constant__ CUtensorMap tm16) {
   using C = TcCfg<D>;
   using T = typename std::conditional<H16, f16, bf16>::type;
@@ -514,11 +613,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 2 * kSlotBars + 4);
   volatile int* ends = reinterpret_cast<volatile int*>(meta + 2 * kSlotBars + 8);  // [2] a slot's number of items
   // four items a slot: the TMA warp is up to two ahead of the output warps
-  volatile TcItem* rings = reinterpret_cast<volatile TcItem*>(meta + 2 * kSlotBars + 16);
+  volatile int* broken = ends + 2;  // [2][first, last item with an output that is not finite]
+  volatile TcItem* rings = reinterpret_cast<volatile TcItem*>(meta + 2 * kSlotBars + 32);
   volatile TcItem* ring = rings + 4 * g;
-  static_assert(2 * kSlotBars + 16 + 8 * sizeof(TcItem) <= C::META_BYTES, "meta layout");
+  static_assert(2 * kSlotBars + 32 + 8 * sizeof(TcItem) <= C::META_BYTES, "meta layout");
   const WinParams& w = p.w;
-  const int entries = (p.batch + p.group - 1) / p.group;
+  const int entries = p.entries;
 
   if (warp == 1 && lane == 0) {
     prefetch_tensormap(&tm64);
@@ -566,6 +666,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     *abort_flag = 0;
     ends[0] = ends[1] = -1;
+    broken[0] = broken[2] = INT32_MAX;
+    broken[1] = broken[3] = -1;
     fence_barrier_init();
   }
   if (warp == 3) tmem_alloc(smem_u32(tslot), 512);  // all of it (one CTA per SM): the base is column 0
@@ -590,48 +692,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int hk_div = w.heads / w.kv_heads;
     for (long long f0 = static_cast<long long>(g) * gridDim.x + blockIdx.x; f0 < items && ok; f0 += 32 * stride) {
       const long long f = f0 + lane * stride;
-      int start = 0, n = 0, h = 0, q0 = 0;  // this lane's candidate
-      if (f < items) {
-        unsigned qb = static_cast<unsigned>(f) / w.heads;
-        h = static_cast<int>(f) - static_cast<int>(qb) * w.heads;
-        int lo = 0, hi = entries;  // prefix[lo] <= qb < prefix[hi]
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (prefix[mid] <= qb) lo = mid;
-          else hi = mid;
-        }
-        qb -= prefix[lo];
-        int b = lo * p.group;
-        const int stop = min(p.batch, b + p.group);
-        TcRow row(p, b);
-        while (qb >= static_cast<unsigned>(row.blocks) && ++b < stop) {
-          qb -= row.blocks;
-          row = TcRow(p, b);
-        }
-        if (qb < static_cast<unsigned>(row.blocks)) {  // always, unless the count above wrapped
-          q0 = static_cast<int>(qb) * p.kq;
-          start = row.start;
-          n = row.n;
-        }
-      }
-      unsigned todo = __ballot_sync(0xffffffffu, f < items && q0 < n);
+      TcPlace mine;  // this lane's candidate
+      if (f < items) mine = TcPlace(p, prefix, static_cast<int>(f));
+      unsigned todo = __ballot_sync(0xffffffffu, mine.n > 0);
       while (todo && ok) {
         const int src = __ffs(todo) - 1;
         todo &= todo - 1;
         TcItem it;
-        it.start = __shfl_sync(0xffffffffu, start, src);
-        it.n = __shfl_sync(0xffffffffu, n, src);
-        it.h = __shfl_sync(0xffffffffu, h, src);
-        it.q0 = __shfl_sync(0xffffffffu, q0, src);
-        const int q_last = min(it.n, it.q0 + p.kq) - 1;
-        const int k_end = q_last + min(w.right, it.n - 1 - q_last) + 1;
-        it.k_begin = it.q0 - min(w.left, it.q0);
-        // no gap between sinks and window, or a row short enough to read whole
-        if (w.sinks >= it.k_begin || (w.sinks > 0 && k_end <= C::KEYS)) it.k_begin = 0;
-        it.s_end = min(w.sinks, it.k_begin);
-        it.nw = k_end - it.k_begin;
+        it.start = __shfl_sync(0xffffffffu, mine.start, src);
+        it.n = __shfl_sync(0xffffffffu, mine.n, src);
+        it.h = __shfl_sync(0xffffffffu, mine.h, src);
+        it.q0 = __shfl_sync(0xffffffffu, mine.q0, src);
+        const TcKeys keys(w, p.kq, it.n, it.q0, C::KEYS);
+        it.k_begin = keys.k_begin;
+        it.s_end = keys.s_end;
+        it.nw = keys.nw;
+        it.nb = keys.nb;
         const int nw16 = ceil16(it.nw), nv = nw16 + ceil16(it.s_end);
-        it.nb = nv <= C::KEYS ? 1 : (nv + 127) / 128;
         const int xk = (w.heads + it.h / hk_div) * D, xv = xk + w.kv_heads * D;
         for (int j = 0; j < it.nb; ++j, ++bc) {
           int v0, v1;
@@ -825,7 +902,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // The reference is the row's score with one key of the item (see ref_col):
           // bf16 P has f32's range, so any reference within 2^100 of the row's
           // maximum gives the same relative rounding, and no maximum is needed.
-          // (A sum outside that range: window_row_exact.)
+          // (A sum outside that range: window_rows_exact.)
           mref = tmem_ld_1(trow + ref_col(nw, nw16, nv, s_end, q0 + 32 * quarter - k_begin + 16)) * w.scale_log2;
         } else if (active) {
           float mx = -INFINITY;
@@ -955,7 +1032,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int rows = min(p.kq, n - q0) - 32 * quarter;  // rows of this warp's quarter (32 and more: all)
       const uint32_t to = s * 256u + (static_cast<uint32_t>(32 * quarter) << 16) + C::O_COL;
       const float* xs = xch + ((s * 4 + 2 + (m & 1)) * 4 + quarter) * 64 + lane;
-      const float l_row = xs[0] + xs[32], inv = 1.f / l_row;
+      // (NaN: see window_rows_exact.  Of one block the sum is taken only where the
+      // reference was near the row's maximum; its outputs may even be 0 otherwise.)
+      const float l_row = xs[0] + xs[32];
+      const float inv = nb > 1 || (l_row > 0x1p-100f && l_row < INFINITY) ? 1.f / l_row : __int_as_float(0x7fffffff);
       T* out = static_cast<T*>(w.ctx) + (static_cast<size_t>(start + q0 + 32 * quarter) * w.heads + h) * D;
       float2 zero2 = make_float2(0.f, 0.f);  // sum of o * 0: NaN if any output is not finite
       constexpr int kSlots = C::SEG / 16, kShift = kSlots == 4 ? 1 : 0;  // 16-byte slots of a staged row
@@ -1008,16 +1088,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      __syncwarp();
-      // One block: a sum far from 1 has a reference far from the row's maximum (its
-      // outputs may even be 0), one that is NaN perhaps a hidden one.  Several
-      // blocks: a NaN sum has a NaN score in it, and the outputs are NaN; else a
-      // value that the row does not see may be the one that is not finite.
-      const bool sound = zero2.x + zero2.y == 0.f && l_row < INFINITY;
-      if (lane < rows && !(sound && (nb > 1 || l_row > 0x1p-100f)) && (nb == 1 || l_row == l_row)) {
-        const int qi = q0 + 32 * quarter + lane;
-        if (nb == 1 || hidden_not_finite<T, D>(w, start, n, h, qi, e.k_begin, e.nw, e.s_end, 0, D))
-          window_row_exact<T, D>(w, start, n, h, qi, 0, D);
+      if (__any_sync(0xffffffffu, lane < rows && !(zero2.x + zero2.y == 0.f)) && lane == 0) {
+        atomicMin(const_cast<int*>(broken) + 2 * s, m);
+        atomicMax(const_cast<int*>(broken) + 2 * s + 1, m);
       }
     }
   }
@@ -1029,6 +1102,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     tmem_dealloc(*tslot, 512);
   }
+  if (!*abort_flag)
+    for (int s = 0; s < 2; ++s) window_rows_exact<T, D>(p, prefix, s, make_int2(broken[2 * s], broken[2 * s + 1]));
 }
 
 // Map over qkv [rows, cols] of 16-bit elements with boxes of row_bytes (64 or
@@ -1086,6 +1161,7 @@ cudaError_t launch_tc(const WindowArgs& a, WinParams w, cudaStream_t s, std::str
   p.w = w;
   p.batch = a.batch;
   p.group = (a.batch + kPrefixRows - 1) / kPrefixRows;
+  p.entries = (a.batch + p.group - 1) / p.group;
   p.err = a.err;
   const long long most = static_cast<long long>(a.batch) * w.q_blocks * a.heads;
   const int grid = static_cast<int>(std::min<long long>(num_sms(dev), most));

@@ -686,6 +686,65 @@ def test_attention_window_infinite_value(dev, left, right, sinks, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 64), (2, 2, 32), (2, 1, 128)])
+@pytest.mark.parametrize("left,right,sinks", [(10 ** 6, 0, 0), (64, 64, 2), (300, 0, 5), (0, 10 ** 6, 0)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_attention_window_channel_that_is_not_finite(dev, bad, left, right, sinks, h, hk, d, dt):
+    """A channel of V that is not finite in some of the tokens: the queries that see one of them have it
+    in that column alone, the others (in blocks that hold such a token, too) keep every column."""
+    t, g, lens = DTYPES[dt], _gen(d + left % 97), [2600, 5, 333]
+    n = sum(lens)
+    qkv = torch.randn((n, (h + 2 * hk) * d), generator=g, device=dev).to(t)
+    clean = qkv.clone()
+    tokens = torch.tensor([900, 1500, 2599, 2602, 2605 + 200], device=dev)
+    col = (h + hk) * d + 7  # of the first key / value head
+    qkv[tokens, col] = bad
+    cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32).to(dev)
+    got = _ops().attention_window(qkv, cu, h, max(lens), left, right, sinks=sinks, kv_heads=hk)
+    _ops().sync()
+    ref = window_ref(clean, lens, h, hk, left, right, sinks)[0].to(t)
+    start = torch.repeat_interleave(cu[:-1].long(), cu.diff().long())
+    end = torch.repeat_interleave(cu[1:].long(), cu.diff().long())
+    i = torch.arange(n, device=dev)[:, None]
+    sees = ((tokens >= start[:, None]) & (tokens < end[:, None]) & (tokens <= i + right) &
+            ((tokens >= i - left) | (tokens - start[:, None] < sinks))).any(1)
+    assert sees.any() and not sees.all()
+    for head in range(h // hk):  # the query heads of that key / value head
+        c = got[:, head * d + 7]
+        assert (c[sees].isnan() if math.isnan(bad) else c[sees] == bad).all()
+        c[sees] = ref[sees, head * d + 7]
+    window_check(got, clean, lens, h, hk, left, right, sinks, t != torch.float32)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_attention_window_long_causal_row_with_an_infinite_channel(dev, dt):
+    """Every query block has hidden values that are not finite, every query tens of thousands of visible
+    keys: nothing waits for the columns that are computed again."""
+    t, n, d = DTYPES[dt], 60000, 64
+    qkv = torch.randn((n, 3 * d), generator=_gen(6), device=dev).to(t)
+    clean = qkv.clone()
+    qkv[:, 2 * d + 9] = math.inf
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    got = _ops().attention_window(qkv, cu, 1, n, n, 0)
+    _ops().sync()
+    assert (got[:, 9] == math.inf).all()
+    got[:, 9] = 0
+    assert got.isfinite().all()
+    rows = torch.tensor([0, 1, 127, 128, 5000, 31999, n - 129, n - 2, n - 1], device=dev)
+    u = torch.finfo(t).eps / 2
+    x = clean.double()
+    for r in rows.tolist():
+        s = x[:r + 1, d:2 * d] @ x[r, :d] / math.sqrt(d)
+        p = torch.softmax(s, 0)
+        top = (x[:r + 1, d:2 * d].abs() @ x[r, :d].abs()).max().item() / math.sqrt(d)
+        want, mag = p @ x[:r + 1, 2 * d:], p @ x[:r + 1, 2 * d:].abs()
+        share = 2 * ((d + 8) * 2.0 ** -24 * top + 2.0 ** -21) + (r + 1) * 2.0 ** -23 + u  # as window_check
+        err = (got[r].double() - want).abs()
+        err[9] = 0
+        assert (err <= share * mag + u * (want.abs() + share * mag)).all(), (r, err.max())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("cu", [[0, 300, 300, 900], [0, 5, -7, 20, 2 ** 31 - 1], [600, 20, -(2 ** 31), 40, 900]])
 def test_attention_window_offsets_that_do_not_fit(dev, cu, dt):
     """Rows longer than max_len are cut; offsets that go back, are negative or lie behind the
