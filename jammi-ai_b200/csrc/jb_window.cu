@@ -462,7 +462,7 @@ __device__ __forceinline__ int ref_col(int nw, int nw16, int nv, int s_end, int 
 
 // The items of a CTA's slot, [it.x, it.y], hold outputs that are not finite: a
 // masked value contributed 0 * v, the softmax reference was far from the row's
-// scores (those rows were set to NaN), or they are so.  All warps of the CTA
+// scores (those outputs were set to NaN), or they are so.  All warps of the CTA
 // take the rows in turn, behind its last item, so that nothing waits for them.
 // The columns of a row that are not finite are computed again from global
 // memory, in f32, over the visible keys only: a key per lane for 32 scores at
@@ -1088,7 +1088,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      if (__any_sync(0xffffffffu, lane < rows && !(zero2.x + zero2.y == 0.f)) && lane == 0) {
+      bool wrong = lane < rows && !(zero2.x + zero2.y == 0.f);
+      // A reference far above the row's scores and small values: outputs whose
+      // products p v fell to where f32 has few bits left, or none
+      const bool far = !H16 && nb == 1 && lane < rows && l_row < 0x1p-24f;
+      if (__any_sync(0xffffffffu, far)) {
+        __syncwarp();  // the rows' outputs are written
+        T* y = out + static_cast<size_t>(lane) * w.heads * D;
+#pragma unroll 1
+        for (int c = 0; far && c < D; ++c) {
+          if (fabsf(to_f(y[c])) * l_row < 0x1p-100f) {
+            y[c] = from_f<T>(__int_as_float(0x7fffffff));
+            wrong = true;
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, wrong) && lane == 0) {
         atomicMin(const_cast<int*>(broken) + 2 * s, m);
         atomicMax(const_cast<int*>(broken) + 2 * s + 1, m);
       }

@@ -645,6 +645,29 @@ def test_attention_window_scores_far_apart(dev, gap, at, of, left, right, dt):
     window_check(got, qkv, [n], 1, 1, left, right, 0, t != torch.float32)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("left,right", [(3, 0), (100, 0), (2, 2)])
+@pytest.mark.parametrize("gap", [20, 40, 70, 95, 110])
+@pytest.mark.parametrize("small", [-20, -40, -75, -100])
+def test_attention_window_small_values_beside_hidden_scores(dev, small, gap, left, right, dt):
+    """Keys that some of the queries do not see score ``gap`` powers of two above the others, and the
+    values are around 2^small (half of the columns; the others around 1): products of weights relative
+    to such a score and the values leave f32's range, the outputs do not."""
+    t, n, d, g = DTYPES[dt], 500, 64, _gen(gap - small)
+    qkv = torch.zeros((n, 3 * d), device=dev)
+    qkv[:, 0] = 8.0
+    qkv[:, 1:4] = torch.randn((n, 3), generator=g, device=dev)
+    qkv[:, d + 1:d + 4] = torch.randn((n, 3), generator=g, device=dev)
+    qkv[16::32, d] = gap * math.log(2)  # 8 k / sqrt(64) log2(e) = gap
+    qkv[:, 2 * d:] = torch.randn((n, d), generator=g, device=dev)
+    qkv[:, 2 * d:2 * d + 32] *= 2.0 ** small
+    qkv = qkv.to(t)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    got = _ops().attention_window(qkv, cu, 1, n, left, right)
+    _ops().sync()
+    window_check(got, qkv, [n], 1, 1, left, right, 0, t != torch.float32)
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("left,right,sinks", [(64, 64, 0), (300, 300, 0), (300, 20, 3)])
