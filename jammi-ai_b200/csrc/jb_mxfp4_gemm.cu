@@ -19,7 +19,8 @@
 //              has its own TMEM columns for the scales, so a copy never meets a
 //              product that still reads them: the stage's shared memory, and
 //              with it its TMEM columns, comes back only after the commit of
-//              its products.
+//              its products.  In the odd CTA of a pair it passes on that its
+//              epilogue has read an accumulator.
 //   warps 2..  epilogue, one warp per 32 rows x 64 columns of the tile: the
 //              accumulators go to registers at once (tcgen05.ld) and are
 //              released before any arithmetic; bias, activation and residual
@@ -79,7 +80,7 @@ struct MxCfg {
   static_assert(2 * BN + STAGES * SF_COLS <= TMEM_COLS, "TMEM columns");
   static constexpr int EPI_WARPS = 4 * (BN / kUnitCols);
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int BARS = 2 * STAGES + 4 + 1 + EPI_WARPS;
+  static constexpr int BARS = 2 * STAGES + 4 + 1 + EPI_WARPS + 2;
   static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * (kUnitBytes + kUnitCols * 4) + 8 * BARS + 16;
   static_assert(SMEM <= 232448, "shared memory");
 };
@@ -156,8 +157,22 @@ __device__ __forceinline__ uint32_t of_cta0(uint32_t addr) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
 }
+// What this thread has seen happens before what follows the wait below in
+// either CTA.
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort) {
+  if (!warp_mbar_wait(bar, parity, abort)) return false;
+  uint32_t done;  // the phase is complete: once more, with the cluster's scope
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return __all_sync(0xffffffffu, done != 0);
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -269,13 +284,15 @@ __global__ void __launch_bounds__(MxCfg<BN, CG>::THREADS, 1)
   const uint32_t scales = boxes + Cfg::EPI_WARPS * kUnitBytes;
   const uint32_t biases = scales + Cfg::STAGES * Cfg::SF_BYTES;
   const uint32_t bars = biases + Cfg::EPI_WARPS * kUnitCols * 4;
-  // CG = 2: full and tempty of the even CTA count for the pair
+  // CG = 2: full of the even CTA counts for the pair, and peer says there that
+  // the odd CTA's epilogue has read its half of an accumulator
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (Cfg::STAGES + s); };
   auto tfull_bar = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + i); };
   auto tempty_bar = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + 2 + i); };
   const uint32_t spare = bars + 8u * (2 * Cfg::STAGES + 4);
   auto res_bar = [&](int w) { return bars + 8u * (2 * Cfg::STAGES + 5 + w); };
+  auto peer_bar = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + 5 + Cfg::EPI_WARPS + i); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + (bars - base) + 8 * Cfg::BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -296,7 +313,8 @@ __global__ void __launch_bounds__(MxCfg<BN, CG>::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull_bar(i), 1);
-      mbar_init(tempty_bar(i), CG * Cfg::EPI_WARPS);
+      mbar_init(tempty_bar(i), Cfg::EPI_WARPS);
+      mbar_init(peer_bar(i), 1);
     }
     mbar_init(spare, 1);
     for (int w = 0; w < Cfg::EPI_WARPS; ++w) mbar_init(res_bar(w), 1);
@@ -368,7 +386,7 @@ __global__ void __launch_bounds__(MxCfg<BN, CG>::THREADS, 1)
       for (int b = max(0, filled - Cfg::STAGES); b < filled; ++b)
         mbar_wait(full_bar(b % Cfg::STAGES), (b / Cfg::STAGES) & 1, &no_abort);
     }
-  } else if (warp == 1) {  // ── MMA issuer (of the even CTA)
+  } else if (warp == 1) {  // ── MMA issuer (of the even CTA), or its odd CTA's relay
     constexpr uint32_t kStageDesc = (Cfg::A_BYTES + Cfg::B_BYTES) >> 4;  // descriptors count 16 bytes
     constexpr uint32_t kTileDesc = kSfTile >> 4;
     const uint64_t da0 = umma_desc_sw128(base), db0 = umma_desc_sw128(base + Cfg::A_BYTES);
@@ -376,9 +394,20 @@ __global__ void __launch_bounds__(MxCfg<BN, CG>::THREADS, 1)
     int acc = 0, st = 0;
     uint32_t acc_ph = 0, ph = 0;
     bool ok = true;
+    // The odd CTA's warp passes its epilogue's reads on: a release at the
+    // cluster's scope takes about 1000 clocks, which the epilogue warps
+    // would all wait for (20479 x 4096 x 1024 GELU 58 us, 80 with theirs).
+    for (int t = rank == 0 ? total : first; t < total && ok; t += step) {
+      ok = warp_mbar_wait(tempty_bar(acc), acc_ph, abort_flag);
+      if (ok && lane == 0) arrive_cluster(of_cta0(peer_bar(acc)));
+      __syncwarp();
+      acc ^= 1;
+      if (acc == 0) acc_ph ^= 1u;
+    }
     for (int t = rank == 0 ? first : total; t < total; t += step) {
       const uint32_t sf_shift = static_cast<uint32_t>((t % n_tiles) * BN % 128) / 32;
       if (ok) ok = warp_mbar_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag);
+      if (CG == 2 && ok) ok = warp_wait_cluster(peer_bar(acc), acc_ph ^ 1u, abort_flag);
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
 #pragma unroll 1
@@ -424,7 +453,7 @@ __global__ void __launch_bounds__(MxCfg<BN, CG>::THREADS, 1)
       acc ^= 1;
       if (acc == 0) acc_ph ^= 1u;
     }
-    if (!ok) {  // every MMA issued completes before TMEM is freed (bounded)
+    if (!ok && rank == 0) {  // every MMA issued completes before TMEM is freed (bounded)
       volatile int no_abort = 0;
       if (elect_one()) commit<CG>(spare);
       __syncwarp();
@@ -477,10 +506,7 @@ __global__ void __launch_bounds__(MxCfg<BN, CG>::THREADS, 1)
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 2) arrive_cluster(of_cta0(tempty_bar(acc)));
-        else mbar_arrive(tempty_bar(acc));
-      }
+      if (lane == 0) mbar_arrive(tempty_bar(acc));
       acc ^= 1;
       if (acc == 0) acc_ph ^= 1u;
       if (!live) continue;

@@ -382,6 +382,28 @@ def test_linear_mxfp4(dev, M, N, K, epi, out):
     linear_check(c, mx_ref(a)[0], mx_ref(w)[0], bias, res, epi, K)
 
 
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("epi", ["none", "gelu", "residual"])
+@pytest.mark.parametrize("M,N,K", [(20001, 1544, 288), (9000, 4096, 64), (40000, 392, 672)])
+def test_linear_mxfp4_accumulators_handed_back(dev, M, N, K, epi, out):
+    """Six and more tiles per CTA or pair of CTAs: each of the two accumulators is written again behind
+    the reads of both CTAs' epilogues, with one set of bits at every run."""
+    from jammi_b200 import _lib as L
+    ops, g, t = _ops(), _gen(M + N + K), DTYPES[out]
+    a = torch.randn((M, K), generator=g, device=dev)
+    w = torch.randn((N, K), generator=g, device=dev) / math.sqrt(K)
+    bias = torch.randn((N,), generator=g, device=dev)
+    res = torch.randn((M, N), generator=g, device=dev).to(t) if epi == "residual" else None
+    aq, wq = ops.quantize_mxfp4(a), ops.quantize_mxfp4(w)
+    codes = {"none": L.EPI_NONE, "gelu": L.EPI_GELU, "residual": L.EPI_RESIDUAL}
+    runs = [ops.linear_mxfp4(*aq, *wq, bias=bias, residual=res, epilogue=codes[epi], out_dtype=t) for _ in range(6)]
+    ops.sync()
+    assert all(torch.equal(r, runs[0]) for r in runs)
+    aw, ww = ops.dequantize_mxfp4(*aq, torch.float32).double(), ops.dequantize_mxfp4(*wq, torch.float32).double()
+    for lo in range(0, M, 4000):
+        linear_check(runs[0][lo:lo + 4000], aw[lo:lo + 4000], ww, bias, None if res is None else res[lo:lo + 4000], epi, K)
+
+
 @pytest.mark.parametrize("epi", ["gelu", "quick_gelu"])
 def test_linear_mxfp4_activations_over_their_range(dev, epi):
     """Weights of zero: the bias is what the activation gets.  Its error is the 1e-6 max(1, |z|) that
