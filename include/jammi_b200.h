@@ -245,7 +245,8 @@ jb_status jb_op_layernorm(const void* x, const void* residual, const float* gamm
  * replayed graphs do not meet) and can be captured; the first
  * jb_op_linear_mxfp4 or jb_op_attention_window on a device allocates that
  * device's error flag, so make it before a capture.  Rows (M, N, batch) are
- * below 2^31 - 2^20, columns (cols, K) at most 2^30. */
+ * below 2^31 - 2^20, columns (cols, K) at most 2^30.  A
+ * buffer without an alignment below is aligned to its elements. */
 /* RMS norm over the last dim with the residual's addition: s = x (+ residual)
  * in f32, y = s * rsqrt(mean(s^2) + eps) * gamma.  `sum` (NULL unless a
  * residual is given; NULL: not wanted) receives s rounded to dtype, the next
@@ -290,8 +291,8 @@ jb_status jb_op_dequantize_mxfp4(const uint8_t* q, const uint8_t* scale, void* y
 /* MXFP4 Linear: C[M,N] = epi(A[M,K] . W[N,K]^T + bias[N]) with A and W as
  * jb_op_quantize_mxfp4 stores them (tcgen05 kind::mxf4 with block scales, f32
  * accumulators).  c_dtype F32, BF16 or F16; residual has c's dtype; bias f32
- * or NULL.  K is a multiple of 32, N of 8; every buffer is 16-byte aligned.
- * C may replace the residual.  A row with a NaN scale gives NaN outputs. */
+ * or NULL.  K is a multiple of 32, N of 8; every buffer but bias is 16-byte
+ * aligned.  C may replace the residual.  A row with a NaN scale gives NaN outputs. */
 jb_status jb_op_linear_mxfp4(const uint8_t* Aq, const uint8_t* a_scale, const uint8_t* Wq,
                              const uint8_t* w_scale, const float* bias, const void* residual,
                              void* C, int c_dtype, int M, int N, int K, int epilogue,

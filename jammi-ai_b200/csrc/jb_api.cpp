@@ -559,6 +559,9 @@ namespace {
 // The kernels step through rows, and through a row's columns, in 32 bits: a last step past the end must not wrap.
 constexpr int kMaxOpRows = INT32_MAX - (1 << 20);
 constexpr int kMaxOpCols = 1 << 30;
+// Not a multiple of its element's size: the device would fault on it.
+bool misplaced(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
+size_t float_size(int dtype) { return dtype == JB_DT_F32 ? 4 : 2; }
 }  // namespace
 
 jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma, void* sum, void* y,
@@ -574,6 +577,11 @@ jb_status jb_op_rmsnorm(const void* x, const void* residual, const float* gamma,
     if (!(eps >= 0.f)) jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: eps must be >= 0");
     if (rows == 0) return;
     if (!x || !gamma) jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: null buffer");
+    for (const void* p : {x, residual, static_cast<const void*>(sum), static_cast<const void*>(y)})
+      if (misplaced(p, float_size(dtype)))
+        jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: x, residual, sum and y must be aligned to their elements");
+    if (misplaced(gamma, 4) || misplaced(scale, 4))
+      jb::fail(JB_ERR_INVALID, "jb_op_rmsnorm: gamma and scale must be 4-byte aligned");
     jb::RmsArgs a;
     a.x = x;
     a.resid = residual;
@@ -598,6 +606,8 @@ jb_status jb_op_dequantize_rows(const int8_t* q, const float* scale, void* y, in
       jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: dtype must be f32, bf16 or f16");
     if (rows == 0) return;
     if (!q || !scale || !y) jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: null buffer");
+    if (misplaced(scale, 4) || misplaced(y, float_size(dtype)))
+      jb::fail(JB_ERR_INVALID, "jb_op_dequantize_rows: scale and y must be aligned to their elements");
     jb::check_cuda(jb::launch_dequantize_rows(q, scale, y, dtype, rows, cols, as_stream(stream)),
                    "jb_op_dequantize_rows");
   });
@@ -660,6 +670,7 @@ jb_status jb_op_linear_mxfp4(const uint8_t* Aq, const uint8_t* a_scale, const ui
     if (!aligned16(Aq) || !aligned16(a_scale) || !aligned16(Wq) || !aligned16(w_scale) || !aligned16(C) ||
         !aligned16(residual))
       jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: buffers must be 16-byte aligned");
+    if (misplaced(bias, 4)) jb::fail(JB_ERR_INVALID, "jb_op_linear_mxfp4: bias must be 4-byte aligned");
     jb::MxGemmArgs g;
     g.aq = Aq;
     g.a_scale = a_scale;
@@ -743,6 +754,7 @@ jb_status jb_op_attention_window(const void* qkv, const int* cu_seqlens, void* c
     if (!qkv || !cu_seqlens || !ctx) jb::fail(JB_ERR_INVALID, "jb_op_attention_window: null buffer");
     if (!aligned16(qkv) || !aligned16(ctx))
       jb::fail(JB_ERR_INVALID, "jb_op_attention_window: qkv and ctx must be 16-byte aligned");
+    if (misplaced(cu_seqlens, 4)) jb::fail(JB_ERR_INVALID, "jb_op_attention_window: cu_seqlens must be 4-byte aligned");
     jb::WindowArgs a;
     a.qkv = qkv;
     a.cu = cu_seqlens;

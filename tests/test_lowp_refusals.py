@@ -80,3 +80,20 @@ def test_columns_that_32_bit_steps_would_pass_are_refused(cols):
         assert "cols" in rms(cols=cols, **kw)
     for dtype in (L.DT_F32, L.DT_BF16, L.DT_F16):
         assert "cols" in refused(L.lib().jb_op_dequantize_rows, P, P, P, dtype, 1, cols, None)
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_buffers_between_elements_are_refused(off):
+    """A load of half an element would fault on the device."""
+    lib = L.lib()
+    for dtype in (L.DT_F32, L.DT_BF16, L.DT_F16):
+        wide = off % (4 if dtype == L.DT_F32 else 2)
+        for kw in ([dict(x=P + off), dict(r=P + off), dict(r=P, sum=P + off), dict(y=P + off)] if wide else []):
+            assert "aligned" in rms(dtype=dtype, **kw)
+        for kw in (dict(gamma=P + off), dict(y=None, q=P, scale=P + off)):
+            assert "aligned" in rms(dtype=dtype, **kw)
+        if wide:
+            assert "aligned" in refused(lib.jb_op_dequantize_rows, P, P, P + off, dtype, 2, 8, None)
+        assert "aligned" in refused(lib.jb_op_dequantize_rows, P, P + off, P, dtype, 2, 8, None)
+    assert "bias" in refused(lib.jb_op_linear_mxfp4, P, P, P, P, P + off, None, P, L.DT_BF16, 4, 16, 64, L.EPI_NONE, None)
+    assert "cu_seqlens" in refused(lib.jb_op_attention_window, P, P + off, P, L.DT_BF16, 2, 4, 2, 64, 16, 32, 4, 4, 0, None)
