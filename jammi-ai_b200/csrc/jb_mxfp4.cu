@@ -120,9 +120,10 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
 // (32 lanes of eight elements, four lanes to a block, two shuffles for its
 // maximum), up to eight pieces in flight.  Scale bytes are gathered in shared
 // memory and written as words: [tile][row] four blocks, 16 bytes apart in the
-// tile.  Memory-bound: 20479 x 4096 bf16 37.3 us, 5.7 TB/s (a copy: 6.5), 20479 x
-// 1024 13 us from and to L2.  (One CTA per scale tile, which reads 256 bytes of
-// a row, took 47.5 us at 20479 x 4096.)
+// tile.  Memory-bound: 20479 x 4096 bf16 35.1 us, 6.0 TB/s (a copy: 6.5); 20479 x
+// 1024 13.0 us, 4.1 TB/s, whose 640 CTAs are 1.08 waves of four to an SM (64
+// registers; the four-segment form spills two of them).  (One CTA per scale tile,
+// which reads 256 bytes of a row, took 47.5 us at 20479 x 4096.)
 template <typename T, int SEGS>
 __global__ void __launch_bounds__(kMxThreads) quantize_mxfp4_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                                     uint8_t* __restrict__ scale, int rows, int cols) {
@@ -207,7 +208,8 @@ __device__ __forceinline__ float2 e2m1_pair(uint32_t byte) {
 }
 
 // y = code * 2^(byte - 127), rounded to T: the quantiser's grid and pieces.
-// Memory-bound: 20479 x 4096 to bf16 37.4 us, 5.7 TB/s.
+// Memory-bound: 20479 x 4096 to bf16 35.5 us, 6.0 TB/s; 20479 x 1024 11.5 us, 4.6
+// TB/s (1.44 waves of three CTAs to an SM).
 template <typename T, int SEGS>
 __global__ void __launch_bounds__(kMxThreads) dequantize_mxfp4_kernel(const uint8_t* __restrict__ q,
                                                                       const uint8_t* __restrict__ scale,

@@ -32,17 +32,27 @@
 // shared memory, at 128 bytes a clock: 128 x 192 by one SM would take 80
 // clocks of reading (and more than that to fill) beside 96 of arithmetic, and
 // did not get past 217 us at 8192^3.  A pair (cta_group::2) gives each SM half
-// of W: 188 us, 5.8 PFLOP/s, 89% of four times the measured bf16 rate.
+// of W: 186 us, 5.9 PFLOP/s, 90% of four times the measured bf16 rate.
 // BN = 192 is the widest tile whose two accumulators leave TMEM columns for
 // the scales (384 + 5 stages x 24).  Its odd tiles start 64 rows into a scale
 // tile of W: the scale address of the product starts two columns (2 x 32
 // rows) later.
 //
-// Measured (bf16 in and out unless said, without the quantisation of A):
-//   20479 x 4096 x 1024, GELU         58.9 us  2.9 PFLOP/s  epilogue: 84 M GELUs
-//   20479 x 1024 x 4096, residual     45.7 us  3.8 PFLOP/s  7 waves of tiles, the last one part full
-//   1777 x 1536 x 384, f16             5.0 us               launch, one tile's latency
-//   12 x 2304 x 768                    3.6 us               launch, one tile's latency
+// Measured (bf16 in and out unless said, without the quantisation of A; captured
+// calls at 1965 MHz):
+//   20479 x 4096 x 1024                49.1 us  3.5 PFLOP/s  f32 out 73.2
+//     GELU                             55.8 us  3.1 PFLOP/s  f32 out 76.3; quick GELU 61.1
+//   20479 x 1024 x 4096                39.8 us  4.3 PFLOP/s
+//     residual                         43.8 us  3.9 PFLOP/s  f32 56.5
+//   777 x 1024 x 4096                   7.0 us               one tile's latency
+//   1777 x 1536 x 384, GELU, f16        6.6 us               launch, one tile's latency
+//   12 x 2304 x 768                     3.5 us               launch, one tile's latency
+//   12 x 1024 x 4096                    6.3 us               16 CTAs, each 64 rows of W alone
+// K = 1024: no pipe is full (GELU: tensor 42%, its memory 49%, XU 43%, issue
+// 54%); each epilogue warp's chain of TMEM read, activation, box, store and
+// wait for the box is the likely bound.  K = 4096, N = 1024: 64% of tensor cycles; N in
+// tiles of 192 is 6 for 5.33, and 480 tiles are 6.5 waves in 7, together 21% of
+// them.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -225,9 +235,11 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 // GELU(x) = max(x, 0) - a h(a), a = min(|x|, 8), h(a) = erfc(a / sqrt 2) / 2.
 // log2 h is smooth and nearly quadratic: a polynomial of degree 6, fitted here
 // to log2(erfc(a / sqrt 2) / 2) on [0, 6] for the least error of a h(a), gives
-// h as one 2^x: |error of GELU| <= 2e-7, 13 instructions per pair with the two
-// exponentials (a 16-bit output keeps 2^-9 of its value).  Behind a = 6 the
-// polynomial stays far below -30 up to the clamp.  NaN stays NaN.
+// h as one 2^x, 13 instructions per pair with the two exponentials.  |error of
+// GELU| <= 2e-7 and the result's own rounding in f32: at most 3e-7 on |x| <= 8.
+// Relative to the result it is within 2^-10 down to x = -6 and passes 2^-9 at
+// -6.16 (2.5% at -7, where GELU is -9e-12); below the clamp it stays at
+// -5.7e-15.  At a = 6 the polynomial is -29.9, and falls from there.  NaN stays NaN.
 __device__ __forceinline__ float max0_nan(float x) {
   float y;
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));

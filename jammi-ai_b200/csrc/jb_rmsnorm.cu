@@ -16,15 +16,21 @@
 // same registers per thread.  Rows whose width or base address rules 16-byte
 // loads out, and rows of more than 4096 vectors, are read element by element.
 //
-// Measured, inputs and outputs out of cache, with residual and sum, bf16 (a
-// copy runs at 6.54 TB/s):
-//   36870 x 768    y 43.0 us, 5.3 TB/s    int8 38.9 us, 5.1 TB/s
-//   9001 x 4096    y 55.2 us, 5.3 TB/s    int8 49.2 us, 5.3 TB/s
-//   3000 x 20000   y 131 us, 3.7 TB/s     int8 139 us  (the scalar kernel: 213, 240)
-//   36870 x 770    y 80 us, 2.8 TB/s      int8 94 us   (single elements)
-//   12 x 768       2.1 us, int8 2.4: launch and one row's latency
+// Measured, inputs and outputs out of cache, with residual and sum, bf16 unless
+// said (captured calls; a copy runs at 6.54 TB/s):
+//   36870 x 768    y 39.3 us, 5.8 TB/s    int8 33.8 us, 5.9 TB/s
+//            f32   y 76.2 us, 5.9 TB/s    int8 58.2 us, 6.3 TB/s
+//   9001 x 4096    y 52.3 us, 5.6 TB/s    int8 44.5 us, 5.8 TB/s
+//            f32   y 91.0 us, 6.5 TB/s
+//            f16, no residual             int8 22.0 us, 5.0 TB/s
+//   3000 x 20000   y 128 us, 3.8 TB/s     int8 136 us  (the scalar kernel: 213, 240)
+//   36870 x 770    y 75 us, 3.0 TB/s      int8 87 us   (single elements)
+//   9001 x 4095    y 86 us, 3.4 TB/s      int8 102 us  (single elements)
+//   12 x 768       2.3 us, int8 2.7: launch and one row's latency
 // What is left to the copy's rate are the reductions between a row's loads
-// and its stores, which the next row's loads cover only in part.
+// and its stores, which the next row's loads cover only in part.  Rows of more
+// than 2048 vectors have no other CTA on their SM to cover them at all and, with a
+// residual, spill 96 to 120 bytes a thread; odd rows issue a load per element.
 #include <algorithm>
 #include <atomic>
 
@@ -93,10 +99,8 @@ constexpr unsigned kInfBits = 0x7f800000u;
 
 // mean(s^2) + eps as summed, unless the squares left f32's range (infinite, or
 // so small that they lost bits): then a row's sum is taken again of s * c.  The
-// test costs ordinary rows nothing up to 1024 columns (36870 x 768 bf16 41.3 us
-// with and without it), 1% at 4096 and 4 to 6% in the wider kernels, where it
-// keeps the next pass's loads behind the statistics (3000 x 20000 125 -> 130.5
-// us, int8 of 9001 x 4095 97 -> 104 us).
+// test costs ordinary rows nothing up to 1024 columns, 1% at 4096 and 4 to 6% in
+// the wider kernels, where it keeps the next pass's loads behind the statistics.
 __device__ __forceinline__ bool in_range(float var) { return var >= 0x1p-90f && var < INFINITY; }
 // c = 2^-floor(log2(max(|s| of the row, sqrt(eps)))): s * c and eps * c^2 are
 // below 4.  0: the row holds a NaN or an infinity, whose statistics stand.
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) rmsnorm_kernel(RmsArgs 
 }
 
 // Narrow rows of any width and alignment: a warp per row with single elements,
-// E of them per lane.  Up to 1024 columns (36870 x 770 bf16 with residual 80 us,
+// E of them per lane (times by calls, launch gaps included).  Up to 1024 columns (36870 x 770 bf16 with residual 80 us,
 // int8 94; f32 without residual 64, int8 74; the form below, a CTA per row, takes
 // 104, 164, 100, 150), but 256 of f32 with a residual, where the misaligned
 // lines of two wide rows do not stay in L1 from one warp access to the next
@@ -500,8 +504,10 @@ void launch_width(const RmsArgs& a, cudaStream_t s) {
 }
 
 // y = q * scale, rounded to T.  A warp per row, eight codes per lane and
-// load; other widths and alignments element by element.  Memory-bound: 36870 x
-// 768 to bf16 22.3 us out of cache (3.8 TB/s), 9001 x 4096 24.6 us (4.5 TB/s).
+// load; other widths and alignments element by element.  36870 x 768 to bf16
+// 17.3 us out of cache (4.9 TB/s), 9001 x 4096 to f16 20.3 us (5.5 TB/s).  Short of
+// the copy's rate for the eight conversions per load (XU pipe 61%) and a
+// row's loads that wait for the row before.
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(const int8_t* __restrict__ q,
                                                               const float* __restrict__ scale, T* y, int rows,

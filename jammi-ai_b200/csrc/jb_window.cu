@@ -48,10 +48,14 @@ __device__ __forceinline__ int row_tokens(const WinParams& p, int b, int start) 
 // dimensions, 16 each (interleaved by four, so that a warp's reads of a key
 // fall on different banks); each thread works on two neighbouring queries, so
 // that a key read from shared memory serves both, and a warp skips the key
-// tiles that none of its consecutive queries sees.  FMA-bound: 4 d per
-// (query, key), two dimensions to an instruction (packed f32x2); f32 tiles are
+// tiles that none of its consecutive queries sees.  Two dimensions to an
+// instruction (packed f32x2); f32 tiles are
 // copied asynchronously, one ahead.  16 rows of 512 tokens, 12 heads of 64, window
-// 64 + 64, f32: 229 us; 64 rows, 12 heads of 16, f32: 328 us.
+// 64 + 64, f32: 228 us, 13 TFLOP/s; 64 rows, 12 heads of 16: f32 324 us, bf16
+// 350 us; of 8: bf16 251 us.  No pipe is full (f32, 64: issue 44%, FMA 36%, shared
+// memory's data pipe 61%): 14 warps an SM wait in turn for shared loads and
+// shuffles, for the FMAs' results and at the two barriers of a key tile; with 16-bit rows,
+// whose tiles are not loaded ahead, at the barriers most of all (issue 29%).
 constexpr int kSimtThreads = 128;
 
 template <typename T, int D>
@@ -272,7 +276,7 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 //                 one still reads.
 // and four warps for both slots' outputs: O / sum goes out through shared
 // memory in whole row segments while the softmax warps are at the next item
-// (256 x [32,256]: 75 us with the softmax warps writing them, 69 us).
+// (256 x [32,256]: 8% less than with the softmax warps writing them).
 // The keys of an item are its window [k_begin, k_end), padded to 16, then the
 // first keys [0, s_end) that the window has left behind, padded to 16.  With
 // head_dim 32 or 64, an item of up to 256 keys is ONE block: no running maximum, no
@@ -295,21 +299,36 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 // replayed graphs share nothing.
 //
 // Measured, bf16 unless said, window 64 + 64 (out of cache):
-//   256 rows of 32 to 256 tokens, 12 heads of 64, 1 sink   67 us  3.3 TB/s
-//   8 rows of 4000 to 8192, 16 heads of 64                100 us  3.7 TB/s, f16 109 us
-//   64 x 512 tokens, 12 heads of 32                         45 us
-//   64 x 512 tokens, 6 heads of 128, 3 key heads            55 us
-//   64 x 512 tokens, 12 heads of 64, unbounded             144 us  357 TFLOP/s
-//   one row of 12 tokens                                   4.8 us from its first instruction to its last
+//   256 rows of 32 to 256 tokens, 12 heads of 64, 1 sink    61 us  3.6 TB/s, f16 76 us
+//   8 rows of 4000 to 8192, 16 heads of 64                  82 us  4.5 TB/s, f16 101 us, with 1 sink 95 us
+//   256 rows of 4 to 16 tokens, 12 heads of 64              27 us  0.6 TB/s
+//   64 x 512 tokens, 12 heads of 64                         47 us  4.3 TB/s, 3 key heads 46 us
+//     window 16 + 16: 40 us; 128 + 0: 48; 255 + 0, 4 sinks: 86; 300 + 300: 135
+//     unbounded                                            141 us  365 TFLOP/s, f16 the same, causal 91 us
+//   64 x 512 tokens, 12 heads of 32                         41 us
+//   64 x 512 tokens, 12 heads of 128                        93 us, 6 heads, 3 key heads 52 us
+//   one row of 12 tokens                                   7.1 us from launch to launch
+// (calls captured into a graph, at 1965 MHz.)
 // What bounds it: an item's chain P -> O -> next S leaves the softmax warps
-// idle for a third of its 6300 clocks; their exponentials take half of them,
-// 16 a clock (two slots' at once).  More code in any role costs more than it
-// saves (a second, unmasked copy of the exponentials: 69 -> 71 us; P V in two
-// parts, the first behind half of P: 69 -> 72 us; an unmasked copy of the
-// maximum: 67 -> 69 us): the roles' loops share small instruction caches.
-// Items dealt by equal cost in contiguous runs instead of in turn: 69 -> 83 us
+// idle for a third of its time; their exponentials take half of it, 16 a clock
+// (two slots' at once).  A row of few tokens costs that chain as a row of 128
+// does.  Several blocks: two passes over each block's scores, a meeting of the
+// two warps of a row between them, and S of block j + 1 behind P V of block j (one
+// S buffer a slot); head_dim 128 has 128-key blocks, so its 64 + 64 window, too.
+// More code in any role costs more than it saves (a second, unmasked copy of
+// the exponentials: 3% more; P V in two parts, the first behind half of P: 4%;
+// an unmasked copy of the maximum: 3%; a call in the output warps' loop and the
+// spills around it: 5%): the roles' loops share small instruction caches.  80
+// registers, the cap of 768 threads, hold every role without spills.  Items
+// dealt by equal cost in contiguous runs instead of in turn: 20% more
 // (neighbouring heads of a token are then not read at the same time).  f16
 // makes the maximum pass that bf16 saves.
+//
+// What is rounded: P to the rows' type, which P V on the tensor core asks for
+// (scores, sums and O are f32; the sum is of the unrounded weights, since
+// unpacking the rounded ones costs bf16 4% of 256 x [32,256] and 12% of the
+// unbounded window).  The outputs' relative error against 64 bits: bf16 2.3e-3, of
+// which their own rounding is 1.7e-3; f16 2.7e-4 and 2.1e-4.
 //
 // Every wait is bounded; on a timeout each role stops, copies and MMAs in
 // flight are waited for (bounded), the error flag is set and TMEM is freed.

@@ -154,7 +154,8 @@ def _rms_args(x, gamma, residual):
 def rmsnorm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual=None):
     """RMS norm of ``x`` [R, C] (+ ``residual``): ``s * rsqrt(mean(s^2) + eps) * gamma`` with
     ``s = x + residual`` in f32.  Returns y, or (y, s rounded to x's dtype) when a residual is
-    given.  x f32, bf16 or f16; gamma f32 [C]."""
+    given.  x f32, bf16 or f16; gamma f32 [C]; C up to 2^30; eps >= 0 (a row of zeros with eps 0
+    is NaN)."""
     index, (R, C) = _rms_args(x, gamma, residual)
     y = torch.empty_like(x)
     h = None if residual is None else torch.empty_like(x)
@@ -293,7 +294,8 @@ def attention_window(qkv: torch.Tensor, cu_seqlens: torch.Tensor, heads: int, ma
     """Windowed attention over packed rows: qkv [T, (heads + 2 * kv_heads) * d] (Q|K|V), cu_seqlens
     int32 [B+1] -> ctx [T, heads*d].  Query i of a row sees key j iff ``j <= i + right and
     (j >= i - left or j < sinks)``; ``kv_heads`` None means ``heads``; d 8, 16, 32, 64 or 128.
-    Rows behind ``cu_seqlens[-1]`` are left unwritten."""
+    ``max_len`` bounds the rows' lengths: of a longer row the first ``max_len`` tokens are a row.
+    What no row holds, behind ``cu_seqlens[-1]`` for instance, is left unwritten."""
     kv_heads = heads if kv_heads is None else kv_heads
     _check("qkv", qkv, None, _FLOATS)
     _check("cu_seqlens", cu_seqlens, None, (torch.int32,), qkv.get_device())

@@ -424,6 +424,25 @@ def test_linear_mxfp4_activations_over_their_range(dev, epi):
     assert ((y[fin] - want).abs() <= 1e-6 * z[fin].abs().clamp(min=1)).all()
 
 
+@pytest.mark.parametrize("out", DTYPES)
+def test_linear_mxfp4_gelu_error_where_it_is_stated(dev, out):
+    """|error| <= 3e-7 before the output's own rounding on |x| <= 8, and 2^-9 of the value down to
+    x = -6.15 (where it is 1e-9)."""
+    from jammi_b200 import _lib as L
+    z = torch.linspace(-8, 8, 64000).to(dev)
+    aq = _ops().quantize_mxfp4(torch.ones((1, 32), device=dev))
+    wq = _ops().quantize_mxfp4(torch.zeros((z.numel(), 32), device=dev))
+    c = _ops().linear_mxfp4(*aq, *wq, bias=z, epilogue=L.EPI_GELU, out_dtype=DTYPES[out])[0]
+    _ops().sync()
+    u = torch.finfo(c.dtype).eps / 2 if out != "f32" else 0  # f32's own is in the 3e-7
+    tiny = torch.finfo(c.dtype).smallest_normal * torch.finfo(c.dtype).eps
+    want = z.double() * torch.special.ndtr(z.double())
+    err = (c.double() - want).abs()
+    assert (err <= 3e-7 * (1 + u) + u * want.abs() + tiny).all(), err.max()
+    near = (z >= -6.15) & (z <= 0)
+    assert (err <= ((2.0 ** -9 * (1 + u) + u) * want.abs() + tiny))[near].all()
+
+
 def test_linear_mxfp4_residual_in_place_and_nan_rows(dev):
     from jammi_b200 import _lib as L
     ops, g = _ops(), _gen(8)
