@@ -1013,3 +1013,33 @@ def test_window_two_calls_at_once_on_two_streams(dev):
     torch.cuda.synchronize()
     ops.sync()
     assert all(torch.equal(g, want[k % 2]) for k, g in enumerate(got))
+
+
+def test_kernels_of_every_kind_at_once_on_four_streams(dev):
+    """Kernels that take an SM's tensor memory, alone and by pairs of SMs, beside each other and beside the
+    framework's own linear: each gives the bits that it gives alone."""
+    ops, g = _ops(), _gen(21)
+    lens = torch.randint(1, 400, (300,), generator=torch.Generator().manual_seed(2)).tolist()
+    cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32).to(dev)
+    T = sum(lens)
+    wide, narrow = (torch.randn((T, 3 * 4 * d), generator=g, device=dev).bfloat16() for d in (128, 32))
+    a, w = ops.quantize_mxfp4(torch.randn((20001, 288), generator=g, device=dev)), ops.quantize_mxfp4(
+        torch.randn((1544, 288), generator=g, device=dev))
+    few, deep = ops.quantize_mxfp4(torch.randn((50, 4096), generator=g, device=dev)), ops.quantize_mxfp4(
+        torch.randn((1024, 4096), generator=g, device=dev))
+    x, m = torch.randn((4000, 768), generator=g, device=dev).bfloat16(), torch.randn((768, 768), generator=g, device=dev).bfloat16()
+    calls = [[lambda: ops.attention_window(wide, cu, 4, 400, 64, 64, sinks=1), lambda: ops.linear_mxfp4(*a, *w)],
+             [lambda: ops.linear_mxfp4(*a, *w), lambda: ops.attention_window(narrow, cu, 4, 400, 300, 0)],
+             [lambda: ops.linear(x, m), lambda: ops.linear_mxfp4(*few, *deep)],
+             [lambda: ops.attention_window(narrow, cu, 4, 400, 20, 20), lambda: ops.rmsnorm(x, torch.ones(768, device=dev), EPS)]]
+    want = [[f() for f in stream] for stream in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in calls], []
+    for _ in range(12):
+        for st, fs, ws in zip(streams, calls, want):
+            with torch.cuda.stream(st):
+                got += [(f(), w) for f, w in zip(fs, ws)]
+    torch.cuda.synchronize()
+    ops.sync()
+    for have, one in got:
+        assert torch.equal(have[:T] if have.shape[0] == T else have, one)
