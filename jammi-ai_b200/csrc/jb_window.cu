@@ -285,7 +285,7 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 // pieces 0 and 1.  That covers windows of up to left + right = 128 around 128
 // queries (and 112 queries with up to 16 sinks), the case this operator is
 // for.  Longer ranges go in blocks of 128 keys with a lazily rescaled running
-// maximum (raised only by more than 2^8).
+// maximum (raised only by more than 2^8, in f16 2^4).
 //
 // A masked value contributes 0 * v, which is not 0 when v is not finite.  V
 // rows behind the item's last key are zeroed in shared memory; for the rest
@@ -338,7 +338,12 @@ constexpr int kGroupWarps = 8;    // softmax warps of a slot
 constexpr int kSlotBars = 128;    // bytes of a slot's barriers
 constexpr int kPrefixRows = 2048;
 constexpr int kRounds = (kPrefixRows + kTcThreads - 1) / kTcThreads;
-constexpr float kRescale = 8.f;   // lazy-rescaling threshold, log2 units
+// Lazy-rescaling threshold, log2 units, and how far above the reference's the
+// weights of 16-bit P are held: f16 has 2^15 above 1 and 2^-14 below, so one
+// block keeps a weight's bits down to 2^-28 of the largest, several down to 2^-25
+// (bf16 has f32's range).
+template <bool H16> constexpr float kRescale = H16 ? 4.f : 8.f;
+constexpr float kLift1 = 14.f, kLift = 11.f;
 
 template <int D>
 struct TcCfg {
@@ -945,7 +950,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mref = mb;
           } else {
             // both threads of a row decide alike; each rescales its half of O
-            const bool up = mb > mref + kRescale;  // always behind scores of -infinity only
+            const bool up = mb > mref + kRescale<H16>;  // always behind scores of -infinity only
             if (__any_sync(0xffffffffu, up)) {
               const float alpha = up ? ex2_approx(mref - mb) : 1.f;
               l *= alpha;
@@ -965,7 +970,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (active) {
           float2 l2 = make_float2(0.f, 0.f);
-          const float ref = mref == -INFINITY ? 0.f : mref;  // nothing seen so far: p stays 0
+          const float lift = !H16 ? 0.f : nb == 1 ? kLift1 : kLift;
+          const float ref = mref == -INFINITY ? 0.f : mref - lift;  // nothing seen so far: p stays 0
 #pragma unroll 1
           for (int c = 32 * half; c < v1 - v0; c += 64) {
             const uint32_t bits = visible(v0 + c);

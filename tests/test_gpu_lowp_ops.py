@@ -686,6 +686,29 @@ def test_attention_window_scores_far_apart(dev, gap, at, of, left, right, dt):
     window_check(got, qkv, [n], 1, 1, left, right, 0, t != torch.float32)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("left,right,sinks", [(64, 64, 0), (300, 20, 3), (10 ** 6, 10 ** 6, 0)])
+@pytest.mark.parametrize("gap", [10, 14, 18, 22])
+def test_attention_window_columns_of_small_weights(dev, gap, left, right, sinks, d, dt):
+    """Some keys outweigh the others by 2^gap, and half of the columns are 0 in their values: what is
+    left there are the small weights, whose bits P has to keep."""
+    t, n, g = DTYPES[dt], 700, _gen(gap + d)
+    qkv = torch.zeros((n, 3 * d), device=dev)
+    qkv[:, 0] = math.sqrt(d)
+    qkv[:, 1:4] = torch.randn((n, 3), generator=g, device=dev)
+    qkv[:, d + 1:d + 4] = torch.randn((n, 3), generator=g, device=dev)
+    heavy = torch.arange(n, device=dev) % 50 == 20
+    qkv[heavy, d] = gap * math.log(2)  # sqrt(d) k / sqrt(d) log2(e) = gap
+    qkv[:, 2 * d:] = torch.randn((n, d), generator=g, device=dev) * 500
+    qkv[heavy, 2 * d:2 * d + d // 2] = 0
+    qkv = qkv.to(t)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    got = _ops().attention_window(qkv, cu, 1, n, left, right, sinks=sinks)
+    _ops().sync()
+    window_check(got, qkv, [n], 1, 1, left, right, sinks, t != torch.float32)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("left,right", [(3, 0), (100, 0), (2, 2)])
 @pytest.mark.parametrize("gap", [20, 40, 70, 95, 110])
