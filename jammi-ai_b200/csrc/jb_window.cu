@@ -299,15 +299,15 @@ cudaError_t launch_simt(const WinParams& p, int d, int batch, int max_len, cudaS
 // replayed graphs share nothing.
 //
 // Measured, bf16 unless said, window 64 + 64 (out of cache):
-//   256 rows of 32 to 256 tokens, 12 heads of 64, 1 sink    61 us  3.6 TB/s, f16 76 us
-//   8 rows of 4000 to 8192, 16 heads of 64                  82 us  4.5 TB/s, f16 101 us, with 1 sink 95 us
+//   256 rows of 32 to 256 tokens, 12 heads of 64, 1 sink    60 us  3.7 TB/s, f16 76 us
+//   8 rows of 4000 to 8192, 16 heads of 64                  82 us  4.5 TB/s, f16 102 us, with 1 sink 95 us
 //   256 rows of 4 to 16 tokens, 12 heads of 64              27 us  0.6 TB/s
 //   64 x 512 tokens, 12 heads of 64                         47 us  4.3 TB/s, 3 key heads 46 us
 //     window 16 + 16: 40 us; 128 + 0: 48; 255 + 0, 4 sinks: 86; 300 + 300: 135
 //     unbounded                                            141 us  365 TFLOP/s, f16 the same, causal 91 us
 //   64 x 512 tokens, 12 heads of 32                         41 us
 //   64 x 512 tokens, 12 heads of 128                        93 us, 6 heads, 3 key heads 52 us
-//   one row of 12 tokens                                   7.1 us from launch to launch
+//   one row of 12 tokens                                   6.7 us from launch to launch
 // (calls captured into a graph, at 1965 MHz.)
 // What bounds it: an item's chain P -> O -> next S leaves the softmax warps
 // idle for a third of its time; their exponentials take half of it, 16 a clock
